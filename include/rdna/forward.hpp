@@ -84,6 +84,69 @@ struct QuantizeInt8Params {
     void* vChannel = nullptr; // float [B, Hkv, D]
 };
 
+/// A paged KV cache and the batch that uses it (extension; no counterpart in the
+/// reference).  K and V are [numPages, numKvHeads, pageSize, headDim] views,
+/// head_dim contiguous, strides in elements.  Sequence b's slot s is row
+/// s % pageSize of page pageTable[b][s / pageSize].
+struct PagedCacheParams {
+    void* kCache = nullptr;
+    void* vCache = nullptr;
+    int64_t kcStrideP = 0, kcStrideH = 0, kcStrideS = 0;
+    int64_t vcStrideP = 0, vcStrideH = 0, vcStrideS = 0;
+    const void* pageTable = nullptr;  // const int32*, [batch][maxPages], rows tableStride apart
+    int64_t tableStride = 0;
+    const void* cacheLens = nullptr;  // const int32*, [batch]: slots in use before the new tokens
+    uint32_t numPages = 0, pageSize = 0, maxPages = 0;
+    uint32_t batchSize = 0, numKvHeads = 0, headDim = 0;
+    int32_t dtype = 0;                // 0 = fp16, 1 = bf16
+};
+/// New tokens into the cache, keys rotated on the way.
+struct PagedAppendParams {
+    PagedCacheParams c;
+    const void* key = nullptr;        // [batch, numKvHeads, seqLen, headDim], head_dim contiguous
+    const void* value = nullptr;
+    int64_t kStrideB = 0, kStrideH = 0, kStrideS = 0;
+    int64_t vStrideB = 0, vStrideH = 0, vStrideS = 0;
+    const void* newLens = nullptr;    // const int32*, [batch], or null: seqLen
+    const void* positions = nullptr;  // const int32*, [batch][seqLen], or null: cacheLens[b] + t
+    const void* rotCos = nullptr;     // const float*, [ropeRows][headDim / 2], or null: no rotation
+    const void* rotSin = nullptr;
+    uint32_t seqLen = 0, ropeRows = 0;
+};
+/// Attention of the new tokens over the cache (they are in it already).
+struct PagedAttentionParams {
+    PagedCacheParams c;
+    const void* q = nullptr;          // [batch, numHeads, seqLen, headDim], head_dim contiguous
+    void* o = nullptr;
+    int64_t qStrideB = 0, qStrideH = 0, qStrideS = 0;
+    int64_t oStrideB = 0, oStrideH = 0, oStrideS = 0;
+    const void* newLens = nullptr;
+    const void* treeMask = nullptr;   // bytes, [batch][seqLen][seqLen], or null: a chain
+    int64_t maskStrideB = 0, maskStrideT = 0;
+    const void* positions = nullptr;
+    const void* rotCos = nullptr;
+    const void* rotSin = nullptr;
+    uint32_t numHeads = 0, seqLen = 0, ropeRows = 0;
+    float scale = 0.0f;
+    int32_t windowSize = -1;
+};
+/// Accepted drafted tokens to the front of the drafted slots.
+struct PagedAcceptParams {
+    PagedCacheParams c;
+    const void* accepted = nullptr;      // const int32*, [batch][maxAccepted]
+    const void* acceptedLens = nullptr;  // const int32*, [batch], or null: maxAccepted
+    uint32_t maxAccepted = 0;
+};
+
+/// Enqueue the paged-cache operators on `stream`. Non-blocking. 0 on success.
+int pagedAppend(const PagedAppendParams& params, void* stream);
+int pagedAccept(const PagedAcceptParams& params, void* stream);
+/// Device workspace pagedAttention() needs (any content, 256-byte aligned).
+size_t pagedAttentionWorkspaceBytes(const PagedAttentionParams& params);
+int pagedAttention(const PagedAttentionParams& params, void* workspace, size_t workspace_bytes, void* stream);
+/// Reason the most recent paged call on this thread failed, or nullptr.
+const char* lastErrorPaged();
+
 /// Enqueues the FP16 forward on `stream` (a cudaStream_t). Non-blocking. 0 on success.
 /// With RoPE it takes a stream-ordered workspace (cudaMallocAsync / cudaFreeAsync).
 int forwardF16(const ForwardParams& params, void* stream);

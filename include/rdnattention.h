@@ -289,4 +289,82 @@ RDNA_API int32_t rdna_ipc_free(void* ptr);
 RDNA_API int32_t rdna_peer_barrier(int32_t world, int32_t rank, void* const* peer_flags, void* my_flags,
                                    uint32_t epoch, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Paged KV cache (extension; no counterpart in the reference): append, attention,
+ * accept.  Element type `dtype`: 0 = fp16, 1 = bf16, for every tensor of a call.
+ *
+ * k_cache / v_cache: [num_pages, num_kv_heads, page_size, head_dim], head_dim
+ * contiguous, strides in elements (16-byte multiples) for the page / head / slot
+ * axes.  page_size: a power of two from 8 up, or any size from 64 up.  head_dim:
+ * a multiple of 32 up to 256.  page_table: int32 [batch, max_pages], rows
+ * `table_stride` entries apart; cache_lens: int32 [batch], the slots in use before
+ * the call's new tokens.  Slot s of sequence b is row s % page_size of page
+ * page_table[b][s / page_size]; max_pages * page_size must not exceed 2^30.
+ *
+ * These lie in device memory, so the kernels check them: lengths are clamped to
+ * [0, max_pages * page_size]; a page outside [0, num_pages) is not written and
+ * reads as zeros; a token whose position lies outside the rotation tables is not
+ * appended, and its attention row is zero.
+ *
+ * rot_cos / rot_sin: fp32 [rope_rows, head_dim / 2], contiguous, interleaved pairs,
+ * or both null.  positions: int32 [batch, seq_len] contiguous, or null for
+ * cache_lens[b] + t.  new_lens: int32 [batch], how many of the seq_len tokens of
+ * each sequence count, or null for all. */
+
+/* Writes token t < new_lens[b] of key / value ([batch, num_kv_heads, seq_len,
+ * head_dim], head_dim contiguous, strides in elements) to slot cache_lens[b] + t,
+ * the key turned to its position; keys are kept rotated. */
+RDNA_API int32_t rdna_paged_kv_append(
+    const void* key, const void* value, void* k_cache, void* v_cache,
+    const void* page_table, const void* cache_lens, const void* new_lens, const void* positions,
+    const void* rot_cos, const void* rot_sin,
+    int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
+    int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_s,
+    int64_t kc_stride_p, int64_t kc_stride_h, int64_t kc_stride_s,
+    int64_t vc_stride_p, int64_t vc_stride_h, int64_t vc_stride_s, int64_t table_stride,
+    uint32_t batch_size, uint32_t num_kv_heads, uint32_t seq_len, uint32_t head_dim,
+    uint32_t num_pages, uint32_t page_size, uint32_t max_pages, uint32_t rope_rows,
+    int32_t dtype, void* stream);
+
+/* Attention of seq_len new tokens per sequence, which are in the cache already
+ * (slots cache_lens[b] + t).  tree_mask null: token t sees slots 0 ..
+ * cache_lens[b] + t.  tree_mask (bytes, nonzero = sees, [batch, seq_len, seq_len]
+ * with strides mask_stride_b, mask_stride_t and 1; seq_len <= 256): token t sees
+ * the slots below cache_lens[b] and the new tokens u < new_lens[b] with
+ * mask[b][t][u].  window_size > 0: only the newest window_size of these, the new
+ * tokens (in index order: parents before children) counting first.  Query rows are
+ * turned to their positions.  Output rows t >= new_lens[b] and rows that see
+ * nothing are zero.  `workspace` (256-byte aligned, any content, for this call
+ * alone until it has run) holds rdna_attention_paged_workspace_size() bytes. */
+RDNA_API int32_t rdna_attention_forward_paged(
+    const void* q, const void* k_cache, const void* v_cache, void* output,
+    const void* page_table, const void* cache_lens, const void* new_lens,
+    const void* tree_mask, const void* positions, const void* rot_cos, const void* rot_sin,
+    int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
+    int64_t kc_stride_p, int64_t kc_stride_h, int64_t kc_stride_s,
+    int64_t vc_stride_p, int64_t vc_stride_h, int64_t vc_stride_s,
+    int64_t o_stride_b, int64_t o_stride_h, int64_t o_stride_s,
+    int64_t mask_stride_b, int64_t mask_stride_t, int64_t table_stride,
+    uint32_t batch_size, uint32_t num_heads, uint32_t num_kv_heads, uint32_t seq_len, uint32_t head_dim,
+    uint32_t num_pages, uint32_t page_size, uint32_t max_pages, uint32_t rope_rows,
+    float scale, int32_t window_size, int32_t dtype,
+    void* workspace, uint64_t workspace_bytes, void* stream);
+RDNA_API uint64_t rdna_attention_paged_workspace_size(
+    uint32_t batch_size, uint32_t num_heads, uint32_t num_kv_heads, uint32_t seq_len, uint32_t head_dim,
+    uint32_t page_size, uint32_t max_pages);
+
+/* After verification: slot cache_lens[b] + i takes the row of slot cache_lens[b] +
+ * accepted[b][i] for i < accepted_lens[b] (null: max_accepted), in every head of K
+ * and V, all rows as they were before the call.  accepted: int32 [batch,
+ * max_accepted] contiguous, max_accepted <= 256; an entry that is negative or
+ * behind the page table moves nothing. */
+RDNA_API int32_t rdna_paged_kv_accept(
+    void* k_cache, void* v_cache, const void* page_table, const void* cache_lens,
+    const void* accepted, const void* accepted_lens,
+    int64_t kc_stride_p, int64_t kc_stride_h, int64_t kc_stride_s,
+    int64_t vc_stride_p, int64_t vc_stride_h, int64_t vc_stride_s, int64_t table_stride,
+    uint32_t batch_size, uint32_t num_kv_heads, uint32_t head_dim,
+    uint32_t num_pages, uint32_t page_size, uint32_t max_pages, uint32_t max_accepted,
+    int32_t dtype, void* stream);
+
 #endif /* RDNATTENTION_H_ */

@@ -109,6 +109,15 @@ def _lib_handle():
         lib.rdna_peer_barrier.restype = i32
         lib.rdna_debug_set_kernel_events.argtypes = [vp, vp]
         lib.rdna_debug_set_kernel_events.restype = i32
+        lib.rdna_paged_kv_append.argtypes = [vp] * 10 + [i64] * 13 + [u32] * 8 + [i32, vp]
+        lib.rdna_paged_kv_append.restype = i32
+        lib.rdna_attention_forward_paged.argtypes = ([vp] * 11 + [i64] * 15 + [u32] * 9 + [f32, i32, i32]
+                                                     + [vp, ctypes.c_uint64, vp])
+        lib.rdna_attention_forward_paged.restype = i32
+        lib.rdna_attention_paged_workspace_size.argtypes = [u32] * 7
+        lib.rdna_attention_paged_workspace_size.restype = ctypes.c_uint64
+        lib.rdna_paged_kv_accept.argtypes = [vp] * 6 + [i64] * 7 + [u32] * 7 + [i32, vp]
+        lib.rdna_paged_kv_accept.restype = i32
         _lib = lib
     return _lib
 
@@ -592,6 +601,19 @@ def debug_read_status():
     return int(out[0]), int(out[1])
 
 
+_PAGED = ("paged_kv_append", "flash_attn_paged", "paged_kv_accept", "SUPPORTED_HEAD_DIMS_PAGED")
+
+
+def __getattr__(name):
+    """The paged-cache operators (paged.py), loaded with torch on first use."""
+    if name in _PAGED:
+        from . import paged
+
+        globals().update({n: getattr(paged, n) for n in _PAGED})
+        return globals()[name]
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
 __all__ = ["flash_attn", "flash_attn_int8qk", "flash_attn_int8qk_quantized", "quantize_int8_perchannel_v",
            "quantize_int8_qk_pertoken", "quantize_int8_qkv", "has_device", "RDNAttentionError", "SUPPORTED_HEAD_DIMS",
-           "SUPPORTED_HEAD_DIMS_INT8", "__version__"]
+           "SUPPORTED_HEAD_DIMS_INT8", "__version__", *_PAGED]

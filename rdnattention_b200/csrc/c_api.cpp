@@ -453,6 +453,154 @@ RDNA_API int32_t rdna_attention_forward_noalloc(
     return 0;
 }
 
+namespace {
+
+rdna::PagedCacheParams paged_cache(
+    const void* k_cache, const void* v_cache, const void* page_table, const void* cache_lens,
+    int64_t kc_stride_p, int64_t kc_stride_h, int64_t kc_stride_s,
+    int64_t vc_stride_p, int64_t vc_stride_h, int64_t vc_stride_s, int64_t table_stride,
+    uint32_t batch_size, uint32_t num_kv_heads, uint32_t head_dim,
+    uint32_t num_pages, uint32_t page_size, uint32_t max_pages, int32_t dtype) {
+    rdna::PagedCacheParams c{};
+    c.kCache = const_cast<void*>(k_cache);
+    c.vCache = const_cast<void*>(v_cache);
+    c.kcStrideP = kc_stride_p;
+    c.kcStrideH = kc_stride_h;
+    c.kcStrideS = kc_stride_s;
+    c.vcStrideP = vc_stride_p;
+    c.vcStrideH = vc_stride_h;
+    c.vcStrideS = vc_stride_s;
+    c.pageTable = page_table;
+    c.tableStride = table_stride;
+    c.cacheLens = cache_lens;
+    c.numPages = num_pages;
+    c.pageSize = page_size;
+    c.maxPages = max_pages;
+    c.batchSize = batch_size;
+    c.numKvHeads = num_kv_heads;
+    c.headDim = head_dim;
+    c.dtype = dtype;
+    return c;
+}
+
+}  // namespace
+
+RDNA_API int32_t rdna_paged_kv_append(
+    const void* key, const void* value, void* k_cache, void* v_cache,
+    const void* page_table, const void* cache_lens, const void* new_lens, const void* positions,
+    const void* rot_cos, const void* rot_sin,
+    int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
+    int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_s,
+    int64_t kc_stride_p, int64_t kc_stride_h, int64_t kc_stride_s,
+    int64_t vc_stride_p, int64_t vc_stride_h, int64_t vc_stride_s, int64_t table_stride,
+    uint32_t batch_size, uint32_t num_kv_heads, uint32_t seq_len, uint32_t head_dim,
+    uint32_t num_pages, uint32_t page_size, uint32_t max_pages, uint32_t rope_rows,
+    int32_t dtype, void* stream) {
+    rdna::PagedAppendParams p{};
+    p.c = paged_cache(k_cache, v_cache, page_table, cache_lens, kc_stride_p, kc_stride_h, kc_stride_s, vc_stride_p,
+                      vc_stride_h, vc_stride_s, table_stride, batch_size, num_kv_heads, head_dim, num_pages,
+                      page_size, max_pages, dtype);
+    p.key = key;
+    p.value = value;
+    p.kStrideB = k_stride_b;
+    p.kStrideH = k_stride_h;
+    p.kStrideS = k_stride_s;
+    p.vStrideB = v_stride_b;
+    p.vStrideH = v_stride_h;
+    p.vStrideS = v_stride_s;
+    p.newLens = new_lens;
+    p.positions = positions;
+    p.rotCos = rot_cos;
+    p.rotSin = rot_sin;
+    p.seqLen = seq_len;
+    p.ropeRows = rope_rows;
+    if (rdna::pagedAppend(p, stream) != 0) {
+        set_error("Paged cache append failed: %s", rdna::lastErrorPaged());
+        return -3;
+    }
+    return 0;
+}
+
+RDNA_API int32_t rdna_attention_forward_paged(
+    const void* q, const void* k_cache, const void* v_cache, void* output,
+    const void* page_table, const void* cache_lens, const void* new_lens,
+    const void* tree_mask, const void* positions, const void* rot_cos, const void* rot_sin,
+    int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
+    int64_t kc_stride_p, int64_t kc_stride_h, int64_t kc_stride_s,
+    int64_t vc_stride_p, int64_t vc_stride_h, int64_t vc_stride_s,
+    int64_t o_stride_b, int64_t o_stride_h, int64_t o_stride_s,
+    int64_t mask_stride_b, int64_t mask_stride_t, int64_t table_stride,
+    uint32_t batch_size, uint32_t num_heads, uint32_t num_kv_heads, uint32_t seq_len, uint32_t head_dim,
+    uint32_t num_pages, uint32_t page_size, uint32_t max_pages, uint32_t rope_rows,
+    float scale, int32_t window_size, int32_t dtype,
+    void* workspace, uint64_t workspace_bytes, void* stream) {
+    rdna::PagedAttentionParams p{};
+    p.c = paged_cache(k_cache, v_cache, page_table, cache_lens, kc_stride_p, kc_stride_h, kc_stride_s, vc_stride_p,
+                      vc_stride_h, vc_stride_s, table_stride, batch_size, num_kv_heads, head_dim, num_pages,
+                      page_size, max_pages, dtype);
+    p.q = q;
+    p.o = output;
+    p.qStrideB = q_stride_b;
+    p.qStrideH = q_stride_h;
+    p.qStrideS = q_stride_s;
+    p.oStrideB = o_stride_b;
+    p.oStrideH = o_stride_h;
+    p.oStrideS = o_stride_s;
+    p.newLens = new_lens;
+    p.treeMask = tree_mask;
+    p.maskStrideB = mask_stride_b;
+    p.maskStrideT = mask_stride_t;
+    p.positions = positions;
+    p.rotCos = rot_cos;
+    p.rotSin = rot_sin;
+    p.numHeads = num_heads;
+    p.seqLen = seq_len;
+    p.ropeRows = rope_rows;
+    p.scale = scale;
+    p.windowSize = window_size;
+    if (rdna::pagedAttention(p, workspace, workspace_bytes, stream) != 0) {
+        set_error("Attention (paged) failed: %s", rdna::lastErrorPaged());
+        return -3;
+    }
+    return 0;
+}
+
+RDNA_API uint64_t rdna_attention_paged_workspace_size(
+    uint32_t batch_size, uint32_t num_heads, uint32_t num_kv_heads, uint32_t seq_len, uint32_t head_dim,
+    uint32_t page_size, uint32_t max_pages) {
+    rdna::PagedAttentionParams p{};
+    p.c.batchSize = batch_size;
+    p.c.numKvHeads = num_kv_heads;
+    p.c.headDim = head_dim;
+    p.c.pageSize = page_size;
+    p.c.maxPages = max_pages;
+    p.numHeads = num_heads;
+    p.seqLen = seq_len;
+    return rdna::pagedAttentionWorkspaceBytes(p);
+}
+
+RDNA_API int32_t rdna_paged_kv_accept(
+    void* k_cache, void* v_cache, const void* page_table, const void* cache_lens,
+    const void* accepted, const void* accepted_lens,
+    int64_t kc_stride_p, int64_t kc_stride_h, int64_t kc_stride_s,
+    int64_t vc_stride_p, int64_t vc_stride_h, int64_t vc_stride_s, int64_t table_stride,
+    uint32_t batch_size, uint32_t num_kv_heads, uint32_t head_dim,
+    uint32_t num_pages, uint32_t page_size, uint32_t max_pages, uint32_t max_accepted,
+    int32_t dtype, void* stream) {
+    rdna::PagedAcceptParams p{};
+    p.c = paged_cache(k_cache, v_cache, page_table, cache_lens, kc_stride_p, kc_stride_h, kc_stride_s, vc_stride_p,
+                      vc_stride_h, vc_stride_s, table_stride, batch_size, num_kv_heads, head_dim, num_pages,
+                      page_size, max_pages, dtype);
+    p.accepted = accepted;
+    p.acceptedLens = accepted_lens;
+    p.maxAccepted = max_accepted;
+    if (rdna::pagedAccept(p, stream) != 0) {
+        set_error("Paged cache accept failed: %s", rdna::lastErrorPaged());
+        return -3;
+    }
+    return 0;
+}
+
 RDNA_API int32_t rdna_debug_read_status(int32_t* out2) {
     const char* why = nullptr;
     if (out2 == nullptr) {

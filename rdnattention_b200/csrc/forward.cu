@@ -18,6 +18,7 @@
 #include "rdna/forward.hpp"
 
 #include "fa_decode.cuh"
+#include "fa_paged.cuh"
 #include "fa_prefill.cuh"
 #include "peer.cuh"
 #include "rope.cuh"
@@ -858,3 +859,5 @@ int debugReadStatus(int32_t* out2, const char** why) {
 }
 
 }  // namespace rdna
+
+#include "paged_host.cuh"

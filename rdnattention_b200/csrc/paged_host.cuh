@@ -1,0 +1,316 @@
+// Host side of the paged KV-cache operators (included by forward.cu, the one
+// translation unit that holds every kernel): checks, tensor maps, launches.
+#pragma once
+
+namespace rdna {
+namespace {
+
+thread_local char g_err_paged[512] = {0};
+
+int pfail(const char* msg) { return fail(g_err_paged, msg); }
+
+bool p16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool p4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+// [n0, n1, n2, head_dim] view: strides positive multiples of 16 bytes on every axis longer than one.
+const char* check_strides(int64_t s0, int64_t s1, int64_t s2, uint64_t n0, uint64_t n1, uint64_t n2) {
+    const int64_t s[3] = {s0, s1, s2};
+    const uint64_t n[3] = {n0, n1, n2};
+    for (int i = 0; i < 3; ++i) {
+        if (n[i] <= 1) continue;
+        if (s[i] <= 0) return "strides must be positive";
+        if (s[i] % 8 != 0) return "strides must be multiples of 16 bytes";
+        // what a tensor map can hold (40 bits of bytes)
+        if (s[i] >= (int64_t(1) << 39)) return "stride too large";
+    }
+    return nullptr;
+}
+
+const char* check_cache(const PagedCacheParams& c) {
+    if (c.kCache == nullptr || c.vCache == nullptr || c.pageTable == nullptr || c.cacheLens == nullptr)
+        return "null tensor pointer";
+    if (c.dtype != paged::DT_F16 && c.dtype != paged::DT_BF16) return "dtype must be 0 (fp16) or 1 (bf16)";
+    if (c.batchSize == 0 || c.numKvHeads == 0 || c.numPages == 0 || c.maxPages == 0)
+        return "empty problem (batch_size, num_kv_heads, num_pages and max_pages must be > 0)";
+    if (c.headDim < 32 || c.headDim > 256 || c.headDim % 32 != 0)
+        return "unsupported head_dim (multiples of 32 from 32 to 256)";
+    const bool pow2 = c.pageSize >= 8 && (c.pageSize & (c.pageSize - 1)) == 0;
+    if (!pow2 && c.pageSize < 64) return "unsupported page_size (a power of two from 8 up, or any size from 64 up)";
+    if (static_cast<uint64_t>(c.maxPages) * c.pageSize > (1u << 30)) return "max_pages * page_size exceeds 2^30";
+    if (c.numPages > INT32_MAX) return "too many pages";
+    if (c.numKvHeads > 65535 || c.batchSize > (1u << 24)) return "too many heads or sequences";
+    if (!p16(c.kCache) || !p16(c.vCache)) return "cache base pointers must be 16-byte aligned";
+    if (!p4(c.pageTable) || !p4(c.cacheLens)) return "page_table and cache_lens must be 4-byte aligned";
+    if (c.batchSize > 1 && c.tableStride < 0) return "strides must be positive";
+    if (const char* e = check_strides(c.kcStrideP, c.kcStrideH, c.kcStrideS, c.numPages, c.numKvHeads, c.pageSize))
+        return e;
+    return check_strides(c.vcStrideP, c.vcStrideH, c.vcStrideS, c.numPages, c.numKvHeads, c.pageSize);
+}
+
+const char* check_rope(const void* cos, const void* sin, const void* positions, uint32_t rows) {
+    if (!p4(positions)) return "positions must be 4-byte aligned";
+    if (cos == nullptr && sin == nullptr) return nullptr;
+    if (cos == nullptr || sin == nullptr) return "pass both rot_cos and rot_sin, or neither";
+    if (!p16(cos) || !p16(sin)) return "rot_cos/rot_sin must be 16-byte aligned";
+    if (rows > INT32_MAX) return "too many rotation table rows";
+    return nullptr;
+}
+
+paged::Table make_table(const PagedCacheParams& c, const void* new_lens, uint32_t T) {
+    paged::Table t{};
+    t.pages = static_cast<const int*>(c.pageTable);
+    t.cache_lens = static_cast<const int*>(c.cacheLens);
+    t.new_lens = static_cast<const int*>(new_lens);
+    t.stride = c.tableStride;
+    t.max_pages = static_cast<int>(c.maxPages);
+    t.num_pages = static_cast<int>(c.numPages);
+    t.P = static_cast<int>(c.pageSize);
+    t.Pmask = t.P - 1;
+    t.Pshift = -1;
+    if ((t.P & t.Pmask) == 0)
+        for (t.Pshift = 0; (1 << t.Pshift) < t.P; ++t.Pshift) {
+        }
+    t.T = static_cast<int>(T);
+    return t;
+}
+
+paged::Cache cache_view(void* p, int64_t sp, int64_t sh, int64_t ss) {
+    return paged::Cache{static_cast<uint16_t*>(p), sp, sh, ss};
+}
+
+int sm_count() {
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return sms;
+}
+
+int launched() {
+    const cudaError_t ce = cudaGetLastError();
+    return ce == cudaSuccess ? 0 : fail(g_err_paged, "%s", cudaGetErrorString(ce));
+}
+
+// How a paged attention call is cut: rows per tile, key tiles per page.
+struct PagedPlan {
+    int dp;     // head_dim rounded up to the kernel's 64, 128 or 256
+    int RT, n_rt, KT, tpp, grid;
+};
+
+PagedPlan paged_plan(uint32_t H, uint32_t Hkv, uint32_t T, uint32_t D, uint32_t P) {
+    PagedPlan f{};
+    f.dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+    const int64_t rows = static_cast<int64_t>(H / Hkv) * T;
+    const int max_rt = f.dp <= 128 ? 64 : 32;
+    f.RT = rows <= 16 ? 16 : rows <= 32 ? 32 : max_rt;
+    f.n_rt = static_cast<int>((rows + f.RT - 1) / f.RT);
+    f.KT = paged::KT;
+    f.tpp = static_cast<int>(P) >= f.KT ? (static_cast<int>(P) + f.KT - 1) / f.KT : 0;
+    f.grid = sm_count();
+    return f;
+}
+
+size_t paged_ws_bytes(const PagedPlan& f, uint32_t D) {
+    return align_up(static_cast<size_t>(2) * f.grid * f.RT * (D + 2) * sizeof(float));
+}
+
+}  // namespace
+
+int pagedAppend(const PagedAppendParams& a, void* stream) {
+    if (const char* e = check_cache(a.c)) return pfail(e);
+    if (a.key == nullptr || a.value == nullptr) return pfail("null tensor pointer");
+    if (a.seqLen == 0) return 0;
+    if (a.seqLen > (1u << 30)) return pfail("sequence too long");
+    if (!p16(a.key) || !p16(a.value)) return pfail("tensor base pointers must be 16-byte aligned");
+    if (!p4(a.newLens)) return pfail("new_lens must be 4-byte aligned");
+    if (const char* e = check_strides(a.kStrideB, a.kStrideH, a.kStrideS, a.c.batchSize, a.c.numKvHeads, a.seqLen))
+        return pfail(e);
+    if (const char* e = check_strides(a.vStrideB, a.vStrideH, a.vStrideS, a.c.batchSize, a.c.numKvHeads, a.seqLen))
+        return pfail(e);
+    if (const char* e = check_rope(a.rotCos, a.rotSin, a.positions, a.ropeRows)) return pfail(e);
+    paged::AppendParams p{};
+    p.k = paged::Rows{static_cast<const uint16_t*>(a.key), a.kStrideB, a.kStrideH, a.kStrideS};
+    p.v = paged::Rows{static_cast<const uint16_t*>(a.value), a.vStrideB, a.vStrideH, a.vStrideS};
+    p.kc = cache_view(a.c.kCache, a.c.kcStrideP, a.c.kcStrideH, a.c.kcStrideS);
+    p.vc = cache_view(a.c.vCache, a.c.vcStrideP, a.c.vcStrideH, a.c.vcStrideS);
+    p.t = make_table(a.c, a.newLens, a.seqLen);
+    p.positions = static_cast<const int*>(a.positions);
+    p.cos = static_cast<const float*>(a.rotCos);
+    p.sin = static_cast<const float*>(a.rotSin);
+    p.rope_rows = static_cast<int>(a.ropeRows);
+    p.B = static_cast<int>(a.c.batchSize);
+    p.Hkv = static_cast<int>(a.c.numKvHeads);
+    p.D = static_cast<int>(a.c.headDim);
+    p.n = static_cast<int64_t>(p.B) * p.Hkv * a.seqLen * (p.D / 8);
+    if (static_cast<int64_t>(p.B) * p.Hkv > INT32_MAX || (p.n + 255) / 256 > INT32_MAX)
+        return pfail("problem too large for one launch");
+    const unsigned grid = static_cast<unsigned>((p.n + 255) / 256);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a.c.dtype == paged::DT_F16)
+        paged::append_kernel<paged::F16><<<grid, 256, 0, st>>>(p);
+    else
+        paged::append_kernel<paged::BF16><<<grid, 256, 0, st>>>(p);
+    return launched();
+}
+
+int pagedAccept(const PagedAcceptParams& a, void* stream) {
+    if (const char* e = check_cache(a.c)) return pfail(e);
+    if (a.maxAccepted == 0) return 0;
+    if (a.accepted == nullptr) return pfail("null tensor pointer");
+    if (a.maxAccepted > static_cast<uint32_t>(paged::kMaxAccept)) return pfail("more than 256 accepted tokens");
+    if (!p4(a.accepted) || !p4(a.acceptedLens)) return pfail("accepted and accepted_lens must be 4-byte aligned");
+    if (a.c.batchSize > 65535) return pfail("too many sequences for one launch");
+    paged::AcceptParams p{};
+    p.kc = cache_view(a.c.kCache, a.c.kcStrideP, a.c.kcStrideH, a.c.kcStrideS);
+    p.vc = cache_view(a.c.vCache, a.c.vcStrideP, a.c.vcStrideH, a.c.vcStrideS);
+    p.t = make_table(a.c, nullptr, 0);
+    p.accepted = static_cast<const int*>(a.accepted);
+    p.accepted_lens = static_cast<const int*>(a.acceptedLens);
+    p.A = static_cast<int>(a.maxAccepted);
+    p.B = static_cast<int>(a.c.batchSize);
+    p.Hkv = static_cast<int>(a.c.numKvHeads);
+    p.D = static_cast<int>(a.c.headDim);
+    p.n = 2 * p.Hkv * (p.D / 8);
+    // threads x rows x 16 bytes of staging: 128 threads up to 96 rows, else 32
+    const int threads = p.A <= 96 ? 128 : 32;
+    const int smem = threads * p.A * 16;
+    cudaError_t ce = cudaFuncSetAttribute(paged::accept_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 196608);
+    if (ce != cudaSuccess) return fail(g_err_paged, "%s", cudaGetErrorString(ce));
+    const dim3 grid((p.n + threads - 1) / threads, p.B);
+    paged::accept_kernel<<<grid, threads, smem, static_cast<cudaStream_t>(stream)>>>(p);
+    return launched();
+}
+
+size_t pagedAttentionWorkspaceBytes(const PagedAttentionParams& a) {
+    if (a.c.numKvHeads == 0 || a.numHeads == 0 || a.numHeads % a.c.numKvHeads != 0 || a.c.headDim == 0 ||
+        a.c.headDim > 256 || a.seqLen == 0 || a.c.pageSize == 0)
+        return 0;
+    return paged_ws_bytes(paged_plan(a.numHeads, a.c.numKvHeads, a.seqLen, a.c.headDim, a.c.pageSize), a.c.headDim);
+}
+
+int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t workspace_bytes, void* stream) {
+    const PagedCacheParams& c = a.c;
+    if (const char* e = check_cache(c)) return pfail(e);
+    if (a.q == nullptr || a.o == nullptr) return pfail("null tensor pointer");
+    if (a.numHeads == 0 || a.numHeads % c.numKvHeads != 0)
+        return pfail("numHeads must be a positive multiple of numKvHeads");
+    if (a.seqLen == 0) return 0;
+    if (a.treeMask != nullptr && a.seqLen > static_cast<uint32_t>(paged::kMaxTree))
+        return pfail("tree_mask: more than 256 tokens");
+    const int64_t rows = static_cast<int64_t>(a.numHeads / c.numKvHeads) * a.seqLen;
+    if (rows > (1 << 28)) return pfail("sequence too long");
+    if (!p16(a.q) || !p16(a.o)) return pfail("tensor base pointers must be 16-byte aligned");
+    if (!p4(a.newLens)) return pfail("new_lens must be 4-byte aligned");
+    if (const char* e = check_strides(a.qStrideB, a.qStrideH, a.qStrideS, c.batchSize, a.numHeads, a.seqLen))
+        return pfail(e);
+    if (const char* e = check_strides(a.oStrideB, a.oStrideH, a.oStrideS, c.batchSize, a.numHeads, a.seqLen))
+        return pfail(e);
+    if (a.treeMask != nullptr && (a.maskStrideB < 0 || a.maskStrideT < 0)) return pfail("strides must be positive");
+    if (const char* e = check_rope(a.rotCos, a.rotSin, a.positions, a.ropeRows)) return pfail(e);
+
+    const PagedPlan f = paged_plan(a.numHeads, c.numKvHeads, a.seqLen, c.headDim, c.pageSize);
+    const size_t need = paged_ws_bytes(f, c.headDim);
+    if (workspace == nullptr || workspace_bytes < need)
+        return pfail("workspace missing or smaller than rdna_attention_paged_workspace_size()");
+    if (reinterpret_cast<uintptr_t>(workspace) & (kWsAlign - 1)) return pfail("workspace must be 256-byte aligned");
+
+    paged::AttnParams p{};
+    p.q = static_cast<const uint16_t*>(a.q);
+    p.o = static_cast<uint16_t*>(a.o);
+    p.qsb = a.qStrideB;
+    p.qsh = a.qStrideH;
+    p.qss = a.qStrideS;
+    p.osb = a.oStrideB;
+    p.osh = a.oStrideH;
+    p.oss = a.oStrideS;
+    p.t = make_table(c, a.newLens, a.seqLen);
+    p.mask = static_cast<const uint8_t*>(a.treeMask);
+    p.msb = a.maskStrideB;
+    p.mst = a.maskStrideT;
+    p.positions = static_cast<const int*>(a.positions);
+    p.cos = static_cast<const float*>(a.rotCos);
+    p.sin = static_cast<const float*>(a.rotSin);
+    p.rope_rows = static_cast<int>(a.ropeRows);
+    p.H = static_cast<int>(a.numHeads);
+    p.Hkv = static_cast<int>(c.numKvHeads);
+    p.G = p.H / p.Hkv;
+    p.D = static_cast<int>(c.headDim);
+    p.rows = static_cast<int>(rows);
+    p.RT = f.RT;
+    p.n_rt = f.n_rt;
+    p.KT = f.KT;
+    p.tpp = f.tpp;
+    p.window = a.windowSize > 0 ? a.windowSize : 0;
+    p.scale_log2 = a.scale * 1.4426950408889634f;
+    p.ws = static_cast<float*>(workspace);
+    p.grid = f.grid;
+
+    // the list positions of one launch are 32-bit: as many sequences per launch as surely fit
+    const int64_t tiles = f.tpp == 0 ? (static_cast<int64_t>(c.maxPages) * c.pageSize + f.KT - 1) / f.KT
+                                     : static_cast<int64_t>(c.maxPages) * f.tpp;
+    const int64_t per_seq = tiles * p.n_rt * p.Hkv;
+    const int64_t join_rows = static_cast<int64_t>(p.Hkv) * p.n_rt * ((f.RT + paged::kJoinWarps - 1) / paged::kJoinWarps);
+    const int64_t fit = INT32_MAX / (per_seq > join_rows ? per_seq : join_rows);
+    if (fit == 0) return pfail("problem too large for one launch");
+    const int64_t step = fit < paged::kMaxBatch ? fit : paged::kMaxBatch;
+
+    CUtensorMap tmK, tmV;
+    const uint32_t box_rows = c.pageSize < static_cast<uint32_t>(f.KT) ? c.pageSize : f.KT;
+    const CUtensorMapDataType dt =
+        c.dtype == paged::DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const View4 vk{c.kCache, {c.headDim, c.pageSize, c.numKvHeads, c.numPages}, {c.kcStrideS, c.kcStrideH, c.kcStrideP}};
+    const View4 vv{c.vCache, {c.headDim, c.pageSize, c.numKvHeads, c.numPages}, {c.vcStrideS, c.vcStrideH, c.vcStrideP}};
+    const char* e = nullptr;
+    if ((e = make_map(&tmK, vk, dt, 2, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B)) ||
+        (e = make_map(&tmV, vv, dt, 2, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B)))
+        return pfail(e);
+
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    for (int64_t b0 = 0; b0 < c.batchSize; b0 += step) {
+        paged::AttnParams s = p;
+        s.B = static_cast<int>(c.batchSize - b0 < step ? c.batchSize - b0 : step);
+        s.q += b0 * p.qsb;
+        s.o += b0 * p.osb;
+        s.t.pages += b0 * p.t.stride;
+        s.t.cache_lens += b0;
+        if (s.t.new_lens != nullptr) s.t.new_lens += b0;
+        if (s.mask != nullptr) s.mask += b0 * p.msb;
+        if (s.positions != nullptr) s.positions += b0 * a.seqLen;
+        auto launch = [&](auto kern, int smem) {
+            cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            if (ce != cudaSuccess) return ce;
+            return launch_timed(st, [&] {
+                kern<<<f.grid, paged::THREADS, smem, st>>>(tmK, tmV, s);
+                return cudaGetLastError();
+            });
+        };
+        auto by_width = [&](auto E) {
+            using T = decltype(E);
+            switch (f.dp) {
+                case 64: return launch(paged::fa_paged_kernel<T, 64>, paged::Layout<64>::SMEM_BYTES);
+                case 128: return launch(paged::fa_paged_kernel<T, 128>, paged::Layout<128>::SMEM_BYTES);
+                default: return launch(paged::fa_paged_kernel<T, 256>, paged::Layout<256>::SMEM_BYTES);
+            }
+        };
+        cudaError_t ce = c.dtype == paged::DT_F16 ? by_width(paged::F16{}) : by_width(paged::BF16{});
+        if (ce != cudaSuccess) return fail(g_err_paged, "%s", cudaGetErrorString(ce));
+        // the join starts while the attention kernel drains and waits for it before it reads
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(static_cast<unsigned>(s.B * join_rows));
+        cfg.blockDim = dim3(32 * paged::kJoinWarps);
+        cfg.stream = st;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        ce = c.dtype == paged::DT_F16 ? cudaLaunchKernelEx(&cfg, paged::join_kernel<paged::F16>, s)
+                                      : cudaLaunchKernelEx(&cfg, paged::join_kernel<paged::BF16>, s);
+        if (ce == cudaSuccess) ce = cudaGetLastError();
+        if (ce != cudaSuccess) return fail(g_err_paged, "%s", cudaGetErrorString(ce));
+    }
+    return 0;
+}
+
+const char* lastErrorPaged() { return g_err_paged[0] ? g_err_paged : nullptr; }
+
+}  // namespace rdna
