@@ -19,7 +19,6 @@
 // joins them in list order, so results do not depend on timing.
 #pragma once
 
-#include <cuda.h>
 #include <limits.h>
 #include <math.h>
 
@@ -30,11 +29,29 @@ namespace paged {
 
 constexpr int kMaxTree = 256;          // drafted tokens under a mask
 constexpr int kMaxBatch = 1024;        // sequences per launch (the host splits larger batches)
-constexpr int kMinTiles = 4;           // tiles per CTA below which fewer CTAs take part
+constexpr int kMinTiles = 2;           // tiles per CTA below which fewer CTAs take part
+constexpr int KT = 64;                 // keys per tile
+
+// n / d for n < 2^31 by a multiplication: with l = ceil(log2 d) and m =
+// floor(2^(31 + l) / d) + 1, m d exceeds 2^(31 + l) by at most 2^l, so the error
+// n (m d - 2^(31 + l)) / d 2^(31 + l) stays below 1 / d.
+struct FastDiv {
+    uint32_t d, m, l;
+    void set(uint32_t div) {
+        d = div;
+        for (l = 0; (uint64_t(1) << l) < d; ++l) {
+        }
+        m = static_cast<uint32_t>((uint64_t(1) << (31 + l)) / d + 1);
+    }
+    __device__ __forceinline__ int div(int n) const {
+        return l == 0 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), m) >> (l - 1));
+    }
+};
 
 struct AttnParams {
     const uint16_t* q;
     uint16_t* o;
+    Cache kc, vc;
     int64_t qsb, qsh, qss, osb, osh, oss;
     Table t;
     const uint8_t* mask;  // [B][T][T] bool or null: chain
@@ -43,11 +60,13 @@ struct AttnParams {
     const float *cos, *sin;
     int rope_rows;
     int B, H, Hkv, G, D;
+    FastDiv by_G;
     int rows;    // T * G
     int RT;      // rows per tile
     int n_rt;    // row tiles
-    int KT;      // keys per tile
-    int tpp;     // tiles per page (pages of at least KT slots), else 0: KT / P pages per tile
+    int tpp;     // key tiles per page (pages of at least KT slots), else 0: KT / P pages per tile
+    FastDiv by_tpp;
+    FastDiv by_P;
     int window;  // 0: none
     float scale_log2;
     float* ws;   // partials: 2 per CTA, each O [RT][D], m [RT], l [RT]
@@ -62,16 +81,15 @@ struct Span {
 
 // Tile that holds key j.
 __device__ __forceinline__ int tile_of(const AttnParams& p, int j) {
-    if (p.tpp == 0) return j / p.KT;
-    int page, row;
-    p.t.split(j, page, row);
-    return page * p.tpp + row / p.KT;
+    if (p.tpp == 0) return j / KT;
+    const int page = p.by_P.div(j);
+    return page * p.tpp + (j - page * p.t.P) / KT;
 }
 
 __device__ __forceinline__ Span row_tile_span(const AttnParams& p, int L, int n, int rt) {
     const int cap = p.t.cap();
-    const int ta = rt * p.RT / p.G;  // tokens of the tile: [ta, tb]
-    const int tb = min((min((rt + 1) * p.RT, p.rows) - 1) / p.G, n - 1);
+    const int ta = p.by_G.div(rt * p.RT);  // tokens of the tile: [ta, tb]
+    const int tb = min(p.by_G.div(min((rt + 1) * p.RT, p.rows) - 1), n - 1);
     Span s{0, 0, 0, 0};
     if (ta >= n) return s;  // padding rows only
     s.hi = min(p.mask != nullptr ? L + n : L + tb + 1, cap);
@@ -82,47 +100,74 @@ __device__ __forceinline__ Span row_tile_span(const AttnParams& p, int L, int n,
     return s;
 }
 
-// Tiles of one KV head of sequence b over all row tiles.
-__device__ __forceinline__ int head_tiles(const AttnParams& p, int b) {
-    const int L = p.t.len(b), n = p.t.news(b);
+// The list of a launch, as each warp sees it.  Up to 32 sequences it lies in the
+// warp's registers (lane b: sequence b), so that no barrier and no second load
+// stands between the lengths and the first key tile; more of them take a prefix
+// array in shared memory.
+struct Sched {
+    int total;    // tiles of the launch
+    int L, n;     // lane b: lengths of sequence b
+    int head;     // lane b: tiles of one of its KV heads
+    int end;      // lane b: list position behind it
+    int q, r;     // the first r CTAs take q + 1 tiles, the others q
+    int ctas;     // CTAs that take part
+};
+
+__device__ __forceinline__ int head_tiles(const AttnParams& p, int L, int n) {
     int w = 0;
     for (int rt = 0; rt < p.n_rt; ++rt) w += row_tile_span(p, L, n, rt).n;
     return w;
 }
 
-// Fills pre[0 .. B] with the exclusive prefix sums of the sequences' tiles (all
-// threads of the block; ends with a barrier).
-__device__ __forceinline__ void schedule_prefix(const AttnParams& p, int* pre) {
-    for (int b = threadIdx.x; b < p.B; b += blockDim.x) pre[b + 1] = head_tiles(p, b) * p.Hkv;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        int carry = 0;
-        for (int b0 = 0; b0 < p.B; b0 += 32) {
-            const int b = b0 + threadIdx.x;
-            int v = b < p.B ? pre[b + 1] : 0;
+__device__ __forceinline__ int warp_scan(int v, int lane) {
 #pragma unroll
-            for (int d = 1; d < 32; d *= 2) {
-                const int u = __shfl_up_sync(0xffffffffu, v, d);
-                if (threadIdx.x >= d) v += u;
-            }
-            v += carry;
-            if (b < p.B) pre[b + 1] = v;
-            carry = __shfl_sync(0xffffffffu, v, 31);
-        }
-        if (threadIdx.x == 0) pre[0] = 0;
+    for (int d = 1; d < 32; d *= 2) {
+        const int u = __shfl_up_sync(0xffffffffu, v, d);
+        if (lane >= d) v += u;
     }
-    __syncthreads();
+    return v;
 }
 
-// CTAs that take part, and the first list position of CTA c.
-__device__ __forceinline__ int active_ctas(const AttnParams& p, int total) {
-    return min(p.grid, max(1, total / kMinTiles));
+// All threads of the block; `pre` [B] is used above 32 sequences only.
+__device__ __forceinline__ Sched make_sched(const AttnParams& p, int* pre) {
+    const int lane = threadIdx.x & 31;
+    Sched s{};
+    if (p.B <= 32) {
+        if (lane < p.B) {
+            s.L = p.t.len(lane);
+            s.n = p.t.news(lane);
+            s.head = head_tiles(p, s.L, s.n);
+        }
+        s.end = warp_scan(s.head * p.Hkv, lane);
+        s.total = __shfl_sync(0xffffffffu, s.end, 31);
+    } else {
+        for (int b = threadIdx.x; b < p.B; b += blockDim.x)
+            pre[b] = head_tiles(p, p.t.len(b), p.t.news(b)) * p.Hkv;
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            int carry = 0;
+            for (int b0 = 0; b0 < p.B; b0 += 32) {
+                const int b = b0 + lane;
+                const int v = warp_scan(b < p.B ? pre[b] : 0, lane) + carry;
+                if (b < p.B) pre[b] = v;
+                carry = __shfl_sync(0xffffffffu, v, 31);
+            }
+        }
+        __syncthreads();
+        s.total = pre[p.B - 1];
+    }
+    // below kMinTiles tiles for each CTA fewer of them take part
+    s.ctas = min(p.grid, max(1, s.total / kMinTiles));
+    s.q = s.total / s.ctas;
+    s.r = s.total - s.q * s.ctas;
+    return s;
 }
-__device__ __forceinline__ int cta_begin(int c, int total, int ctas) {
-    return static_cast<int>(static_cast<int64_t>(c) * total / ctas);
-}
-__device__ __forceinline__ int cta_of(int pos, int total, int ctas) {
-    return static_cast<int>(((static_cast<int64_t>(pos) + 1) * ctas - 1) / total);
+
+__device__ __forceinline__ int cta_begin(const Sched& s, int c) { return c * s.q + min(c, s.r); }
+// CTA that holds list position pos < total.
+__device__ __forceinline__ int cta_of(const Sched& s, int pos) {
+    const int wide = s.r * (s.q + 1);
+    return pos < wide ? pos / (s.q + 1) : s.r + (pos - wide) / s.q;
 }
 
 // One unit's share of a CTA: list positions [pos, pos + count) are the unit's
@@ -133,22 +178,34 @@ struct Segment {
     int first, count;
 };
 
-__device__ __forceinline__ Segment segment_at(const AttnParams& p, const int* pre, int pos, int end, int& b) {
-    while (pre[b + 1] <= pos) ++b;  // pos < total, so b stays below B
+// The segment at list position pos < total (a whole warp; b: a sequence at or
+// before it, kept from call to call).
+__device__ __forceinline__ Segment segment_at(const AttnParams& p, const Sched& sc, const int* pre, int pos, int end,
+                                              int& b) {
     Segment g;
+    int off, head;
+    if (p.B <= 32) {
+        b = __ffs(__ballot_sync(0xffffffffu, sc.end > pos)) - 1;
+        const int start = __shfl_sync(0xffffffffu, sc.end - sc.head * p.Hkv, b);
+        head = __shfl_sync(0xffffffffu, sc.head, b);
+        g.L = __shfl_sync(0xffffffffu, sc.L, b);
+        g.n = __shfl_sync(0xffffffffu, sc.n, b);
+        off = pos - start;
+    } else {
+        while (pre[b] <= pos) ++b;
+        const int start = b > 0 ? pre[b - 1] : 0;
+        head = (pre[b] - start) / p.Hkv;
+        g.L = p.t.len(b);
+        g.n = p.t.news(b);
+        off = pos - start;
+    }
     g.b = b;
-    g.L = p.t.len(b);
-    g.n = p.t.news(b);
-    const int per_head = (pre[b + 1] - pre[b]) / p.Hkv;
-    int off = pos - pre[b];
-    g.kvh = off / per_head;
-    off -= g.kvh * per_head;
-    g.rt = 0;
-    g.s = row_tile_span(p, g.L, g.n, 0);
-    while (off >= g.s.n) {
-        off -= g.s.n;
-        ++g.rt;
+    g.kvh = off / head;
+    off -= g.kvh * head;
+    for (g.rt = 0;; ++g.rt) {
         g.s = row_tile_span(p, g.L, g.n, g.rt);
+        if (off < g.s.n) break;
+        off -= g.s.n;
     }
     g.first = off;
     g.count = min(g.s.n - off, end - pos);
@@ -159,12 +216,12 @@ __device__ __forceinline__ Segment segment_at(const AttnParams& p, const int* pr
 // inside a tile; the rows behind its end are zero fill).
 __device__ __forceinline__ void tile_keys(const AttnParams& p, int tile, int& k0, int& valid) {
     if (p.tpp == 0) {
-        k0 = tile * p.KT;
-        valid = p.KT;
+        k0 = tile * KT;
+        valid = KT;
     } else {
-        const int page = tile / p.tpp, off = (tile - page * p.tpp) * p.KT;
+        const int page = p.by_tpp.div(tile), off = (tile - page * p.tpp) * KT;
         k0 = page * p.t.P + off;
-        valid = min(p.KT, p.t.P - off);
+        valid = min(KT, p.t.P - off);
     }
 }
 
@@ -179,8 +236,8 @@ __device__ __forceinline__ float* partial_slot(const AttnParams& p, int slot) {
 __device__ __forceinline__ void build_mask(const AttnParams& p, const Segment& g, uint32_t* words, int* ctx_lo,
                                            int tid, int nthreads) {
     const int nw = (p.t.T + 31) / 32;
-    const int ta = g.rt * p.RT / p.G;
-    const int nt = min((min((g.rt + 1) * p.RT, p.rows) - 1) / p.G, g.n - 1) - ta + 1;
+    const int ta = p.by_G.div(g.rt * p.RT);
+    const int nt = min(p.by_G.div(min((g.rt + 1) * p.RT, p.rows) - 1), g.n - 1) - ta + 1;
     const int lane = tid & 31;
     for (int i = tid / 32; i < nt; i += nthreads / 32) {
         const uint8_t* row = p.mask + g.b * p.msb + (ta + i) * p.mst;
@@ -215,101 +272,132 @@ __device__ __forceinline__ void build_mask(const AttnParams& p, const Segment& g
 // One warp per row of a split unit: O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i
 // over the CTAs that hold a part, in list order.  Units with no visible key get
 // their zeros here; whole units were written by the attention kernel.
-constexpr int kJoinWarps = 8;
+constexpr int kJoinWarps = 4;
 
 template <class E>
 __global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ AttnParams p) {
-    __shared__ int pre[kMaxBatch + 1];
-    grid_dependency_wait();
-    schedule_prefix(p, pre);
-    const int total = pre[p.B];
-    const int ctas = active_ctas(p, total);
+    __shared__ int pre[kMaxBatch];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // the lengths may be read before the attention kernel has ended: it started
+    // only after what wrote them
+    const Sched sc = make_sched(p, pre);
     const int groups = (p.RT + kJoinWarps - 1) / kJoinWarps;
     const int unit = blockIdx.x / groups;  // (b, kvh, rt)
     const int rt = unit % p.n_rt, kvh = unit / p.n_rt % p.Hkv, b = unit / p.n_rt / p.Hkv;
     const int lr = blockIdx.x % groups * kJoinWarps + threadIdx.x / 32;  // row of the tile
     const int r = rt * p.RT + lr;
-    if (lr >= p.RT || r >= p.rows) return;
+    const int lane = threadIdx.x & 31;
     const int L = p.t.len(b), n = p.t.news(b);
-    int pos = pre[b], per_head = 0, before = 0, tiles = 0;
+    int head = 0, before = 0, tiles = 0;
     for (int i = 0; i < p.n_rt; ++i) {
         const int w = row_tile_span(p, L, n, i).n;
         if (i < rt) before += w;
         if (i == rt) tiles = w;
-        per_head += w;
+        head += w;
     }
-    pos += kvh * per_head + before;
-    const int t = r / p.G, h = kvh * p.G + r % p.G;
+    const int end = p.B <= 32 ? __shfl_sync(0xffffffffu, sc.end, b & 31) : pre[b];
+    const int pos = end - head * p.Hkv + kvh * head + before;
+    const int c0 = tiles > 0 ? cta_of(sc, pos) : 0, c1 = tiles > 0 ? cta_of(sc, pos + tiles - 1) : 0;
+    grid_dependency_wait();
+    if (lr >= p.RT || r >= p.rows || (tiles > 0 && c0 == c1)) return;
+    const int t = p.by_G.div(r), h = kvh * p.G + r - t * p.G;
     uint16_t* out = p.o + b * p.osb + h * p.osh + t * p.oss;
-    const int lane = threadIdx.x & 31;
     if (tiles == 0) {
         for (int d = lane * 4; d < p.D; d += 128) *reinterpret_cast<uint2*>(out + d) = uint2{0u, 0u};
         return;
     }
-    const int c0 = cta_of(pos, total, ctas), c1 = cta_of(pos + tiles - 1, total, ctas);
-    if (c0 == c1) return;
-    auto part = [&](int c) { return partial_slot(p, 2 * c + (pos <= cta_begin(c, total, ctas) ? 0 : 1)); };
-    float M = -INFINITY;
-    for (int c = c0; c <= c1; ++c) M = fmaxf(M, part(c)[p.RT * p.D + lr]);
-    float l = 0.f;
+    // the unit starts in CTA c0 (its slot 0 if the CTA starts with it); every later
+    // part is the first of its CTA
+    const int slot0 = 2 * c0 + (pos == cta_begin(sc, c0) ? 0 : 1);
+    const int parts = c1 - c0 + 1;
+    auto part = [&](int i) { return partial_slot(p, i == 0 ? slot0 : 2 * (c0 + i)); };
+    float M = -INFINITY, l = 0.f;
     float4 o[2] = {};
-    for (int c = c0; c <= c1; ++c) {
-        const float* w = part(c);
-        const float m = w[p.RT * p.D + lr];
-        const float f = m == -INFINITY ? 0.f : ex2(m - M);
-        l += f * w[p.RT * p.D + p.RT + lr];
+    for (int i0 = 0; i0 < parts; i0 += 32) {
+        // lane i: the weight of part i0 + i
+        float m = -INFINITY, li = 0.f;
+        if (i0 + lane < parts) {
+            const float* w = part(i0 + lane) + p.RT * p.D + lr;
+            m = w[0];
+            li = w[p.RT];
+        }
+        float mx = fmaxf(M, m);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int d = lane * 4 + 128 * i;
-            if (d < p.D) {
-                const float4 x = *reinterpret_cast<const float4*>(w + lr * p.D + d);
-                o[i].x += f * x.x;
-                o[i].y += f * x.y;
-                o[i].z += f * x.z;
-                o[i].w += f * x.w;
+        for (int d = 16; d > 0; d /= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+        const float f = m == -INFINITY ? 0.f : ex2(m - mx);
+        const float g = M == -INFINITY ? 0.f : ex2(M - mx);
+        M = mx;
+        l = l * g + li * f;  // per lane, summed at the end
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            o[k].x *= g;
+            o[k].y *= g;
+            o[k].z *= g;
+            o[k].w *= g;
+        }
+        const int here = min(32, parts - i0);
+#pragma unroll 4
+        for (int i = 0; i < here; ++i) {
+            const float fi = __shfl_sync(0xffffffffu, f, i);
+            const float* w = part(i0 + i) + lr * p.D;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int d = lane * 4 + 128 * k;
+                if (d < p.D) {
+                    const float4 x = *reinterpret_cast<const float4*>(w + d);
+                    o[k].x += fi * x.x;
+                    o[k].y += fi * x.y;
+                    o[k].z += fi * x.z;
+                    o[k].w += fi * x.w;
+                }
             }
         }
     }
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int d = lane * 4 + 128 * i;
+    for (int k = 0; k < 2; ++k) {
+        const int d = lane * 4 + 128 * k;
         if (d < p.D)
             *reinterpret_cast<uint2*>(out + d) =
-                uint2{E::pack(o[i].x * inv, o[i].y * inv), E::pack(o[i].z * inv, o[i].w * inv)};
+                uint2{E::pack(o[k].x * inv, o[k].y * inv), E::pack(o[k].z * inv, o[k].w * inv)};
     }
 }
 
 // -------------------------------------------------------- the few-rows kernel
-// Up to 64 rows per tile as row groups of 16, each the M = 16 of m16n8k16.
-//   warp 4       TMA producer: 32-key tiles of K and V through an NST-stage ring
-//   warps 0..3   consumers, tile i -> warps of class i % (4 / NRG), one per row
-//                group: S = Q K^T and O += P V on mma.sync with the online
-//                softmax in registers
-// The bound is HBM as long as the rows are few: per 32-key tile of head_dim 128
-// a CTA moves 16 KB (about 670 cycles of its share of the bandwidth) and needs
-// NRG * 128 MMAs on four schedulers.
-constexpr int KT = 32;
-constexpr int NCW = 4;
-constexpr int THREADS = 32 * (NCW + 1);
-
+// Row groups of 16 (the M = 16 of m16n8k16), NRG of them per tile.
+//   warps NCW..     producers: 64-key tiles of K and V through an NST-stage ring
+//   warps 0..NCW-1  consumers: the 32-key halves of the tiles go round the NCW /
+//                   NRG warps of each row group: S = Q K^T and O += P V on mma.sync
+//                   with the online softmax in registers
+// Q is kept as the sum of two values of the cache's type, hi + lo (the rotated query
+// in 32 bits splits into them but for 2^-22 / 2^-16 of it in fp16 / bf16), and both
+// are multiplied with K: the bound is HBM, so the extra MMAs are free, and the
+// scores are as exact as an fp32 product.
 template <int DP>
 struct Layout {
+    static constexpr int NCW = DP <= 128 ? 8 : 4;
+    static constexpr int NPW = 4;
+    static constexpr int THREADS = 32 * (NCW + NPW);
     static constexpr int NBOX = DP / 64;  // 64-element boxes (128 B, SWIZZLE_128B)
     static constexpr int BOX_BYTES = KT * 128;
     static constexpr int TILE = NBOX * BOX_BYTES;
     static constexpr int STAGE = 2 * TILE;
-    static constexpr int NST = DP <= 128 ? 8 : 4;
-    static_assert(NST % NCW == 0, "each ring slot has one class of consumer warps");
-    static constexpr int MAX_RG = DP <= 128 ? 4 : 2;
-    static constexpr int RT = 16 * MAX_RG;
+    static constexpr int NST = 512 / DP;  // 128 KB in flight
+    // a slot's halves always go to the same warps, so no waiter is more than one phase behind
+    static_assert(2 * NST % NCW == 0, "each ring slot has its own consumer warps");
+    static constexpr int MAX_RT = DP <= 128 ? 16 : 32;
     static constexpr int PSTR = DP + 4;  // floats per partial row: O, m, l, padding
     static constexpr int OFF_RING = 1024;
-    static constexpr int OFF_Q = OFF_RING + NST * STAGE;              // [RT][DP], swizzled like a K tile
-    static constexpr int OFF_PART = OFF_Q + NBOX * RT * 128;          // [NCW][16][PSTR] fp32
-    static constexpr int OFF_MASK = OFF_PART + NCW * 16 * PSTR * 4;   // [RT][kMaxTree / 32], then [RT]
-    static constexpr int OFF_PRE = OFF_MASK + RT * (kMaxTree / 32) * 4 + RT * 4;
-    static constexpr int SMEM_BYTES = OFF_PRE + (kMaxBatch + 1) * 4 + 1024;  // + alignment slack
+    static constexpr int OFF_Q = OFF_RING + NST * STAGE;  // hi, lo: [RT][DP], swizzled like a K tile
+    static constexpr int Q_BYTES = NBOX * MAX_RT * 128;
+    static constexpr bool ALIAS = DP > 128;               // the partials take Q's place
+    static constexpr int OFF_PART = ALIAS ? OFF_Q : OFF_Q + 2 * Q_BYTES;  // [NCW][16][PSTR] fp32
+    static constexpr int OFF_MASK = OFF_PART + NCW * 16 * PSTR * 4;       // [RT][kMaxTree / 32], then [RT]
+    static constexpr int OFF_PRE = OFF_MASK + MAX_RT * (kMaxTree / 32) * 4 + MAX_RT * 4;
+    static constexpr int SMEM_BYTES = OFF_PRE + kMaxBatch * 4 + 1024;  // + alignment slack
+    static_assert(!ALIAS || NCW * 16 * PSTR * 4 >= 2 * Q_BYTES, "Q fits below the partials");
     static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
 };
 
@@ -350,28 +438,34 @@ __device__ __forceinline__ void mma16816<BF16>(float* c, const uint32_t* a, uint
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Loads (and turns) one 16-byte chunk of row r of a row tile; zeros for rows
-// that are padding or whose position lies outside the tables.
+// Loads 16 bytes of row r of a row tile and turns them; hi + lo (see above).
+// Zeros for rows that are padding or whose position lies outside the tables.
 template <class E>
-__device__ __forceinline__ uint4 load_q_chunk(const AttnParams& p, const Segment& g, int r, int ch) {
-    const int t = r / p.G;
-    if (r >= p.rows || t >= g.n || ch * 8 >= p.D) return uint4{0u, 0u, 0u, 0u};
-    uint4 x = *reinterpret_cast<const uint4*>(p.q + g.b * p.qsb + (g.kvh * p.G + r % p.G) * p.qsh + t * p.qss + ch * 8);
+__device__ __forceinline__ void load_q_chunk(const AttnParams& p, const Segment& g, int r, int ch, uint4& hi, uint4& lo) {
+    const int t = p.by_G.div(r);
+    hi = lo = uint4{0u, 0u, 0u, 0u};
+    if (r >= p.rows || t >= g.n || ch * 8 >= p.D) return;
+    int pos = 0;
     if (p.cos != nullptr) {
-        const int pos = p.positions != nullptr ? p.positions[static_cast<int64_t>(g.b) * p.t.T + t] : g.L + t;
-        if (static_cast<unsigned>(pos) >= static_cast<unsigned>(p.rope_rows)) return uint4{0u, 0u, 0u, 0u};
-        const int64_t at = static_cast<int64_t>(pos) * (p.D / 2) + ch * 4;
-        x = rotate4<E>(x, __ldg(reinterpret_cast<const float4*>(p.cos + at)),
-                       __ldg(reinterpret_cast<const float4*>(p.sin + at)));
+        pos = p.positions != nullptr ? p.positions[static_cast<int64_t>(g.b) * p.t.T + t] : g.L + t;
+        if (static_cast<unsigned>(pos) >= static_cast<unsigned>(p.rope_rows)) return;
     }
-    return x;
+    hi = *reinterpret_cast<const uint4*>(p.q + g.b * p.qsb + (g.kvh * p.G + r - t * p.G) * p.qsh + t * p.qss + ch * 8);
+    if (p.cos == nullptr) return;
+    const int64_t at = static_cast<int64_t>(pos) * (p.D / 2) + ch * 4;
+    const float4 c = __ldg(reinterpret_cast<const float4*>(p.cos + at));
+    const float4 s = __ldg(reinterpret_cast<const float4*>(p.sin + at));
+    turn_split<E>(hi.x, lo.x, c.x, s.x);
+    turn_split<E>(hi.y, lo.y, c.y, s.y);
+    turn_split<E>(hi.z, lo.z, c.z, s.z);
+    turn_split<E>(hi.w, lo.w, c.w, s.w);
 }
 
 // Keys row r sees: [lo, hi), and with a mask the drafted slots from L on by bit.
 // A row that is padding, or whose position lies outside the tables, sees none.
-__device__ __forceinline__ void row_limits(const AttnParams& p, const Segment& g, int r, const int* ctx_lo, int& lo,
-                                           int& hi) {
-    const int t = r / p.G;
+__device__ __forceinline__ void row_limits(const AttnParams& p, const Segment& g, int r, int ta, const int* ctx_lo,
+                                           int& lo, int& hi) {
+    const int t = p.by_G.div(r);
     bool ok = r < p.rows && t < g.n;
     if (ok && p.cos != nullptr) {
         const int pos = p.positions != nullptr ? p.positions[static_cast<int64_t>(g.b) * p.t.T + t] : g.L + t;
@@ -381,7 +475,7 @@ __device__ __forceinline__ void row_limits(const AttnParams& p, const Segment& g
         lo = 1;
         hi = 0;
     } else if (p.mask != nullptr) {
-        lo = ctx_lo[t - g.rt * p.RT / p.G];
+        lo = ctx_lo[t - ta];
         hi = g.s.hi;
     } else {
         lo = p.window > 0 ? max(0, g.L + t + 1 - p.window) : 0;
@@ -389,11 +483,112 @@ __device__ __forceinline__ void row_limits(const AttnParams& p, const Segment& g
     }
 }
 
+// 16 bytes to shared memory.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint64_t pol) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(pol)
+                 : "memory");
+}
+// The same, or 16 zero bytes (src is then not read).
+__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+// Arrives on `bar` (once per thread) when the thread's copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// The producers' part of a segment (NPW warps, ptid = thread among them): its tiles
+// into the ring by 16-byte asynchronous copies, thread -> one chunk column and every
+// (32 NPW / chunks)-th row.  Rows that are not keys of the unit (behind a page's end,
+// outside what its rows see, on a page outside the cache) become zeros, so that
+// whatever lies there cannot reach the products.  Copies by TMA boxes were bound by
+// the engine's rate for pages below 64 slots: about 180 cycles a box, 16 boxes per
+// tile at 16 slots (ragged decode batch of 552 MB: 173 us).  i: running tile number.
+// False when a wait expired.
+template <class L>
+__device__ __forceinline__ bool produce(const AttnParams& p, const Segment& g, int i, uint32_t bars, uint32_t ring,
+                                        const Abort& ab, int ptid) {
+    constexpr int NCH = L::NBOX * 8;            // 16-byte chunks per row
+    constexpr int RSTEP = 32 * L::NPW / NCH;    // rows between a thread's copies
+    const uint64_t pol = policy_evict_first();
+    const int lane = ptid & 31, ch = ptid % NCH, r0 = ptid / NCH;
+    const bool col = ch * 8 < p.D;              // the columns behind head_dim stay zero
+    const int* pages = p.t.pages + g.b * p.t.stride;
+    const uint16_t* kbase = p.kc.p + g.kvh * p.kc.sh + ch * 8;
+    const uint16_t* vbase = p.vc.p + g.kvh * p.vc.sh + ch * 8;
+    const uint32_t dst0 = chunk_off(KT, r0, ch);  // (8 rows further the swizzle is the same)
+    const int shift = p.tpp == 0 ? p.t.Pshift : 31;           // row of the tile -> page of the tile
+    const int mask = p.tpp == 0 ? p.t.Pmask : KT - 1;          // and row within it
+    const int ppt = p.tpp == 0 ? KT >> p.t.Pshift : 1;         // pages per tile
+    const int tile0 = g.s.t0 + g.first;
+    int lp = p.tpp == 0 ? tile0 * ppt : p.by_tpp.div(tile0);   // logical page, first row in it
+    int sub = p.tpp == 0 ? 0 : (tile0 - lp * p.tpp) * KT;
+    int win = -1, ids = -1;  // 32 consecutive page table entries, one per lane
+    uint32_t bad = 0;        // of these, the ones outside the cache
+    for (int k = 0; k < g.count; ++k, ++i) {
+        if (lp / 32 != win) {
+            win = lp / 32;
+            const int e = win * 32 + lane;
+            ids = e < p.t.max_pages ? __ldg(pages + e) : -1;
+            bad = __ballot_sync(0xffffffffu, static_cast<unsigned>(ids) >= static_cast<unsigned>(p.t.num_pages));
+        }
+        const int k0 = lp * p.t.P + sub;  // the tile's rows are the keys k0 ..
+        const int lo = g.s.lo - k0, hi = min(g.s.hi - k0, p.tpp == 0 ? KT : min(KT, p.t.P - sub));
+        const uint32_t here = (bad >> (lp & 31)) & ((1u << ppt) - 1u);
+        const int s = i % L::NST;
+        bool ok = mbar_wait(bars + 8u * (L::NST + s), (i / L::NST & 1) ^ 1, ab, 0x601);
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        const uint32_t dst = ring + s * L::STAGE;
+        const bool inner = lo <= 0 && hi == KT && here == 0;
+        if (inner && p.tpp != 0) {
+            // a tile inside one page
+            const int page = __shfl_sync(0xffffffffu, ids, lp & 31);
+            const uint16_t* ks = kbase + page * p.kc.sp + (sub + r0) * p.kc.ss;
+            const uint16_t* vs = vbase + page * p.vc.sp + (sub + r0) * p.vc.ss;
+            if (col) {
+#pragma unroll
+                for (int r = r0, j = 0; j < KT / RSTEP; r += RSTEP, ++j) {
+                    const uint32_t d = dst + (RSTEP % 8 == 0 ? dst0 + j * RSTEP * 128 : chunk_off(KT, r, ch));
+                    cp_async16(d, ks + j * RSTEP * p.kc.ss, pol);
+                    cp_async16(d + L::TILE, vs + j * RSTEP * p.vc.ss, pol);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int r = r0, j = 0; j < KT / RSTEP; r += RSTEP, ++j) {
+                const int page = __shfl_sync(0xffffffffu, ids, (lp + (r >> shift)) & 31);
+                const uint32_t d = dst + (RSTEP % 8 == 0 ? dst0 + j * RSTEP * 128 : chunk_off(KT, r, ch));
+                const int row = sub + (r & mask);
+                const uint16_t* ks = kbase + page * p.kc.sp + row * p.kc.ss;
+                const uint16_t* vs = vbase + page * p.vc.sp + row * p.vc.ss;
+                if (!col) continue;
+                if (inner) {
+                    cp_async16(d, ks, pol);
+                    cp_async16(d + L::TILE, vs, pol);
+                } else {
+                    const bool real = r >= lo && r < hi && !(here >> (r >> shift) & 1u);
+                    cp_async16_or_zero(d, real ? ks : kbase, real);
+                    cp_async16_or_zero(d + L::TILE, real ? vs : vbase, real);
+                }
+            }
+        }
+        cp_async_arrive(bars + 8u * s);
+        if (p.tpp == 0) {
+            lp += ppt;
+        } else if ((sub += KT) >= p.t.P) {
+            sub = 0;
+            ++lp;
+        }
+    }
+    return true;
+}
+
 template <class E, int DP>
-__global__ void __launch_bounds__(THREADS, 1) fa_paged_kernel(const __grid_constant__ CUtensorMap tmK,
-                                                              const __grid_constant__ CUtensorMap tmV,
-                                                              const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
+    const __grid_constant__ AttnParams p) {
     using L = Layout<DP>;
+    constexpr int NCW = L::NCW;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -409,102 +604,59 @@ __global__ void __launch_bounds__(THREADS, 1) fa_paged_kernel(const __grid_const
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int s = 0; s < L::NST; ++s) {
-            mbar_init(full_bar(s), 1);
-            mbar_init(empty_bar(s), NRG);
+            mbar_init(full_bar(s), 32 * L::NPW);
+            mbar_init(empty_bar(s), NRG * min(2, NTG));
         }
         fence_barrier_init();
     }
+    // columns behind head_dim are never copied: zero for good
+    for (int idx = threadIdx.x; idx < 2 * L::NST * KT * (DP / 8); idx += L::THREADS)
+        if (idx % (DP / 8) * 8 >= p.D)
+            *reinterpret_cast<uint4*>(ring + idx / (DP / 8) / KT * L::TILE +
+                                      chunk_off(KT, idx / (DP / 8) % KT, idx % (DP / 8))) = uint4{0u, 0u, 0u, 0u};
+    __syncthreads();
+    grid_dependency_wait();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    schedule_prefix(p, pre);  // its barriers also publish the mbarriers
-    const int total = pre[p.B];
-    const int ctas = active_ctas(p, total);
-    if (total == 0 || static_cast<int>(blockIdx.x) >= ctas) return;
-    const int begin = cta_begin(blockIdx.x, total, ctas), end = cta_begin(blockIdx.x + 1, total, ctas);
+    const Sched sched = make_sched(p, pre);
+    if (sched.total == 0 || static_cast<int>(blockIdx.x) >= sched.ctas) return;
+    const int begin = cta_begin(sched, blockIdx.x), end = cta_begin(sched, blockIdx.x + 1);
 
-    if (warp == NCW) {
-        // ------------------------------------------------------------ producer
-        const uint64_t pol = policy_evict_first();
-        const int box_rows = min(p.t.P, KT);
-        const int ppt = p.tpp == 0 ? KT / p.t.P : 1;  // pages per tile
-        int i = 0, b = 0;
-        uint32_t filled = 0;  // slots that received a copy
-        bool ok = true;
-        for (int pos = begin; pos < end && ok;) {
-            const Segment g = segment_at(p, pre, pos, end, b);
-            const int* pages = p.t.pages + g.b * p.t.stride;
-            int win = -1, ids = -1;  // 32 consecutive page table entries, one per lane
-            for (int k = 0; k < g.count; ++k, ++i) {
-                const int tile = g.s.t0 + g.first + k;
-                const int lp0 = p.tpp == 0 ? tile * ppt : tile / p.tpp;
-                const int row0 = p.tpp == 0 ? 0 : (tile - lp0 * p.tpp) * KT;
-                if (lp0 / 32 != win) {
-                    win = lp0 / 32;
-                    const int e = win * 32 + lane;
-                    ids = e < p.t.max_pages ? __ldg(pages + e) : -1;
-                    if (static_cast<unsigned>(ids) >= static_cast<unsigned>(p.t.num_pages)) ids = -1;  // zero fill
-                }
-                const int s = i % L::NST, n = i / L::NST;
-                if (lane == 0) ok = mbar_wait(empty_bar(s), (n & 1) ^ 1, ab, 0x601);
-                ok = __shfl_sync(0xffffffffu, ok, 0);
-                if (!ok) break;
-                if (lane == 0) mbar_arrive_expect_tx(full_bar(s), L::STAGE);
-                filled |= 1u << s;
-                const uint32_t dst = smem_u32(ring + s * L::STAGE);
-                for (int j = 0; j < ppt; ++j) {
-                    const int page = __shfl_sync(0xffffffffu, ids, (lp0 + j) & 31);
-                    if (lane == 0) {
-                        const uint32_t d = dst + j * box_rows * 128;
-#pragma unroll
-                        for (int bx = 0; bx < L::NBOX; ++bx) {
-                            tma_load_4d(d + bx * L::BOX_BYTES, &tmK, full_bar(s), bx * 64, row0, g.kvh, page, pol);
-                            tma_load_4d(d + L::TILE + bx * L::BOX_BYTES, &tmV, full_bar(s), bx * 64, row0, g.kvh,
-                                        page, pol);
-                        }
-                    }
-                    __syncwarp();
-                }
-            }
-            pos += g.count;
-        }
-        if (!ok && lane == 0) {
-            // tile i was not issued; slot s last received tile j = the largest j < i with j % NST == s
-            for (int s = 0; s < L::NST; ++s)
-                if (filled >> s & 1u) {
-                    const int j = (i - 1) - ((i - 1 - s) % L::NST + L::NST) % L::NST;
-                    mbar_wait_drain(full_bar(s), (j / L::NST) & 1);
-                }
-        }
-        __syncwarp();
-        return;
-    }
-
-    // ---------------------------------------------------------------- consumers
     const int wrg = warp % NRG, wtg = warp / NRG;
     const int gq = lane >> 2, tq = lane & 3;
     uint32_t* words = reinterpret_cast<uint32_t*>(smem + L::OFF_MASK);
-    int* ctx_lo = reinterpret_cast<int*>(smem + L::OFF_MASK + L::RT * (kMaxTree / 32) * 4);
+    int* ctx_lo = reinterpret_cast<int*>(smem + L::OFF_MASK + L::MAX_RT * (kMaxTree / 32) * 4);
     const int nw = (p.t.T + 31) / 32;
     const uint32_t qs = smem_u32(smem + L::OFF_Q);
     float* part = reinterpret_cast<float*>(smem + L::OFF_PART);
     const float sl2 = p.scale_log2;
-    bool aborted = false;
+    bool aborted = false;       // consumers: a wait expired
     int i0 = 0, b = 0;  // running tile number of the segment's first tile
     for (int pos = begin; pos < end;) {
-        const Segment g = segment_at(p, pre, pos, end, b);
-        const int row0 = g.rt * p.RT;
-        // Q of the row tile (rotated) into shared memory, and the mask bits
+        const Segment g = segment_at(p, sched, pre, pos, end, b);
+        if (warp >= NCW) {
+            if (!produce<L>(p, g, i0, bars, smem_u32(ring), ab, threadIdx.x - 32 * NCW)) break;
+            i0 += g.count;
+            pos += g.count;
+            continue;
+        }
+        // ------------------------------------------------------------ consumers
+        const int row0 = g.rt * p.RT, ta = p.by_G.div(row0);
+        // Q of the row tile (turned, hi and lo) into shared memory, and the mask bits
         for (int idx = threadIdx.x; idx < p.RT * (DP / 8); idx += 32 * NCW) {
             const int r = idx / (DP / 8), ch = idx % (DP / 8);
-            *reinterpret_cast<uint4*>(smem + L::OFF_Q + chunk_off(p.RT, r, ch)) = load_q_chunk<E>(p, g, row0 + r, ch);
+            uint4 hi, lo;
+            load_q_chunk<E>(p, g, row0 + r, ch, hi, lo);
+            *reinterpret_cast<uint4*>(smem + L::OFF_Q + chunk_off(p.RT, r, ch)) = hi;
+            *reinterpret_cast<uint4*>(smem + L::OFF_Q + L::Q_BYTES + chunk_off(p.RT, r, ch)) = lo;
         }
         if (p.mask != nullptr) build_mask(p, g, words, ctx_lo, threadIdx.x, 32 * NCW);
         named_bar_sync(1, 32 * NCW);
         int rlo[2], rhi[2];
         const uint32_t* rw[2];
         for (int e = 0; e < 2; ++e) {
-            const int r = row0 + wrg * 16 + gq + 8 * e;
-            row_limits(p, g, r, ctx_lo, rlo[e], rhi[e]);
-            rw[e] = words + (p.mask != nullptr && r < p.rows && r / p.G < g.n ? (r / p.G - row0 / p.G) * nw : 0);
+            const int r = row0 + wrg * 16 + gq + 8 * e, t = p.by_G.div(r);
+            row_limits(p, g, r, ta, ctx_lo, rlo[e], rhi[e]);
+            rw[e] = words + (r < p.rows && t < g.n ? (t - ta) * nw : 0);
         }
         // keys in [all_lo, all_hi) are seen by every row of the group that sees any; what the
         // others (padding, empty) add up there is dropped at the end of the segment
@@ -512,127 +664,137 @@ __global__ void __launch_bounds__(THREADS, 1) fa_paged_kernel(const __grid_const
         int all_lo = max(dead[0] ? 0 : rlo[0], dead[1] ? 0 : rlo[1]);
         int all_hi = min(dead[0] ? INT_MAX : rhi[0], dead[1] ? INT_MAX : rhi[1]);
         if (p.mask != nullptr) all_hi = min(all_hi, g.L);
-        for (int d = 4; d < 32; d *= 2) {
-            all_lo = max(all_lo, __shfl_xor_sync(0xffffffffu, all_lo, d));
-            all_hi = min(all_hi, __shfl_xor_sync(0xffffffffu, all_hi, d));
-        }
-        uint32_t qa[DP <= 128 ? DP / 16 : 1][4];
-        auto load_q = [&](int kk, uint32_t* a) {
-            ldsm4(qs + chunk_off(p.RT, wrg * 16 + (lane & 15), 2 * kk + (lane >> 4)), a);
+        all_lo = __reduce_max_sync(0xffffffffu, all_lo);
+        all_hi = __reduce_min_sync(0xffffffffu, all_hi);
+        auto load_q = [&](int kk, int half, uint32_t* a) {
+            ldsm4(qs + half * L::Q_BYTES + chunk_off(p.RT, wrg * 16 + (lane & 15), 2 * kk + (lane >> 4)), a);
         };
-        if constexpr (DP <= 128) {
-#pragma unroll
-            for (int kk = 0; kk < DP / 16; ++kk) load_q(kk, qa[kk]);
-        }
         float oacc[DP / 8][4];
 #pragma unroll
         for (int j = 0; j < DP / 8; ++j) oacc[j][0] = oacc[j][1] = oacc[j][2] = oacc[j][3] = 0.f;
         float m_run[2] = {-INFINITY, -INFINITY};
         float l_run[2] = {0.f, 0.f};
 
-        // this warp's tiles of the segment: running numbers i with i % NTG == wtg
-        for (int i = i0 + ((wtg - i0) % NTG + NTG) % NTG; i < i0 + g.count; i += NTG) {
-            const int s = i % L::NST, n = i / L::NST;
+        // this warp's halves of the segment: running numbers hh with hh % NTG == wtg
+        for (int hh = 2 * i0 + ((wtg - 2 * i0) & (NTG - 1)); hh < 2 * (i0 + g.count); hh += NTG) {
+            const int i = hh >> 1, s = i % L::NST, kh = (hh & 1) * 32;  // first key row of the half
             int k0, valid;
             tile_keys(p, g.s.t0 + g.first + (i - i0), k0, valid);
-            bool ok = !aborted && mbar_wait(full_bar(s), n & 1, ab, 0x602);
+            k0 += kh;
+            valid -= kh;
+            bool ok = !aborted && mbar_wait(full_bar(s), i / L::NST & 1, ab, 0x602);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) {
                 aborted = true;
                 continue;
             }
-            const uint32_t kb = smem_u32(ring + s * L::STAGE), vb = kb + L::TILE;
-            const bool edge = valid < KT || k0 < all_lo || k0 + KT > all_hi;
-            // slots no row of the unit sees may hold anything: V rows there become zeros (0 * NaN)
-            const bool dirty = k0 < g.s.lo || k0 + KT > g.s.hi;
-            if (dirty) {
-                for (int idx = lane; idx < KT * (DP / 8); idx += 32) {
-                    const int r = idx / (DP / 8);
-                    if (k0 + r < g.s.lo || k0 + r >= g.s.hi)
-                        *reinterpret_cast<uint4*>(ring + s * L::STAGE + L::TILE + chunk_off(KT, r, idx % (DP / 8))) =
-                            uint4{0u, 0u, 0u, 0u};
+            // the last warp-half of a tile to finish frees its slot
+            const bool last = NTG > 1 || (hh & 1);
+            const bool none = valid <= 0 || k0 >= g.s.hi || k0 + 32 <= g.s.lo;
+            const uint32_t kb = smem_u32(ring) + s * L::STAGE, vb = kb + L::TILE;
+            const bool edge = valid < 32 || k0 < all_lo || k0 + 32 > all_hi;
+            if (!none) {
+                float sc[4][4];
+#pragma unroll
+                for (int nt = 0; nt < 4; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+                // fragments of step kk + 1 load while step kk multiplies (Q's too: kept in
+                // registers it would cost the eight warps their 168 registers each)
+                const int krow = kh + (lane & 7) + 8 * (lane >> 4), kch = lane >> 3 & 1;
+                uint32_t bk[2][2][4], al[2][4], ah[2][4];
+                auto load_k = [&](int kk) {
+                    ldsm4(kb + chunk_off(KT, krow, 2 * kk + kch), bk[kk & 1][0]);
+                    ldsm4(kb + chunk_off(KT, krow + 16, 2 * kk + kch), bk[kk & 1][1]);
+                    load_q(kk, 1, al[kk & 1]);
+                    load_q(kk, 0, ah[kk & 1]);
+                };
+                load_k(0);
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk) {
+                    if (kk + 1 < DP / 16) load_k(kk + 1);
+#pragma unroll
+                    for (int nt = 0; nt < 4; ++nt)
+                        mma16816<E>(sc[nt], ah[kk & 1], bk[kk & 1][nt >> 1][2 * (nt & 1)], bk[kk & 1][nt >> 1][2 * (nt & 1) + 1]);
+#pragma unroll
+                    for (int nt = 0; nt < 4; ++nt)
+                        mma16816<E>(sc[nt], al[kk & 1], bk[kk & 1][nt >> 1][2 * (nt & 1)],
+                                    bk[kk & 1][nt >> 1][2 * (nt & 1) + 1]);
                 }
-                __syncwarp();
-            }
-            float sc[4][4];
+                float mx[2] = {-INFINITY, -INFINITY};
+                if (edge) {
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+                    for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
-            for (int kk = 0; kk < DP / 16; ++kk) {
-                uint32_t a_[4];
-                if constexpr (DP > 128) load_q(kk, a_);
-                const uint32_t* a = DP <= 128 ? qa[DP <= 128 ? kk : 0] : a_;
-#pragma unroll
-                for (int np = 0; np < 2; ++np) {
-                    const int key = 16 * np + (lane & 7) + 8 * (lane >> 4), chunk = 2 * kk + (lane >> 3 & 1);
-                    uint32_t bk[4];
-                    ldsm4(kb + chunk_off(KT, key, chunk), bk);
-                    mma16816<E>(sc[2 * np], a, bk[0], bk[1]);
-                    mma16816<E>(sc[2 * np + 1], a, bk[2], bk[3]);
+                        for (int e = 0; e < 4; ++e) {
+                            const int ri = e >> 1, kr = 8 * nt + 2 * tq + (e & 1), key = k0 + kr;
+                            bool see = kr < valid && key >= rlo[ri] && key < rhi[ri];
+                            if (p.mask != nullptr && see && key >= g.L)
+                                see = rw[ri][(key - g.L) >> 5] >> ((key - g.L) & 31) & 1u;
+                            if (!see) sc[nt][e] = -INFINITY * (sl2 < 0.f ? -1.f : 1.f);
+                        }
                 }
-            }
-            float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int nt = 0; nt < 4; ++nt)
+                for (int nt = 0; nt < 4; ++nt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float v = sc[nt][e] * sl2;
-                    if (edge) {
-                        const int ri = e >> 1, kr = 8 * nt + 2 * tq + (e & 1), key = k0 + kr;
-                        bool see = kr < valid && key >= rlo[ri] && key < rhi[ri];
-                        if (p.mask != nullptr && see && key >= g.L)
-                            see = rw[ri][(key - g.L) >> 5] >> ((key - g.L) & 31) & 1u;
-                        if (!see) v = -INFINITY;
+                    for (int e = 0; e < 4; ++e) {
+                        sc[nt][e] *= sl2;
+                        mx[e >> 1] = fmaxf(mx[e >> 1], sc[nt][e]);
                     }
-                    sc[nt][e] = v;
-                    mx[e >> 1] = fmaxf(mx[e >> 1], v);
+                float corr[2], mref[2];
+#pragma unroll
+                for (int ri = 0; ri < 2; ++ri) {
+                    mx[ri] = fmaxf(mx[ri], __shfl_xor_sync(0xffffffffu, mx[ri], 1));
+                    mx[ri] = fmaxf(mx[ri], __shfl_xor_sync(0xffffffffu, mx[ri], 2));
+                    const float mn = fmaxf(m_run[ri], mx[ri]);
+                    corr[ri] = mn == -INFINITY ? 1.f : ex2(m_run[ri] - mn);
+                    m_run[ri] = mn;
+                    mref[ri] = mn == -INFINITY ? 0.f : mn;
+                    l_run[ri] *= corr[ri];
                 }
-            float corr[2], mref[2];
+                if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
 #pragma unroll
-            for (int ri = 0; ri < 2; ++ri) {
-                mx[ri] = fmaxf(mx[ri], __shfl_xor_sync(0xffffffffu, mx[ri], 1));
-                mx[ri] = fmaxf(mx[ri], __shfl_xor_sync(0xffffffffu, mx[ri], 2));
-                const float mn = fmaxf(m_run[ri], mx[ri]);
-                corr[ri] = mn == -INFINITY ? 1.f : ex2(m_run[ri] - mn);
-                m_run[ri] = mn;
-                mref[ri] = mn == -INFINITY ? 0.f : mn;
-                l_run[ri] *= corr[ri];
-            }
-#pragma unroll
-            for (int j = 0; j < DP / 8; ++j) {
-                oacc[j][0] *= corr[0];
-                oacc[j][1] *= corr[0];
-                oacc[j][2] *= corr[1];
-                oacc[j][3] *= corr[1];
-            }
-            // P is rounded to the cache's type, the operand type of the second product;
-            // the row sums take it unrounded
-            uint32_t pa[2][4];
-#pragma unroll
-            for (int k2 = 0; k2 < 2; ++k2)
-#pragma unroll
-                for (int h2 = 0; h2 < 2; ++h2) {
-                    const int nt = 2 * k2 + h2;
-                    const float p0 = ex2(sc[nt][0] - mref[0]), p1 = ex2(sc[nt][1] - mref[0]);
-                    const float p2 = ex2(sc[nt][2] - mref[1]), p3 = ex2(sc[nt][3] - mref[1]);
-                    l_run[0] += p0 + p1;
-                    l_run[1] += p2 + p3;
-                    pa[k2][2 * h2] = E::pack(p0, p1);
-                    pa[k2][2 * h2 + 1] = E::pack(p2, p3);
+                    for (int j = 0; j < DP / 8; ++j) {
+                        oacc[j][0] *= corr[0];
+                        oacc[j][1] *= corr[0];
+                        oacc[j][2] *= corr[1];
+                        oacc[j][3] *= corr[1];
+                    }
                 }
+                // P is rounded to the cache's type, the operand type of the second product;
+                // the row sums take it unrounded
+                uint32_t pa[2][4];
 #pragma unroll
-            for (int k2 = 0; k2 < 2; ++k2)
+                for (int k2 = 0; k2 < 2; ++k2)
+#pragma unroll
+                    for (int h2 = 0; h2 < 2; ++h2) {
+                        const int nt = 2 * k2 + h2;
+                        const float p0 = ex2(sc[nt][0] - mref[0]), p1 = ex2(sc[nt][1] - mref[0]);
+                        const float p2 = ex2(sc[nt][2] - mref[1]), p3 = ex2(sc[nt][3] - mref[1]);
+                        l_run[0] += p0 + p1;
+                        l_run[1] += p2 + p3;
+                        pa[k2][2 * h2] = E::pack(p0, p1);
+                        pa[k2][2 * h2 + 1] = E::pack(p2, p3);
+                    }
+                constexpr int VB = DP <= 128 ? 2 : 1;  // buffers: registers are short at 256
+                uint32_t bv[VB][2][4];
+                auto load_v = [&](int dp) {
+#pragma unroll
+                    for (int k2 = 0; k2 < 2; ++k2)
+                        ldsm4_t(vb + chunk_off(KT, kh + 16 * k2 + (lane & 15), 2 * dp + (lane >> 4)), bv[dp % VB][k2]);
+                };
+                load_v(0);
 #pragma unroll
                 for (int dp = 0; dp < DP / 16; ++dp) {
-                    const int key = 16 * k2 + (lane & 15), chunk = 2 * dp + (lane >> 4);
-                    uint32_t bv[4];
-                    ldsm4_t(vb + chunk_off(KT, key, chunk), bv);
-                    mma16816<E>(oacc[2 * dp], pa[k2], bv[0], bv[1]);
-                    mma16816<E>(oacc[2 * dp + 1], pa[k2], bv[2], bv[3]);
+                    if (VB > 1 && dp + 1 < DP / 16) load_v(dp + 1);
+#pragma unroll
+                    for (int k2 = 0; k2 < 2; ++k2) {
+                        mma16816<E>(oacc[2 * dp], pa[k2], bv[dp % VB][k2][0], bv[dp % VB][k2][1]);
+                        mma16816<E>(oacc[2 * dp + 1], pa[k2], bv[dp % VB][k2][2], bv[dp % VB][k2][3]);
+                    }
+                    if (VB == 1 && dp + 1 < DP / 16) load_v(dp + 1);
                 }
-            if (dirty) fence_proxy_async_smem();  // the zeros before the slot's next copy
+            }
             __syncwarp();
-            if (lane == 0) mbar_arrive(empty_bar(s));
+            if (lane == 0 && last) mbar_arrive(empty_bar(s));
         }
 #pragma unroll
         for (int ri = 0; ri < 2; ++ri) {
@@ -641,6 +803,7 @@ __global__ void __launch_bounds__(THREADS, 1) fa_paged_kernel(const __grid_const
         }
         // join the NTG warps of each row group in shared memory, then write the
         // rows out (a whole unit) or to the workspace (a part)
+        if constexpr (L::ALIAS) named_bar_sync(1, 32 * NCW);
         float* wp = part + warp * 16 * L::PSTR;
 #pragma unroll
         for (int ri = 0; ri < 2; ++ri) {
@@ -659,31 +822,33 @@ __global__ void __launch_bounds__(THREADS, 1) fa_paged_kernel(const __grid_const
         float* slot = partial_slot(p, 2 * blockIdx.x + (pos - g.first <= begin ? 0 : 1));
         const int rows = min(p.RT, p.rows - row0);
         if (!*abort_flag) {
-            for (int idx = threadIdx.x; idx < rows * (p.D / 8); idx += 32 * NCW) {
-                const int lr = idx / (p.D / 8), c8 = idx % (p.D / 8);
-                const float* row = part + (lr / 16) * 16 * L::PSTR + (lr % 16) * L::PSTR;
+            for (int idx = threadIdx.x; idx < rows * (DP / 4); idx += 32 * NCW) {
+                const int lr = idx / (DP / 4), c = idx % (DP / 4) * 4;
+                if (c >= p.D) continue;
+                const float* row = part + ((lr / 16) * 16 + lr % 16) * L::PSTR;
+                const int step = NRG * 16 * L::PSTR;
                 float M = -INFINITY;
-                for (int k = 0; k < NTG; ++k) M = fmaxf(M, row[k * NRG * 16 * L::PSTR + DP]);
-                float o[8] = {}, l = 0.f;
+                for (int k = 0; k < NTG; ++k) M = fmaxf(M, row[k * step + DP]);
+                float4 o{};
+                float l = 0.f;
                 for (int k = 0; k < NTG; ++k) {
-                    const float* x = row + k * NRG * 16 * L::PSTR;
+                    const float* x = row + k * step;
                     const float f = x[DP] == -INFINITY ? 0.f : ex2(x[DP] - M);
+                    const float4 v = *reinterpret_cast<const float4*>(x + c);
                     l += f * x[DP + 1];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) o[e] += f * x[8 * c8 + e];
+                    o.x += f * v.x;
+                    o.y += f * v.y;
+                    o.z += f * v.z;
+                    o.w += f * v.w;
                 }
                 if (whole) {
                     const float inv = l == 0.f ? 0.f : 1.f / l;
-                    const int r = row0 + lr;
-                    const uint4 v{E::pack(o[0] * inv, o[1] * inv), E::pack(o[2] * inv, o[3] * inv),
-                                  E::pack(o[4] * inv, o[5] * inv), E::pack(o[6] * inv, o[7] * inv)};
-                    *reinterpret_cast<uint4*>(p.o + g.b * p.osb + (g.kvh * p.G + r % p.G) * p.osh +
-                                              (r / p.G) * p.oss + 8 * c8) = v;
+                    const int r = row0 + lr, t = p.by_G.div(r);
+                    *reinterpret_cast<uint2*>(p.o + g.b * p.osb + (g.kvh * p.G + r - t * p.G) * p.osh + t * p.oss + c) =
+                        uint2{E::pack(o.x * inv, o.y * inv), E::pack(o.z * inv, o.w * inv)};
                 } else {
-                    float4* d = reinterpret_cast<float4*>(slot + lr * p.D + 8 * c8);
-                    d[0] = make_float4(o[0], o[1], o[2], o[3]);
-                    d[1] = make_float4(o[4], o[5], o[6], o[7]);
-                    if (c8 == 0) {
+                    *reinterpret_cast<float4*>(slot + lr * p.D + c) = o;
+                    if (c == 0) {
                         slot[p.RT * p.D + lr] = M;
                         slot[p.RT * p.D + p.RT + lr] = l;
                     }
@@ -694,6 +859,7 @@ __global__ void __launch_bounds__(THREADS, 1) fa_paged_kernel(const __grid_const
         i0 += g.count;
         pos += g.count;
     }
+    if (warp >= NCW) cp_async_wait_all();  // after an expired wait too, no copy outlives the CTA
 }
 
 }  // namespace paged

@@ -53,6 +53,16 @@ __device__ __forceinline__ uint32_t rotate_pair(uint32_t v, float c, float s) {
     return E::pack(__fmaf_rn(x.x, c, -__fmul_rn(x.y, s)), __fmaf_rn(x.x, s, __fmul_rn(x.y, c)));
 }
 
+// The same, as hi + lo: the rounded pair and what the rounding left, rounded again.
+template <class E>
+__device__ __forceinline__ void turn_split(uint32_t& hi, uint32_t& lo, float c, float s) {
+    const float2 x = E::unpack(hi);
+    const float a = __fmaf_rn(x.x, c, -__fmul_rn(x.y, s)), b = __fmaf_rn(x.x, s, __fmul_rn(x.y, c));
+    hi = E::pack(a, b);
+    const float2 h = E::unpack(hi);
+    lo = E::pack(a - h.x, b - h.y);
+}
+
 // 16 bytes = 4 pairs.
 template <class E>
 __device__ __forceinline__ uint4 rotate4(const uint4& x, const float4& c, const float4& s) {

@@ -93,18 +93,16 @@ int launched() {
 // How a paged attention call is cut: rows per tile, key tiles per page.
 struct PagedPlan {
     int dp;     // head_dim rounded up to the kernel's 64, 128 or 256
-    int RT, n_rt, KT, tpp, grid;
+    int RT, n_rt, tpp, grid;
 };
 
 PagedPlan paged_plan(uint32_t H, uint32_t Hkv, uint32_t T, uint32_t D, uint32_t P) {
     PagedPlan f{};
     f.dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
     const int64_t rows = static_cast<int64_t>(H / Hkv) * T;
-    const int max_rt = f.dp <= 128 ? 64 : 32;
-    f.RT = rows <= 16 ? 16 : rows <= 32 ? 32 : max_rt;
+    f.RT = f.dp <= 128 || rows <= 16 ? 16 : 32;
     f.n_rt = static_cast<int>((rows + f.RT - 1) / f.RT);
-    f.KT = paged::KT;
-    f.tpp = static_cast<int>(P) >= f.KT ? (static_cast<int>(P) + f.KT - 1) / f.KT : 0;
+    f.tpp = static_cast<int>(P) >= paged::KT ? (static_cast<int>(P) + paged::KT - 1) / paged::KT : 0;
     f.grid = sm_count();
     return f;
 }
@@ -222,6 +220,8 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
     p.osb = a.oStrideB;
     p.osh = a.oStrideH;
     p.oss = a.oStrideS;
+    p.kc = cache_view(c.kCache, c.kcStrideP, c.kcStrideH, c.kcStrideS);
+    p.vc = cache_view(c.vCache, c.vcStrideP, c.vcStrideH, c.vcStrideS);
     p.t = make_table(c, a.newLens, a.seqLen);
     p.mask = static_cast<const uint8_t*>(a.treeMask);
     p.msb = a.maskStrideB;
@@ -237,32 +237,23 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
     p.rows = static_cast<int>(rows);
     p.RT = f.RT;
     p.n_rt = f.n_rt;
-    p.KT = f.KT;
     p.tpp = f.tpp;
+    p.by_G.set(static_cast<uint32_t>(p.G));
+    p.by_P.set(c.pageSize);
+    p.by_tpp.set(f.tpp == 0 ? 1 : static_cast<uint32_t>(f.tpp));
     p.window = a.windowSize > 0 ? a.windowSize : 0;
     p.scale_log2 = a.scale * 1.4426950408889634f;
     p.ws = static_cast<float*>(workspace);
     p.grid = f.grid;
 
     // the list positions of one launch are 32-bit: as many sequences per launch as surely fit
-    const int64_t tiles = f.tpp == 0 ? (static_cast<int64_t>(c.maxPages) * c.pageSize + f.KT - 1) / f.KT
+    const int64_t tiles = f.tpp == 0 ? (static_cast<int64_t>(c.maxPages) * c.pageSize + paged::KT - 1) / paged::KT
                                      : static_cast<int64_t>(c.maxPages) * f.tpp;
     const int64_t per_seq = tiles * p.n_rt * p.Hkv;
     const int64_t join_rows = static_cast<int64_t>(p.Hkv) * p.n_rt * ((f.RT + paged::kJoinWarps - 1) / paged::kJoinWarps);
     const int64_t fit = INT32_MAX / (per_seq > join_rows ? per_seq : join_rows);
     if (fit == 0) return pfail("problem too large for one launch");
     const int64_t step = fit < paged::kMaxBatch ? fit : paged::kMaxBatch;
-
-    CUtensorMap tmK, tmV;
-    const uint32_t box_rows = c.pageSize < static_cast<uint32_t>(f.KT) ? c.pageSize : f.KT;
-    const CUtensorMapDataType dt =
-        c.dtype == paged::DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    const View4 vk{c.kCache, {c.headDim, c.pageSize, c.numKvHeads, c.numPages}, {c.kcStrideS, c.kcStrideH, c.kcStrideP}};
-    const View4 vv{c.vCache, {c.headDim, c.pageSize, c.numKvHeads, c.numPages}, {c.vcStrideS, c.vcStrideH, c.vcStrideP}};
-    const char* e = nullptr;
-    if ((e = make_map(&tmK, vk, dt, 2, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B)) ||
-        (e = make_map(&tmV, vv, dt, 2, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B)))
-        return pfail(e);
 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     for (int64_t b0 = 0; b0 < c.batchSize; b0 += step) {
@@ -275,34 +266,41 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
         if (s.t.new_lens != nullptr) s.t.new_lens += b0;
         if (s.mask != nullptr) s.mask += b0 * p.msb;
         if (s.positions != nullptr) s.positions += b0 * a.seqLen;
-        auto launch = [&](auto kern, int smem) {
-            cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-            if (ce != cudaSuccess) return ce;
-            return launch_timed(st, [&] {
-                kern<<<f.grid, paged::THREADS, smem, st>>>(tmK, tmV, s);
-                return cudaGetLastError();
-            });
-        };
-        auto by_width = [&](auto E) {
-            using T = decltype(E);
-            switch (f.dp) {
-                case 64: return launch(paged::fa_paged_kernel<T, 64>, paged::Layout<64>::SMEM_BYTES);
-                case 128: return launch(paged::fa_paged_kernel<T, 128>, paged::Layout<128>::SMEM_BYTES);
-                default: return launch(paged::fa_paged_kernel<T, 256>, paged::Layout<256>::SMEM_BYTES);
-            }
-        };
-        cudaError_t ce = c.dtype == paged::DT_F16 ? by_width(paged::F16{}) : by_width(paged::BF16{});
-        if (ce != cudaSuccess) return fail(g_err_paged, "%s", cudaGetErrorString(ce));
-        // the join starts while the attention kernel drains and waits for it before it reads
+        // Both kernels may start while the one before them on the stream ends: the
+        // attention kernel waits for it before it reads or writes global memory, the join
+        // waits for the attention kernel.
         cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(static_cast<unsigned>(s.B * join_rows));
-        cfg.blockDim = dim3(32 * paged::kJoinWarps);
-        cfg.stream = st;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
+        cfg.stream = st;
+        cfg.gridDim = dim3(static_cast<unsigned>(f.grid));
+        auto launch = [&](auto kern, int threads, int smem) {
+            cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+            if (ce != cudaSuccess) return ce;
+            cfg.blockDim = dim3(threads);
+            cfg.dynamicSmemBytes = smem;
+            return launch_timed(st, [&] { return cudaLaunchKernelEx(&cfg, kern, s); });
+        };
+        auto by_width = [&](auto E) {
+            using T = decltype(E);
+            using L64 = paged::Layout<64>;
+            using L128 = paged::Layout<128>;
+            using L256 = paged::Layout<256>;
+            switch (f.dp) {
+                case 64: return launch(paged::fa_paged_kernel<T, 64>, L64::THREADS, L64::SMEM_BYTES);
+                case 128: return launch(paged::fa_paged_kernel<T, 128>, L128::THREADS, L128::SMEM_BYTES);
+                default: return launch(paged::fa_paged_kernel<T, 256>, L256::THREADS, L256::SMEM_BYTES);
+            }
+        };
+        cudaError_t ce = c.dtype == paged::DT_F16 ? by_width(paged::F16{}) : by_width(paged::BF16{});
+        if (ce == cudaSuccess) ce = cudaGetLastError();
+        if (ce != cudaSuccess) return fail(g_err_paged, "%s", cudaGetErrorString(ce));
+        cfg.gridDim = dim3(static_cast<unsigned>(s.B * join_rows));
+        cfg.blockDim = dim3(32 * paged::kJoinWarps);
+        cfg.dynamicSmemBytes = 0;
         ce = c.dtype == paged::DT_F16 ? cudaLaunchKernelEx(&cfg, paged::join_kernel<paged::F16>, s)
                                       : cudaLaunchKernelEx(&cfg, paged::join_kernel<paged::BF16>, s);
         if (ce == cudaSuccess) ce = cudaGetLastError();
