@@ -68,10 +68,22 @@ struct AttnParams {
     FastDiv by_tpp;
     FastDiv by_P;
     int window;  // 0: none
-    float scale_log2;
-    float* ws;   // partials: 2 per CTA, each O [RT][D], m [RT], l [RT]
+    float scale_log2;  // |scale| log2 e (never 0: masked scores are -inf times it)
+    uint32_t flip;     // 0x80008000 for a negative scale: the query's signs turn instead
+    float* ws;   // partials: 2 per CTA, each O [D / 4][RT] float4, m [RT], l [RT]
+    int2* units; // per unit (b, kvh, rt): first partial's slot, number of parts (0 or 1: nothing to join)
     int grid;    // CTAs of the attention kernel
 };
+
+// Touches every line of the parameters once (one word per lane and 64 bytes), so that
+// the constant-cache misses of a fresh launch overlap each other and the wait for the
+// kernel before, instead of standing one by one in the way of the schedule.
+__device__ __forceinline__ void warm_params(const AttnParams& p) {
+    const int* w = reinterpret_cast<const int*>(&p);
+    const int at = (threadIdx.x & 31) * 16;
+    int v = w[at < static_cast<int>(sizeof(AttnParams) / 4) ? at : 0];
+    asm volatile("" ::"r"(v));
+}
 
 // ---------------------------------------------------------------- the schedule
 struct Span {
@@ -100,17 +112,11 @@ __device__ __forceinline__ Span row_tile_span(const AttnParams& p, int L, int n,
     return s;
 }
 
-// The list of a launch, as each warp sees it.  Up to 32 sequences it lies in the
-// warp's registers (lane b: sequence b), so that no barrier and no second load
-// stands between the lengths and the first key tile; more of them take a prefix
-// array in shared memory.
+// The list of a launch: pre[b] (shared memory) = list position behind sequence b.
 struct Sched {
-    int total;    // tiles of the launch
-    int L, n;     // lane b: lengths of sequence b
-    int head;     // lane b: tiles of one of its KV heads
-    int end;      // lane b: list position behind it
-    int q, r;     // the first r CTAs take q + 1 tiles, the others q
-    int ctas;     // CTAs that take part
+    int total;  // tiles of the launch
+    int ctas;   // CTAs that take part
+    int q, r;   // the first r of them take q + 1 tiles, the others q
 };
 
 __device__ __forceinline__ int head_tiles(const AttnParams& p, int L, int n) {
@@ -128,18 +134,19 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {
     return v;
 }
 
-// All threads of the block; `pre` [B] is used above 32 sequences only.
+// All threads of the block.  Up to 32 sequences every warp computes the whole list and
+// writes the same values, so that no barrier stands between the lengths and the first
+// key tile.
 __device__ __forceinline__ Sched make_sched(const AttnParams& p, int* pre) {
     const int lane = threadIdx.x & 31;
-    Sched s{};
+    Sched s;
     if (p.B <= 32) {
-        if (lane < p.B) {
-            s.L = p.t.len(lane);
-            s.n = p.t.news(lane);
-            s.head = head_tiles(p, s.L, s.n);
-        }
-        s.end = warp_scan(s.head * p.Hkv, lane);
-        s.total = __shfl_sync(0xffffffffu, s.end, 31);
+        int v = 0;
+        if (lane < p.B) v = head_tiles(p, p.t.len(lane), p.t.news(lane)) * p.Hkv;
+        v = warp_scan(v, lane);
+        if (lane < p.B) pre[lane] = v;
+        s.total = __shfl_sync(0xffffffffu, v, 31);
+        __syncwarp();
     } else {
         for (int b = threadIdx.x; b < p.B; b += blockDim.x)
             pre[b] = head_tiles(p, p.t.len(b), p.t.news(b)) * p.Hkv;
@@ -180,26 +187,21 @@ struct Segment {
 
 // The segment at list position pos < total (a whole warp; b: a sequence at or
 // before it, kept from call to call).
-__device__ __forceinline__ Segment segment_at(const AttnParams& p, const Sched& sc, const int* pre, int pos, int end,
-                                              int& b) {
-    Segment g;
-    int off, head;
-    if (p.B <= 32) {
-        b = __ffs(__ballot_sync(0xffffffffu, sc.end > pos)) - 1;
-        const int start = __shfl_sync(0xffffffffu, sc.end - sc.head * p.Hkv, b);
-        head = __shfl_sync(0xffffffffu, sc.head, b);
-        g.L = __shfl_sync(0xffffffffu, sc.L, b);
-        g.n = __shfl_sync(0xffffffffu, sc.n, b);
-        off = pos - start;
-    } else {
-        while (pre[b] <= pos) ++b;
-        const int start = b > 0 ? pre[b - 1] : 0;
-        head = (pre[b] - start) / p.Hkv;
-        g.L = p.t.len(b);
-        g.n = p.t.news(b);
-        off = pos - start;
+__device__ __forceinline__ Segment segment_at(const AttnParams& p, const int* pre, int pos, int end, int& b) {
+    const int lane = threadIdx.x & 31;
+    for (;; b += 32) {
+        const uint32_t past = __ballot_sync(0xffffffffu, b + lane < p.B && pre[b + lane] > pos);
+        if (past != 0) {
+            b += __ffs(past) - 1;
+            break;
+        }
     }
+    Segment g;
     g.b = b;
+    g.L = p.t.len(b);
+    g.n = p.t.news(b);
+    const int start = b > 0 ? pre[b - 1] : 0, head = (pre[b] - start) / p.Hkv;
+    int off = pos - start;
     g.kvh = off / head;
     off -= g.kvh * head;
     for (g.rt = 0;; ++g.rt) {
@@ -227,6 +229,36 @@ __device__ __forceinline__ void tile_keys(const AttnParams& p, int tile, int& k0
 
 __device__ __forceinline__ float* partial_slot(const AttnParams& p, int slot) {
     return p.ws + static_cast<int64_t>(slot) * p.RT * (p.D + 2);
+}
+__device__ __forceinline__ int unit_index(const AttnParams& p, int b, int kvh, int rt) {
+    return (b * p.Hkv + kvh) * p.n_rt + rt;
+}
+// The slot of a segment's partial: a CTA starts with at most one unit that began before it
+// (or with it) and ends with at most one other that goes on.
+__device__ __forceinline__ int segment_slot(const Segment& g, int pos, int begin) {
+    return 2 * static_cast<int>(blockIdx.x) + (pos - g.first <= begin ? 0 : 1);
+}
+// What the join needs to know about a unit, from the CTA that holds its first tile.
+__device__ __forceinline__ void describe_unit(const AttnParams& p, const Sched& sc, const Segment& g, int pos,
+                                              int begin) {
+    const int parts = g.count == g.s.n ? 1 : cta_of(sc, pos + g.s.n - 1) - static_cast<int>(blockIdx.x) + 1;
+    p.units[unit_index(p, g.b, g.kvh, g.rt)] = make_int2(segment_slot(g, pos, begin), parts);
+}
+
+// Row tiles that see no key belong to no CTA's list: their output rows are zeroed, and
+// described, by CTA (b, rt) modulo the grid.  tid .. of nthreads threads.
+__device__ __forceinline__ void zero_empty_units(const AttnParams& p, int tid, int nthreads) {
+    for (int u = blockIdx.x; u < p.B * p.n_rt; u += gridDim.x) {
+        const int b = u / p.n_rt, rt = u - b * p.n_rt;
+        if (row_tile_span(p, p.t.len(b), p.t.news(b), rt).n > 0) continue;
+        const int rows = min(p.RT, p.rows - rt * p.RT), nch = p.D / 8;
+        for (int i = tid; i < p.Hkv * rows * nch; i += nthreads) {
+            const int ch = i % nch, r = i / nch % rows, kvh = i / nch / rows, row = rt * p.RT + r;
+            const int t = p.by_G.div(row), h = kvh * p.G + row - t * p.G;
+            *reinterpret_cast<uint4*>(p.o + b * p.osb + h * p.osh + t * p.oss + ch * 8) = uint4{0u, 0u, 0u, 0u};
+        }
+        for (int kvh = tid; kvh < p.Hkv; kvh += nthreads) p.units[unit_index(p, b, kvh, rt)] = make_int2(0, 0);
+    }
 }
 
 // Bits of the drafted tokens that the tokens of a row tile see: words[i * nw + w]
@@ -269,100 +301,68 @@ __device__ __forceinline__ void build_mask(const AttnParams& p, const Segment& g
 }
 
 // ------------------------------------------------------------- the join kernel
-// One warp per row of a split unit: O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i
-// over the CTAs that hold a part, in list order.  Units with no visible key get
-// their zeros here; whole units were written by the attention kernel.
-constexpr int kJoinWarps = 4;
+// O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a split unit's parts, in list
+// order.  A block takes 16 rows; a thread one row (lanes side by side, so the partials
+// are read in whole lines) and 8 columns.  Bound by the latency of three dependent reads
+// (the unit, its parts, the store); four parts' loads are in flight at a time.
+constexpr int kJoinRows = 16;
 
 template <class E>
-__global__ void __launch_bounds__(32 * kJoinWarps) join_kernel(const __grid_constant__ AttnParams p) {
-    __shared__ int pre[kMaxBatch];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    // the lengths may be read before the attention kernel has ended: it started
-    // only after what wrote them
-    const Sched sc = make_sched(p, pre);
-    const int groups = (p.RT + kJoinWarps - 1) / kJoinWarps;
-    const int unit = blockIdx.x / groups;  // (b, kvh, rt)
-    const int rt = unit % p.n_rt, kvh = unit / p.n_rt % p.Hkv, b = unit / p.n_rt / p.Hkv;
-    const int lr = blockIdx.x % groups * kJoinWarps + threadIdx.x / 32;  // row of the tile
-    const int r = rt * p.RT + lr;
-    const int lane = threadIdx.x & 31;
-    const int L = p.t.len(b), n = p.t.news(b);
-    int head = 0, before = 0, tiles = 0;
-    for (int i = 0; i < p.n_rt; ++i) {
-        const int w = row_tile_span(p, L, n, i).n;
-        if (i < rt) before += w;
-        if (i == rt) tiles = w;
-        head += w;
-    }
-    const int end = p.B <= 32 ? __shfl_sync(0xffffffffu, sc.end, b & 31) : pre[b];
-    const int pos = end - head * p.Hkv + kvh * head + before;
-    const int c0 = tiles > 0 ? cta_of(sc, pos) : 0, c1 = tiles > 0 ? cta_of(sc, pos + tiles - 1) : 0;
+__global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ AttnParams p) {
+    const int groups = (p.RT + kJoinRows - 1) / kJoinRows;
+    const int unit = blockIdx.x / groups;
+    const int lr = blockIdx.x % groups * kJoinRows + threadIdx.x % kJoinRows;  // row of the tile
+    const int c = threadIdx.x / kJoinRows * 8;                                 // first column
     grid_dependency_wait();
-    if (lr >= p.RT || r >= p.rows || (tiles > 0 && c0 == c1)) return;
-    const int t = p.by_G.div(r), h = kvh * p.G + r - t * p.G;
-    uint16_t* out = p.o + b * p.osb + h * p.osh + t * p.oss;
-    if (tiles == 0) {
-        for (int d = lane * 4; d < p.D; d += 128) *reinterpret_cast<uint2*>(out + d) = uint2{0u, 0u};
-        return;
-    }
-    // the unit starts in CTA c0 (its slot 0 if the CTA starts with it); every later
-    // part is the first of its CTA
-    const int slot0 = 2 * c0 + (pos == cta_begin(sc, c0) ? 0 : 1);
-    const int parts = c1 - c0 + 1;
-    auto part = [&](int i) { return partial_slot(p, i == 0 ? slot0 : 2 * (c0 + i)); };
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int2 u = p.units[unit];
+    const int rt = unit % p.n_rt, r = rt * p.RT + lr;
+    if (u.y < 2 || r >= p.rows) return;
     float M = -INFINITY, l = 0.f;
-    float4 o[2] = {};
-    for (int i0 = 0; i0 < parts; i0 += 32) {
-        // lane i: the weight of part i0 + i
-        float m = -INFINITY, li = 0.f;
-        if (i0 + lane < parts) {
-            const float* w = part(i0 + lane) + p.RT * p.D + lr;
-            m = w[0];
-            li = w[p.RT];
-        }
-        float mx = fmaxf(M, m);
+    float o[8] = {};
+    for (int i0 = 0; i0 < u.y; i0 += 4) {
+        float m[4], li[4];
+        float4 x[4][2];
 #pragma unroll
-        for (int d = 16; d > 0; d /= 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-        const float f = m == -INFINITY ? 0.f : ex2(m - mx);
-        const float g = M == -INFINITY ? 0.f : ex2(M - mx);
-        M = mx;
-        l = l * g + li * f;  // per lane, summed at the end
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            o[k].x *= g;
-            o[k].y *= g;
-            o[k].z *= g;
-            o[k].w *= g;
-        }
-        const int here = min(32, parts - i0);
-#pragma unroll 4
-        for (int i = 0; i < here; ++i) {
-            const float fi = __shfl_sync(0xffffffffu, f, i);
-            const float* w = part(i0 + i) + lr * p.D;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const int d = lane * 4 + 128 * k;
-                if (d < p.D) {
-                    const float4 x = *reinterpret_cast<const float4*>(w + d);
-                    o[k].x += fi * x.x;
-                    o[k].y += fi * x.y;
-                    o[k].z += fi * x.z;
-                    o[k].w += fi * x.w;
-                }
+        for (int k = 0; k < 4; ++k) {
+            const int i = i0 + k;
+            m[k] = -INFINITY;
+            li[k] = 0.f;
+            x[k][0] = x[k][1] = float4{};
+            if (i < u.y) {
+                const float* w = partial_slot(p, i == 0 ? u.x : 2 * (u.x / 2 + i));
+                m[k] = w[p.RT * p.D + lr];
+                li[k] = w[p.RT * p.D + p.RT + lr];
+                x[k][0] = *reinterpret_cast<const float4*>(w + (c / 4 * p.RT + lr) * 4);
+                x[k][1] = *reinterpret_cast<const float4*>(w + ((c / 4 + 1) * p.RT + lr) * 4);
             }
         }
-    }
+        const float mx = fmaxf(fmaxf(M, fmaxf(m[0], m[1])), fmaxf(m[2], m[3]));
+        const float g = M == -INFINITY ? 0.f : ex2(M - mx);
+        M = mx;
+        l *= g;
 #pragma unroll
-    for (int d = 16; d > 0; d /= 2) l += __shfl_xor_sync(0xffffffffu, l, d);
+        for (int e = 0; e < 8; ++e) o[e] *= g;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const float f = m[k] == -INFINITY ? 0.f : ex2(m[k] - mx);
+            l += f * li[k];
+            o[0] += f * x[k][0].x;
+            o[1] += f * x[k][0].y;
+            o[2] += f * x[k][0].z;
+            o[3] += f * x[k][0].w;
+            o[4] += f * x[k][1].x;
+            o[5] += f * x[k][1].y;
+            o[6] += f * x[k][1].z;
+            o[7] += f * x[k][1].w;
+        }
+    }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const int d = lane * 4 + 128 * k;
-        if (d < p.D)
-            *reinterpret_cast<uint2*>(out + d) =
-                uint2{E::pack(o[k].x * inv, o[k].y * inv), E::pack(o[k].z * inv, o[k].w * inv)};
-    }
+    const int kvh = unit / p.n_rt % p.Hkv, b = unit / p.n_rt / p.Hkv;
+    const int t = p.by_G.div(r), h = kvh * p.G + r - t * p.G;
+    *reinterpret_cast<uint4*>(p.o + b * p.osb + h * p.osh + t * p.oss + c) =
+        uint4{E::pack(o[0] * inv, o[1] * inv), E::pack(o[2] * inv, o[3] * inv), E::pack(o[4] * inv, o[5] * inv),
+              E::pack(o[6] * inv, o[7] * inv)};
 }
 
 // -------------------------------------------------------- the few-rows kernel
@@ -451,6 +451,10 @@ __device__ __forceinline__ void load_q_chunk(const AttnParams& p, const Segment&
         if (static_cast<unsigned>(pos) >= static_cast<unsigned>(p.rope_rows)) return;
     }
     hi = *reinterpret_cast<const uint4*>(p.q + g.b * p.qsb + (g.kvh * p.G + r - t * p.G) * p.qsh + t * p.qss + ch * 8);
+    hi.x ^= p.flip;
+    hi.y ^= p.flip;
+    hi.z ^= p.flip;
+    hi.w ^= p.flip;
     if (p.cos == nullptr) return;
     const int64_t at = static_cast<int64_t>(pos) * (p.D / 2) + ch * 4;
     const float4 c = __ldg(reinterpret_cast<const float4*>(p.cos + at));
@@ -550,8 +554,10 @@ __device__ __forceinline__ bool produce(const AttnParams& p, const Segment& g, i
 #pragma unroll
                 for (int r = r0, j = 0; j < KT / RSTEP; r += RSTEP, ++j) {
                     const uint32_t d = dst + (RSTEP % 8 == 0 ? dst0 + j * RSTEP * 128 : chunk_off(KT, r, ch));
-                    cp_async16(d, ks + j * RSTEP * p.kc.ss, pol);
-                    cp_async16(d + L::TILE, vs + j * RSTEP * p.vc.ss, pol);
+                    cp_async16(d, ks, pol);
+                    cp_async16(d + L::TILE, vs, pol);
+                    ks += RSTEP * p.kc.ss;
+                    vs += RSTEP * p.vc.ss;
                 }
             }
         } else {
@@ -614,11 +620,15 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
         if (idx % (DP / 8) * 8 >= p.D)
             *reinterpret_cast<uint4*>(ring + idx / (DP / 8) / KT * L::TILE +
                                       chunk_off(KT, idx / (DP / 8) % KT, idx % (DP / 8))) = uint4{0u, 0u, 0u, 0u};
+    warm_params(p);
     __syncthreads();
     grid_dependency_wait();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const Sched sched = make_sched(p, pre);
-    if (sched.total == 0 || static_cast<int>(blockIdx.x) >= sched.ctas) return;
+    if (sched.total == 0 || static_cast<int>(blockIdx.x) >= sched.ctas) {
+        zero_empty_units(p, threadIdx.x, L::THREADS);
+        return;
+    }
     const int begin = cta_begin(sched, blockIdx.x), end = cta_begin(sched, blockIdx.x + 1);
 
     const int wrg = warp % NRG, wtg = warp / NRG;
@@ -632,7 +642,7 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
     bool aborted = false;       // consumers: a wait expired
     int i0 = 0, b = 0;  // running tile number of the segment's first tile
     for (int pos = begin; pos < end;) {
-        const Segment g = segment_at(p, sched, pre, pos, end, b);
+        const Segment g = segment_at(p, pre, pos, end, b);
         if (warp >= NCW) {
             if (!produce<L>(p, g, i0, bars, smem_u32(ring), ab, threadIdx.x - 32 * NCW)) break;
             i0 += g.count;
@@ -729,7 +739,7 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
                             bool see = kr < valid && key >= rlo[ri] && key < rhi[ri];
                             if (p.mask != nullptr && see && key >= g.L)
                                 see = rw[ri][(key - g.L) >> 5] >> ((key - g.L) & 31) & 1u;
-                            if (!see) sc[nt][e] = -INFINITY * (sl2 < 0.f ? -1.f : 1.f);
+                            if (!see) sc[nt][e] = -INFINITY;
                         }
                 }
 #pragma unroll
@@ -819,12 +829,14 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
         }
         named_bar_sync(1, 32 * NCW);
         const bool whole = g.count == g.s.n;
-        float* slot = partial_slot(p, 2 * blockIdx.x + (pos - g.first <= begin ? 0 : 1));
+        float* slot = partial_slot(p, segment_slot(g, pos, begin));
+        if (g.first == 0 && threadIdx.x == 0) describe_unit(p, sched, g, pos, begin);
         const int rows = min(p.RT, p.rows - row0);
         if (!*abort_flag) {
-            for (int idx = threadIdx.x; idx < rows * (DP / 4); idx += 32 * NCW) {
-                const int lr = idx / (DP / 4), c = idx % (DP / 4) * 4;
-                if (c >= p.D) continue;
+            // rows side by side: whole lines of the partial's [D / 4][RT] layout
+            for (int idx = threadIdx.x; idx < p.RT * (DP / 4); idx += 32 * NCW) {
+                const int lr = idx & (p.RT - 1), c = idx / p.RT * 4;
+                if (c >= p.D || lr >= rows) continue;
                 const float* row = part + ((lr / 16) * 16 + lr % 16) * L::PSTR;
                 const int step = NRG * 16 * L::PSTR;
                 float M = -INFINITY;
@@ -847,7 +859,7 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
                     *reinterpret_cast<uint2*>(p.o + g.b * p.osb + (g.kvh * p.G + r - t * p.G) * p.osh + t * p.oss + c) =
                         uint2{E::pack(o.x * inv, o.y * inv), E::pack(o.z * inv, o.w * inv)};
                 } else {
-                    *reinterpret_cast<float4*>(slot + lr * p.D + c) = o;
+                    *reinterpret_cast<float4*>(slot + (c / 4 * p.RT + lr) * 4) = o;
                     if (c == 0) {
                         slot[p.RT * p.D + lr] = M;
                         slot[p.RT * p.D + p.RT + lr] = l;
@@ -859,7 +871,10 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
         i0 += g.count;
         pos += g.count;
     }
-    if (warp >= NCW) cp_async_wait_all();  // after an expired wait too, no copy outlives the CTA
+    if (warp >= NCW)
+        cp_async_wait_all();  // after an expired wait too, no copy outlives the CTA
+    else
+        zero_empty_units(p, threadIdx.x, 32 * NCW);
 }
 
 }  // namespace paged

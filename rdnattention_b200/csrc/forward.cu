@@ -19,6 +19,7 @@
 
 #include "fa_decode.cuh"
 #include "fa_paged.cuh"
+#include "fa_paged_mma.cuh"
 #include "fa_prefill.cuh"
 #include "peer.cuh"
 #include "rope.cuh"

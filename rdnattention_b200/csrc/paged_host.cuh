@@ -2,6 +2,8 @@
 // translation unit that holds every kernel): checks, tensor maps, launches.
 #pragma once
 
+#include <cmath>
+
 namespace rdna {
 namespace {
 
@@ -93,22 +95,24 @@ int launched() {
 // How a paged attention call is cut: rows per tile, key tiles per page.
 struct PagedPlan {
     int dp;     // head_dim rounded up to the kernel's 64, 128 or 256
+    bool mma;   // the tcgen05 kernel's row tiles of 128
     int RT, n_rt, tpp, grid;
+    size_t partials, bytes;  // workspace: bytes of the partials, in all
 };
 
-PagedPlan paged_plan(uint32_t H, uint32_t Hkv, uint32_t T, uint32_t D, uint32_t P) {
+PagedPlan paged_plan(uint32_t B, uint32_t H, uint32_t Hkv, uint32_t T, uint32_t D, uint32_t P) {
     PagedPlan f{};
     f.dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
     const int64_t rows = static_cast<int64_t>(H / Hkv) * T;
-    f.RT = f.dp <= 128 || rows <= 16 ? 16 : 32;
+    f.mma = f.dp <= 128 && rows > 16;
+    f.RT = f.mma ? 128 : f.dp <= 128 || rows <= 16 ? 16 : 32;
     f.n_rt = static_cast<int>((rows + f.RT - 1) / f.RT);
     f.tpp = static_cast<int>(P) >= paged::KT ? (static_cast<int>(P) + paged::KT - 1) / paged::KT : 0;
     f.grid = sm_count();
+    f.partials = align_up(static_cast<size_t>(2) * f.grid * f.RT * (D + 2) * sizeof(float));
+    const size_t seqs = B < static_cast<uint32_t>(paged::kMaxBatch) ? B : paged::kMaxBatch;
+    f.bytes = f.partials + align_up(seqs * Hkv * f.n_rt * sizeof(int2));
     return f;
-}
-
-size_t paged_ws_bytes(const PagedPlan& f, uint32_t D) {
-    return align_up(static_cast<size_t>(2) * f.grid * f.RT * (D + 2) * sizeof(float));
 }
 
 }  // namespace
@@ -182,7 +186,7 @@ size_t pagedAttentionWorkspaceBytes(const PagedAttentionParams& a) {
     if (a.c.numKvHeads == 0 || a.numHeads == 0 || a.numHeads % a.c.numKvHeads != 0 || a.c.headDim == 0 ||
         a.c.headDim > 256 || a.seqLen == 0 || a.c.pageSize == 0)
         return 0;
-    return paged_ws_bytes(paged_plan(a.numHeads, a.c.numKvHeads, a.seqLen, a.c.headDim, a.c.pageSize), a.c.headDim);
+    return paged_plan(a.c.batchSize, a.numHeads, a.c.numKvHeads, a.seqLen, a.c.headDim, a.c.pageSize).bytes;
 }
 
 int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t workspace_bytes, void* stream) {
@@ -205,9 +209,8 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
     if (a.treeMask != nullptr && (a.maskStrideB < 0 || a.maskStrideT < 0)) return pfail("strides must be positive");
     if (const char* e = check_rope(a.rotCos, a.rotSin, a.positions, a.ropeRows)) return pfail(e);
 
-    const PagedPlan f = paged_plan(a.numHeads, c.numKvHeads, a.seqLen, c.headDim, c.pageSize);
-    const size_t need = paged_ws_bytes(f, c.headDim);
-    if (workspace == nullptr || workspace_bytes < need)
+    const PagedPlan f = paged_plan(c.batchSize, a.numHeads, c.numKvHeads, a.seqLen, c.headDim, c.pageSize);
+    if (workspace == nullptr || workspace_bytes < f.bytes)
         return pfail("workspace missing or smaller than rdna_attention_paged_workspace_size()");
     if (reinterpret_cast<uintptr_t>(workspace) & (kWsAlign - 1)) return pfail("workspace must be 256-byte aligned");
 
@@ -242,16 +245,20 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
     p.by_P.set(c.pageSize);
     p.by_tpp.set(f.tpp == 0 ? 1 : static_cast<uint32_t>(f.tpp));
     p.window = a.windowSize > 0 ? a.windowSize : 0;
-    p.scale_log2 = a.scale * 1.4426950408889634f;
+    // (a scale of 0 becomes one whose scores are 0 in fp32)
+    p.scale_log2 = std::fabs(a.scale) * 1.4426950408889634f;
+    if (p.scale_log2 < 1e-30f) p.scale_log2 = 1e-30f;
+    p.flip = a.scale < 0.f ? 0x80008000u : 0u;
     p.ws = static_cast<float*>(workspace);
+    p.units = reinterpret_cast<int2*>(static_cast<char*>(workspace) + f.partials);
     p.grid = f.grid;
 
     // the list positions of one launch are 32-bit: as many sequences per launch as surely fit
     const int64_t tiles = f.tpp == 0 ? (static_cast<int64_t>(c.maxPages) * c.pageSize + paged::KT - 1) / paged::KT
                                      : static_cast<int64_t>(c.maxPages) * f.tpp;
     const int64_t per_seq = tiles * p.n_rt * p.Hkv;
-    const int64_t join_rows = static_cast<int64_t>(p.Hkv) * p.n_rt * ((f.RT + paged::kJoinWarps - 1) / paged::kJoinWarps);
-    const int64_t fit = INT32_MAX / (per_seq > join_rows ? per_seq : join_rows);
+    const int64_t join_blocks = static_cast<int64_t>(p.Hkv) * p.n_rt * ((f.RT + paged::kJoinRows - 1) / paged::kJoinRows);
+    const int64_t fit = INT32_MAX / (per_seq > join_blocks ? per_seq : join_blocks);
     if (fit == 0) return pfail("problem too large for one launch");
     const int64_t step = fit < paged::kMaxBatch ? fit : paged::kMaxBatch;
 
@@ -277,9 +284,17 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
         cfg.numAttrs = 1;
         cfg.stream = st;
         cfg.gridDim = dim3(static_cast<unsigned>(f.grid));
-        auto launch = [&](auto kern, int threads, int smem) {
+        // regs != 0: the kernel moves registers between its warps and must have been given
+        // exactly that many per thread (an increase waits for registers the CTA has)
+        auto launch = [&](auto kern, int threads, int smem, int regs) {
             cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
             if (ce != cudaSuccess) return ce;
+            if (regs != 0) {
+                cudaFuncAttributes fa{};
+                ce = cudaFuncGetAttributes(&fa, kern);
+                if (ce != cudaSuccess) return ce;
+                if (fa.numRegs != regs) return cudaErrorInvalidKernelImage;
+            }
             cfg.blockDim = dim3(threads);
             cfg.dynamicSmemBytes = smem;
             return launch_timed(st, [&] { return cudaLaunchKernelEx(&cfg, kern, s); });
@@ -289,17 +304,22 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
             using L64 = paged::Layout<64>;
             using L128 = paged::Layout<128>;
             using L256 = paged::Layout<256>;
+            using M64 = paged::MmaLayout<64>;
+            using M128 = paged::MmaLayout<128>;
+            if (f.mma)
+                return f.dp == 64 ? launch(paged::fa_paged_mma_kernel<T, 64>, M64::THREADS, M64::SMEM_BYTES, M64::LAUNCH_REGS)
+                                  : launch(paged::fa_paged_mma_kernel<T, 128>, M128::THREADS, M128::SMEM_BYTES, M128::LAUNCH_REGS);
             switch (f.dp) {
-                case 64: return launch(paged::fa_paged_kernel<T, 64>, L64::THREADS, L64::SMEM_BYTES);
-                case 128: return launch(paged::fa_paged_kernel<T, 128>, L128::THREADS, L128::SMEM_BYTES);
-                default: return launch(paged::fa_paged_kernel<T, 256>, L256::THREADS, L256::SMEM_BYTES);
+                case 64: return launch(paged::fa_paged_kernel<T, 64>, L64::THREADS, L64::SMEM_BYTES, 0);
+                case 128: return launch(paged::fa_paged_kernel<T, 128>, L128::THREADS, L128::SMEM_BYTES, 0);
+                default: return launch(paged::fa_paged_kernel<T, 256>, L256::THREADS, L256::SMEM_BYTES, 0);
             }
         };
         cudaError_t ce = c.dtype == paged::DT_F16 ? by_width(paged::F16{}) : by_width(paged::BF16{});
         if (ce == cudaSuccess) ce = cudaGetLastError();
         if (ce != cudaSuccess) return fail(g_err_paged, "%s", cudaGetErrorString(ce));
-        cfg.gridDim = dim3(static_cast<unsigned>(s.B * join_rows));
-        cfg.blockDim = dim3(32 * paged::kJoinWarps);
+        cfg.gridDim = dim3(static_cast<unsigned>(s.B * join_blocks));
+        cfg.blockDim = dim3(paged::kJoinRows * (c.headDim / 8));
         cfg.dynamicSmemBytes = 0;
         ce = c.dtype == paged::DT_F16 ? cudaLaunchKernelEx(&cfg, paged::join_kernel<paged::F16>, s)
                                       : cudaLaunchKernelEx(&cfg, paged::join_kernel<paged::BF16>, s);
