@@ -11,10 +11,10 @@
 // Rows t >= n and rows that see nothing are written as zeros.
 //
 // Work: a unit = (sequence, KV head, tile of RT rows) times the key tiles that
-// some row of it sees.  The tiles of all units form one list, and CTA c takes
-// the c-th equal part of it: every CTA streams the same number of bytes whatever
-// the lengths are, and the lengths stay on the device (a captured graph replays
-// with new ones).  A unit that lies inside one CTA is finished there; the parts
+// some row of it sees.  The tiles of all units, each unit's led by W positions for
+// what starting a unit costs, form one list, and CTA c takes the c-th equal part of
+// it: every CTA has the same time's work whatever the lengths are, and the lengths
+// stay on the device (a captured graph replays with new ones).  A unit that lies inside one CTA is finished there; the parts
 // of the others go to a workspace as (O, m, l) in fp32 and the combine kernel
 // joins them in list order, so results do not depend on timing.
 #pragma once
@@ -29,8 +29,8 @@ namespace paged {
 
 constexpr int kMaxTree = 256;          // drafted tokens under a mask
 constexpr int kMaxBatch = 1024;        // sequences per launch (the host splits larger batches)
-constexpr int kMinTiles = 2;           // tiles per CTA below which fewer CTAs take part
 constexpr int KT = 64;                 // keys per tile
+constexpr int kLead = 3, kLeadMma = 4; // AttnParams::W of the two kernels
 
 // n / d for n < 2^31 by a multiplication: with l = ceil(log2 d) and m =
 // floor(2^(31 + l) / d) + 1, m d exceeds 2^(31 + l) by at most 2^l, so the error
@@ -60,7 +60,7 @@ struct AttnParams {
     const float *cos, *sin;
     int rope_rows;
     int B, H, Hkv, G, D;
-    FastDiv by_G;
+    FastDiv by_G, by_Hkv;
     int rows;    // T * G
     int RT;      // rows per tile
     int n_rt;    // row tiles
@@ -73,6 +73,7 @@ struct AttnParams {
     float* ws;   // partials: 2 per CTA, each O [D / 4][RT] float4, m [RT], l [RT]
     int2* units; // per unit (b, kvh, rt): first partial's slot, number of parts (0 or 1: nothing to join)
     int grid;    // CTAs of the attention kernel
+    int W;       // list positions that a unit costs besides its tiles
 };
 
 // Touches every line of the parameters once (one word per lane and 64 bytes), so that
@@ -114,14 +115,18 @@ __device__ __forceinline__ Span row_tile_span(const AttnParams& p, int L, int n,
 
 // The list of a launch: pre[b] (shared memory) = list position behind sequence b.
 struct Sched {
-    int total;  // tiles of the launch
+    int total;  // positions of the launch
     int ctas;   // CTAs that take part
-    int q, r;   // the first r of them take q + 1 tiles, the others q
+    int q, r;   // the first r of them take q + 1 positions, the others q
 };
 
-__device__ __forceinline__ int head_tiles(const AttnParams& p, int L, int n) {
+// Positions of one KV head of a sequence.
+__device__ __forceinline__ int head_cost(const AttnParams& p, int L, int n) {
     int w = 0;
-    for (int rt = 0; rt < p.n_rt; ++rt) w += row_tile_span(p, L, n, rt).n;
+    for (int rt = 0; rt < p.n_rt; ++rt) {
+        const int tiles = row_tile_span(p, L, n, rt).n;
+        w += tiles > 0 ? p.W + tiles : 0;
+    }
     return w;
 }
 
@@ -142,14 +147,14 @@ __device__ __forceinline__ Sched make_sched(const AttnParams& p, int* pre) {
     Sched s;
     if (p.B <= 32) {
         int v = 0;
-        if (lane < p.B) v = head_tiles(p, p.t.len(lane), p.t.news(lane)) * p.Hkv;
+        if (lane < p.B) v = head_cost(p, p.t.len(lane), p.t.news(lane)) * p.Hkv;
         v = warp_scan(v, lane);
         if (lane < p.B) pre[lane] = v;
         s.total = __shfl_sync(0xffffffffu, v, 31);
         __syncwarp();
     } else {
         for (int b = threadIdx.x; b < p.B; b += blockDim.x)
-            pre[b] = head_tiles(p, p.t.len(b), p.t.news(b)) * p.Hkv;
+            pre[b] = head_cost(p, p.t.len(b), p.t.news(b)) * p.Hkv;
         __syncthreads();
         if (threadIdx.x < 32) {
             int carry = 0;
@@ -163,8 +168,7 @@ __device__ __forceinline__ Sched make_sched(const AttnParams& p, int* pre) {
         __syncthreads();
         s.total = pre[p.B - 1];
     }
-    // below kMinTiles tiles for each CTA fewer of them take part
-    s.ctas = min(p.grid, max(1, s.total / kMinTiles));
+    s.ctas = min(p.grid, max(1, s.total));
     s.q = s.total / s.ctas;
     s.r = s.total - s.q * s.ctas;
     return s;
@@ -177,12 +181,14 @@ __device__ __forceinline__ int cta_of(const Sched& s, int pos) {
     return pos < wide ? pos / (s.q + 1) : s.r + (pos - wide) / s.q;
 }
 
-// One unit's share of a CTA: list positions [pos, pos + count) are the unit's
-// tiles first .. first + count - 1.
+// One unit's share of a CTA: its tiles first .. first + count - 1 (count may be 0: only
+// the unit's lead lies in the CTA).
 struct Segment {
     int b, kvh, rt, L, n;
     Span s;
     int first, count;
+    int pos0;  // list position of the unit's tile 0
+    int next;  // list position behind the segment
 };
 
 // The segment at list position pos < total (a whole warp; b: a sequence at or
@@ -200,17 +206,20 @@ __device__ __forceinline__ Segment segment_at(const AttnParams& p, const int* pr
     g.b = b;
     g.L = p.t.len(b);
     g.n = p.t.news(b);
-    const int start = b > 0 ? pre[b - 1] : 0, head = (pre[b] - start) / p.Hkv;
+    const int start = b > 0 ? pre[b - 1] : 0, head = p.by_Hkv.div(pre[b] - start);
     int off = pos - start;
     g.kvh = off / head;
     off -= g.kvh * head;
     for (g.rt = 0;; ++g.rt) {
         g.s = row_tile_span(p, g.L, g.n, g.rt);
-        if (off < g.s.n) break;
-        off -= g.s.n;
+        const int cost = g.s.n > 0 ? p.W + g.s.n : 0;
+        if (off < cost) break;
+        off -= cost;
     }
-    g.first = off;
-    g.count = min(g.s.n - off, end - pos);
+    g.pos0 = pos - off + p.W;
+    g.first = max(0, off - p.W);
+    g.count = max(0, min(g.s.n - g.first, end - g.pos0 - g.first));
+    g.next = min(g.pos0 + g.first + g.count, end);
     return g;
 }
 
@@ -235,14 +244,13 @@ __device__ __forceinline__ int unit_index(const AttnParams& p, int b, int kvh, i
 }
 // The slot of a segment's partial: a CTA starts with at most one unit that began before it
 // (or with it) and ends with at most one other that goes on.
-__device__ __forceinline__ int segment_slot(const Segment& g, int pos, int begin) {
-    return 2 * static_cast<int>(blockIdx.x) + (pos - g.first <= begin ? 0 : 1);
+__device__ __forceinline__ int segment_slot(const Segment& g, int begin) {
+    return 2 * static_cast<int>(blockIdx.x) + (g.pos0 <= begin ? 0 : 1);
 }
 // What the join needs to know about a unit, from the CTA that holds its first tile.
-__device__ __forceinline__ void describe_unit(const AttnParams& p, const Sched& sc, const Segment& g, int pos,
-                                              int begin) {
-    const int parts = g.count == g.s.n ? 1 : cta_of(sc, pos + g.s.n - 1) - static_cast<int>(blockIdx.x) + 1;
-    p.units[unit_index(p, g.b, g.kvh, g.rt)] = make_int2(segment_slot(g, pos, begin), parts);
+__device__ __forceinline__ void describe_unit(const AttnParams& p, const Sched& sc, const Segment& g, int begin) {
+    const int parts = g.count == g.s.n ? 1 : cta_of(sc, g.pos0 + g.s.n - 1) - static_cast<int>(blockIdx.x) + 1;
+    p.units[unit_index(p, g.b, g.kvh, g.rt)] = make_int2(segment_slot(g, begin), parts);
 }
 
 // Row tiles that see no key belong to no CTA's list: their output rows are zeroed, and
@@ -301,61 +309,84 @@ __device__ __forceinline__ void build_mask(const AttnParams& p, const Segment& g
 }
 
 // ------------------------------------------------------------- the join kernel
-// O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a split unit's parts, in list
-// order.  A block takes 16 rows; a thread one row (lanes side by side, so the partials
-// are read in whole lines) and 8 columns.  Bound by the latency of three dependent reads
-// (the unit, its parts, the store); four parts' loads are in flight at a time.
+// O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a split unit's parts, always in
+// the same order.  A block takes 16 rows; a thread one row (lanes side by side, so the
+// partials are read in whole lines), 8 columns and every n-th part, n = blockDim / (2 D)
+// (2 D threads cover the rows and columns); the n shares join in shared memory.  Bound
+// by the latency of dependent reads (the unit, its parts), so eight parts' loads are in
+// flight at a time.
 constexpr int kJoinRows = 16;
+constexpr int kJoinThreads = 512;
+constexpr int kJoinFlight = 8;
 
 template <class E>
-__global__ void __launch_bounds__(512) join_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttnParams p) {
+    extern __shared__ float joined[];  // [n - 1][10][2 D]
     const int groups = (p.RT + kJoinRows - 1) / kJoinRows;
     const int unit = blockIdx.x / groups;
-    const int lr = blockIdx.x % groups * kJoinRows + threadIdx.x % kJoinRows;  // row of the tile
-    const int c = threadIdx.x / kJoinRows * 8;                                 // first column
+    const int width = 2 * p.D, n = blockDim.x / width, split = threadIdx.x / width, tid = threadIdx.x - split * width;
+    const int lr = blockIdx.x % groups * kJoinRows + tid % kJoinRows;  // row of the tile
+    const int c = tid / kJoinRows * 8;                                 // first column
     grid_dependency_wait();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int2 u = p.units[unit];
     const int rt = unit % p.n_rt, r = rt * p.RT + lr;
-    if (u.y < 2 || r >= p.rows) return;
+    if (u.y < 2) return;
     float M = -INFINITY, l = 0.f;
     float o[8] = {};
-    for (int i0 = 0; i0 < u.y; i0 += 4) {
-        float m[4], li[4];
-        float4 x[4][2];
+    auto add = [&](float m, float li, const float* x, float mx) {
+        const float f = m == -INFINITY ? 0.f : ex2(m - mx);
+        l += f * li;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int i = i0 + k;
-            m[k] = -INFINITY;
-            li[k] = 0.f;
-            x[k][0] = x[k][1] = float4{};
-            if (i < u.y) {
-                const float* w = partial_slot(p, i == 0 ? u.x : 2 * (u.x / 2 + i));
-                m[k] = w[p.RT * p.D + lr];
-                li[k] = w[p.RT * p.D + p.RT + lr];
-                x[k][0] = *reinterpret_cast<const float4*>(w + (c / 4 * p.RT + lr) * 4);
-                x[k][1] = *reinterpret_cast<const float4*>(w + ((c / 4 + 1) * p.RT + lr) * 4);
-            }
-        }
-        const float mx = fmaxf(fmaxf(M, fmaxf(m[0], m[1])), fmaxf(m[2], m[3]));
+        for (int e = 0; e < 8; ++e) o[e] += f * x[e];
+    };
+    auto rescale = [&](float mx) {
         const float g = M == -INFINITY ? 0.f : ex2(M - mx);
         M = mx;
         l *= g;
 #pragma unroll
         for (int e = 0; e < 8; ++e) o[e] *= g;
+    };
+    for (int i0 = split; i0 < u.y; i0 += kJoinFlight * n) {
+        float m[kJoinFlight], li[kJoinFlight], x[kJoinFlight][8];
+        float mx = M;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float f = m[k] == -INFINITY ? 0.f : ex2(m[k] - mx);
-            l += f * li[k];
-            o[0] += f * x[k][0].x;
-            o[1] += f * x[k][0].y;
-            o[2] += f * x[k][0].z;
-            o[3] += f * x[k][0].w;
-            o[4] += f * x[k][1].x;
-            o[5] += f * x[k][1].y;
-            o[6] += f * x[k][1].z;
-            o[7] += f * x[k][1].w;
+        for (int k = 0; k < kJoinFlight; ++k) {
+            const int i = i0 + k * n;
+            m[k] = -INFINITY;
+            li[k] = 0.f;
+            if (i < u.y) {
+                const float* w = partial_slot(p, i == 0 ? u.x : 2 * (u.x / 2 + i));
+                m[k] = w[p.RT * p.D + lr];
+                li[k] = w[p.RT * p.D + p.RT + lr];
+                *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(w + (c / 4 * p.RT + lr) * 4);
+                *reinterpret_cast<float4*>(x[k] + 4) = *reinterpret_cast<const float4*>(w + ((c / 4 + 1) * p.RT + lr) * 4);
+            }
         }
+#pragma unroll
+        for (int k = 0; k < kJoinFlight; ++k) mx = fmaxf(mx, m[k]);
+        rescale(mx);
+#pragma unroll
+        for (int k = 0; k < kJoinFlight; ++k)
+            if (i0 + k * n < u.y) add(m[k], li[k], x[k], M);
+    }
+    if (split > 0) {
+        float* s = joined + (split - 1) * 10 * width + tid;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[e * width] = o[e];
+        s[8 * width] = M;
+        s[9 * width] = l;
+    }
+    __syncthreads();
+    if (split > 0 || r >= p.rows) return;
+    for (int k = 1; k < n; ++k) {
+        const float* s = joined + (k - 1) * 10 * width + tid;
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = s[e * width];
+        const float m = s[8 * width];
+        rescale(fmaxf(M, m));
+        add(m, s[9 * width], x, M);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int kvh = unit / p.n_rt % p.Hkv, b = unit / p.n_rt / p.Hkv;
@@ -392,10 +423,14 @@ struct Layout {
     static constexpr int OFF_RING = 1024;
     static constexpr int OFF_Q = OFF_RING + NST * STAGE;  // hi, lo: [RT][DP], swizzled like a K tile
     static constexpr int Q_BYTES = NBOX * MAX_RT * 128;
+    // what a segment needs besides its tiles, NQ times (the producers fill the next one's)
+    static constexpr int NQ = DP <= 128 ? 2 : 1;
     static constexpr bool ALIAS = DP > 128;               // the partials take Q's place
-    static constexpr int OFF_PART = ALIAS ? OFF_Q : OFF_Q + 2 * Q_BYTES;  // [NCW][16][PSTR] fp32
-    static constexpr int OFF_MASK = OFF_PART + NCW * 16 * PSTR * 4;       // [RT][kMaxTree / 32], then [RT]
-    static constexpr int OFF_PRE = OFF_MASK + MAX_RT * (kMaxTree / 32) * 4 + MAX_RT * 4;
+    static constexpr int OFF_PART = ALIAS ? OFF_Q : OFF_Q + NQ * 2 * Q_BYTES;  // [NCW][16][PSTR] fp32
+    static constexpr int OFF_MASK = OFF_PART + NCW * 16 * PSTR * 4;  // [NQ] of: bits [RT][kMaxTree / 32], ctx_lo [RT],
+    static constexpr int MASK_BYTES = MAX_RT * (kMaxTree / 32) * 4 + MAX_RT * 4 + MAX_RT * 8;  // limits [RT]
+    static constexpr int OFF_PRE = OFF_MASK + NQ * MASK_BYTES;
+    static constexpr int Q_FULL = 2 * NST, Q_EMPTY = Q_FULL + NQ, OFF_ABORT = 8 * (Q_EMPTY + NQ);  // barriers
     static constexpr int SMEM_BYTES = OFF_PRE + kMaxBatch * 4 + 1024;  // + alignment slack
     static_assert(!ALIAS || NCW * 16 * PSTR * 4 >= 2 * Q_BYTES, "Q fits below the partials");
     static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
@@ -519,8 +554,8 @@ __device__ __forceinline__ bool produce(const AttnParams& p, const Segment& g, i
     const int lane = ptid & 31, ch = ptid % NCH, r0 = ptid / NCH;
     const bool col = ch * 8 < p.D;              // the columns behind head_dim stay zero
     const int* pages = p.t.pages + g.b * p.t.stride;
-    const uint16_t* kbase = p.kc.p + g.kvh * p.kc.sh + ch * 8;
-    const uint16_t* vbase = p.vc.p + g.kvh * p.vc.sh + ch * 8;
+    char* const kbase = p.kc.head(g.kvh, ch);
+    char* const vbase = p.vc.head(g.kvh, ch);
     const uint32_t dst0 = chunk_off(KT, r0, ch);  // (8 rows further the swizzle is the same)
     const int shift = p.tpp == 0 ? p.t.Pshift : 31;           // row of the tile -> page of the tile
     const int mask = p.tpp == 0 ? p.t.Pmask : KT - 1;          // and row within it
@@ -548,26 +583,26 @@ __device__ __forceinline__ bool produce(const AttnParams& p, const Segment& g, i
         if (inner && p.tpp != 0) {
             // a tile inside one page
             const int page = __shfl_sync(0xffffffffu, ids, lp & 31);
-            const uint16_t* ks = kbase + page * p.kc.sp + (sub + r0) * p.kc.ss;
-            const uint16_t* vs = vbase + page * p.vc.sp + (sub + r0) * p.vc.ss;
+            const char* ks = p.kc.at(kbase, page, sub + r0);
+            const char* vs = p.vc.at(vbase, page, sub + r0);
             if (col) {
 #pragma unroll
                 for (int r = r0, j = 0; j < KT / RSTEP; r += RSTEP, ++j) {
                     const uint32_t d = dst + (RSTEP % 8 == 0 ? dst0 + j * RSTEP * 128 : chunk_off(KT, r, ch));
                     cp_async16(d, ks, pol);
                     cp_async16(d + L::TILE, vs, pol);
-                    ks += RSTEP * p.kc.ss;
-                    vs += RSTEP * p.vc.ss;
+                    ks += static_cast<uint64_t>(p.kc.ss) * RSTEP;
+                    vs += static_cast<uint64_t>(p.vc.ss) * RSTEP;
                 }
             }
         } else {
-#pragma unroll
+#pragma unroll 4
             for (int r = r0, j = 0; j < KT / RSTEP; r += RSTEP, ++j) {
                 const int page = __shfl_sync(0xffffffffu, ids, (lp + (r >> shift)) & 31);
                 const uint32_t d = dst + (RSTEP % 8 == 0 ? dst0 + j * RSTEP * 128 : chunk_off(KT, r, ch));
                 const int row = sub + (r & mask);
-                const uint16_t* ks = kbase + page * p.kc.sp + row * p.kc.ss;
-                const uint16_t* vs = vbase + page * p.vc.sp + row * p.vc.ss;
+                const char* ks = p.kc.at(kbase, page, row);
+                const char* vs = p.vc.at(vbase, page, row);
                 if (!col) continue;
                 if (inner) {
                     cp_async16(d, ks, pol);
@@ -596,12 +631,12 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
     using L = Layout<DP>;
     constexpr int NCW = L::NCW;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset keeps the address space known)
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t bars = smem_u32(smem);
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (L::NST + s); };
-    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + 16 * L::NST);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::OFF_ABORT);
     const Abort ab{abort_flag};
     uint8_t* ring = smem + L::OFF_RING;
     int* pre = reinterpret_cast<int*>(smem + L::OFF_PRE);
@@ -613,9 +648,14 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
             mbar_init(full_bar(s), 32 * L::NPW);
             mbar_init(empty_bar(s), NRG * min(2, NTG));
         }
+        for (int k = 0; k < L::NQ; ++k) {
+            mbar_init(bars + 8u * (L::Q_FULL + k), 32 * L::NPW);
+            mbar_init(bars + 8u * (L::Q_EMPTY + k), 1);
+        }
         fence_barrier_init();
     }
     // columns behind head_dim are never copied: zero for good
+    if (p.D < DP)
     for (int idx = threadIdx.x; idx < 2 * L::NST * KT * (DP / 8); idx += L::THREADS)
         if (idx % (DP / 8) * 8 >= p.D)
             *reinterpret_cast<uint4*>(ring + idx / (DP / 8) / KT * L::TILE +
@@ -633,40 +673,54 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
 
     const int wrg = warp % NRG, wtg = warp / NRG;
     const int gq = lane >> 2, tq = lane & 3;
-    uint32_t* words = reinterpret_cast<uint32_t*>(smem + L::OFF_MASK);
-    int* ctx_lo = reinterpret_cast<int*>(smem + L::OFF_MASK + L::MAX_RT * (kMaxTree / 32) * 4);
     const int nw = (p.t.T + 31) / 32;
-    const uint32_t qs = smem_u32(smem + L::OFF_Q);
     float* part = reinterpret_cast<float*>(smem + L::OFF_PART);
     const float sl2 = p.scale_log2;
-    bool aborted = false;       // consumers: a wait expired
-    int i0 = 0, b = 0;  // running tile number of the segment's first tile
+    bool aborted = false;    // consumers: a wait expired
+    int i0 = 0, b = 0, nseg = 0;  // running tile number of the segment's first tile; segments so far
     for (int pos = begin; pos < end;) {
         const Segment g = segment_at(p, pre, pos, end, b);
+        pos = g.next;
+        if (g.count == 0) continue;
+        const int row0 = g.rt * p.RT, ta = p.by_G.div(row0);
+        const int qb = nseg % L::NQ, qn = nseg / L::NQ;
+        ++nseg;
+        uint8_t* qmem = smem + L::OFF_Q + qb * 2 * L::Q_BYTES;
+        uint32_t* words = reinterpret_cast<uint32_t*>(smem + L::OFF_MASK + qb * L::MASK_BYTES);
+        int* ctx_lo = reinterpret_cast<int*>(words + L::MAX_RT * (kMaxTree / 32));
+        int2* limits = reinterpret_cast<int2*>(ctx_lo + L::MAX_RT);
         if (warp >= NCW) {
-            if (!produce<L>(p, g, i0, bars, smem_u32(ring), ab, threadIdx.x - 32 * NCW)) break;
+            // Q of the row tile (turned, hi and lo), the mask bits and the rows' limits, then the tiles
+            const int ptid = threadIdx.x - 32 * NCW;
+            if (!__all_sync(0xffffffffu, mbar_wait(bars + 8u * (L::Q_EMPTY + qb), (qn & 1) ^ 1, ab, 0x603))) break;
+            for (int idx = ptid; idx < p.RT * (DP / 8); idx += 32 * L::NPW) {
+                const int r = idx / (DP / 8), ch = idx % (DP / 8);
+                uint4 hi, lo;
+                load_q_chunk<E>(p, g, row0 + r, ch, hi, lo);
+                *reinterpret_cast<uint4*>(qmem + chunk_off(p.RT, r, ch)) = hi;
+                *reinterpret_cast<uint4*>(qmem + L::Q_BYTES + chunk_off(p.RT, r, ch)) = lo;
+            }
+            if (p.mask != nullptr) {
+                build_mask(p, g, words, ctx_lo, ptid, 32 * L::NPW);
+                named_bar_sync(2, 32 * L::NPW);
+            }
+            if (ptid < p.RT) row_limits(p, g, row0 + ptid, ta, ctx_lo, limits[ptid].x, limits[ptid].y);
+            mbar_arrive(bars + 8u * (L::Q_FULL + qb));
+            if (!produce<L>(p, g, i0, bars, smem_u32(ring), ab, ptid)) break;
             i0 += g.count;
-            pos += g.count;
             continue;
         }
         // ------------------------------------------------------------ consumers
-        const int row0 = g.rt * p.RT, ta = p.by_G.div(row0);
-        // Q of the row tile (turned, hi and lo) into shared memory, and the mask bits
-        for (int idx = threadIdx.x; idx < p.RT * (DP / 8); idx += 32 * NCW) {
-            const int r = idx / (DP / 8), ch = idx % (DP / 8);
-            uint4 hi, lo;
-            load_q_chunk<E>(p, g, row0 + r, ch, hi, lo);
-            *reinterpret_cast<uint4*>(smem + L::OFF_Q + chunk_off(p.RT, r, ch)) = hi;
-            *reinterpret_cast<uint4*>(smem + L::OFF_Q + L::Q_BYTES + chunk_off(p.RT, r, ch)) = lo;
-        }
-        if (p.mask != nullptr) build_mask(p, g, words, ctx_lo, threadIdx.x, 32 * NCW);
-        named_bar_sync(1, 32 * NCW);
+        if (!aborted && !__all_sync(0xffffffffu, mbar_wait(bars + 8u * (L::Q_FULL + qb), qn & 1, ab, 0x604)))
+            aborted = true;
+        const uint32_t qs = smem_u32(qmem);
         int rlo[2], rhi[2];
         const uint32_t* rw[2];
         for (int e = 0; e < 2; ++e) {
-            const int r = row0 + wrg * 16 + gq + 8 * e, t = p.by_G.div(r);
-            row_limits(p, g, r, ta, ctx_lo, rlo[e], rhi[e]);
-            rw[e] = words + (r < p.rows && t < g.n ? (t - ta) * nw : 0);
+            const int lr = wrg * 16 + gq + 8 * e, t = p.by_G.div(row0 + lr);
+            rlo[e] = limits[lr].x;
+            rhi[e] = limits[lr].y;
+            rw[e] = words + (rlo[e] < rhi[e] ? (t - ta) * nw : 0);
         }
         // keys in [all_lo, all_hi) are seen by every row of the group that sees any; what the
         // others (padding, empty) add up there is dropped at the end of the segment
@@ -829,8 +883,8 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
         }
         named_bar_sync(1, 32 * NCW);
         const bool whole = g.count == g.s.n;
-        float* slot = partial_slot(p, segment_slot(g, pos, begin));
-        if (g.first == 0 && threadIdx.x == 0) describe_unit(p, sched, g, pos, begin);
+        float* slot = partial_slot(p, segment_slot(g, begin));
+        if (g.first == 0 && threadIdx.x == 0) describe_unit(p, sched, g, begin);
         const int rows = min(p.RT, p.rows - row0);
         if (!*abort_flag) {
             // rows side by side: whole lines of the partial's [D / 4][RT] layout
@@ -868,8 +922,8 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
             }
         }
         named_bar_sync(1, 32 * NCW);  // the partials, Q and mask areas are free again
+        if (threadIdx.x == 0) mbar_arrive(bars + 8u * (L::Q_EMPTY + qb));
         i0 += g.count;
-        pos += g.count;
     }
     if (warp >= NCW)
         cp_async_wait_all();  // after an expired wait too, no copy outlives the CTA

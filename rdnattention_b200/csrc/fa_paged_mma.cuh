@@ -32,7 +32,7 @@ struct MmaLayout {
     static constexpr int THREADS = 32 * (NSW + NPW + 4);
     // Registers: launched with LAUNCH_REGS per thread (16 warps fill the register file),
     // moved to the softmax warps, which hold 64 scores each.
-    static constexpr int LAUNCH_REGS = 128, SOFTMAX_REGS = 168, OTHER_REGS = 88;
+    static constexpr int LAUNCH_REGS = 128, SOFTMAX_REGS = 160, OTHER_REGS = 96;
     static_assert(NSW * SOFTMAX_REGS + (NPW + 4) * OTHER_REGS <= (NSW + NPW + 4) * LAUNCH_REGS,
                   "register split exceeds the launch allocation");
     static constexpr int NBOX = DP / 64;
@@ -50,7 +50,9 @@ struct MmaLayout {
     static constexpr int OFF_RING = 1024;
     static constexpr int OFF_MASK = OFF_RING + NST * STAGE;  // [RT][NW + 2] (two words of padding), then [RT]
     static constexpr int OFF_ML = OFF_MASK + RT * NW * 4 + RT * 4;  // [2][RT] (m, l)
-    static constexpr int OFF_PRE = OFF_ML + 2 * RT * 8;
+    static constexpr int OFF_SEG = OFF_ML + 2 * RT * 8;  // [NSW] Segment
+    static constexpr int OFF_PRE = OFF_SEG + NSW * 64;
+    static_assert(sizeof(Segment) <= 64, "a segment's slot");
     static constexpr int SMEM_BYTES = OFF_PRE + kMaxBatch * 4 + 1024;  // + alignment slack
     static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
     // TMEM columns
@@ -103,7 +105,7 @@ template <class E, int DP>
 __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel(const __grid_constant__ AttnParams p) {
     using L = MmaLayout<DP>;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset keeps the address space known)
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t bars = smem_u32(smem);
     auto bar = [&](int i) { return bars + 8u * i; };
@@ -127,6 +129,7 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
         fence_barrier_init();
     }
     // columns behind head_dim are never copied: zero for good
+    if (p.D < DP)
     for (int idx = threadIdx.x; idx < 2 * L::NST * KT * (DP / 8); idx += L::THREADS)
         if (idx % (DP / 8) * 8 >= p.D)
             *reinterpret_cast<uint4*>(ring + idx / (DP / 8) / KT * L::TILE +
@@ -160,7 +163,7 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
             const Segment g = segment_at(p, pre, pos, end, b);
             if (!produce<L>(p, g, i0, bars, smem_u32(ring), ab, threadIdx.x - 32 * L::NSW)) break;
             i0 += g.count;
-            pos += g.count;
+            pos = g.next;
         }
         cp_async_wait_all();  // after an expired wait too, no copy outlives the CTA
     } else if (warp >= L::NSW + L::NPW) {
@@ -213,7 +216,7 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
                 }
                 ok = __shfl_sync(0xffffffffu, ok, 0);
                 i0 += g.count;
-                pos += g.count;
+                pos = g.next;
             }
             if (lane == 0) {
                 // nothing of this thread's is in flight when the TMEM goes
@@ -240,7 +243,18 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
             return !aborted;
         };
         for (int pos = begin; pos < end;) {
-            const Segment g = segment_at(p, pre, pos, end, b);
+            // (each warp keeps its segment in shared memory: registers are for the scores)
+            Segment& g = reinterpret_cast<Segment*>(smem + L::OFF_SEG)[warp];
+            {
+                const Segment found = segment_at(p, pre, pos, end, b);
+                if (lane == 0) g = found;
+                __syncwarp();
+                pos = found.next;
+            }
+            if (g.count == 0) {
+                __syncwarp();
+                continue;
+            }
             const int row0 = g.rt * p.RT, ta = p.by_G.div(row0), r = row0 + lr;
             {
                 // this row's Q, half of the columns each group, turned and split, into TMEM
@@ -284,20 +298,21 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
             int all_hi = __reduce_min_sync(0xffffffffu, dead ? INT_MAX : rhi);
             if (p.mask != nullptr) all_hi = min(all_hi, g.L);
             float m = -INFINITY, l = 0.f;
+            const int behind = i0 + g.count, tile0 = g.s.t0 + g.first - i0, L0 = g.L;
             const int first = i0 + ((w - i0) & 1);
-            for (int i = first; i < i0 + g.count; i += 2, ++n) {
+            for (int i = first; i < behind; i += 2, ++n) {
                 if (!wait(L::S_FULL + w, n & 1, 0x701)) continue;
                 if (!idle) {
                     tc_fence_after();
                     int k0, valid;
-                    tile_keys(p, g.s.t0 + g.first + (i - i0), k0, valid);
+                    tile_keys(p, tile0 + i, k0, valid);
                     uint32_t raw[KT];
                     tmem_ld_x64(tS, raw);
                     float* x = reinterpret_cast<float*>(raw);
                     if (valid < KT || k0 < all_lo || k0 + KT > all_hi) {
                         uint64_t see = bits_between(rlo - k0, min(rhi - k0, valid));
-                        if (p.mask != nullptr && k0 + KT > g.L)
-                            see &= bits_between(0, g.L - k0) | draft_bits(words + rw, nw, k0 - g.L);
+                        if (p.mask != nullptr && k0 + KT > L0)
+                            see &= bits_between(0, L0 - k0) | draft_bits(words + rw, nw, k0 - L0);
                         const uint32_t see0 = static_cast<uint32_t>(see), see1 = static_cast<uint32_t>(see >> 32);
 #pragma unroll
                         for (int c = 0; c < 32; ++c) {
@@ -332,17 +347,17 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
                     const uint64_t mul2 = f2(sl2, sl2), nm2 = f2(nm, nm);
                     uint64_t ls[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-                    for (int c0 = 0; c0 < KT; c0 += 32) {
-                        uint32_t pk[16];
+                    for (int c0 = 0; c0 < KT; c0 += 16) {
+                        uint32_t pk[8];
 #pragma unroll
-                        for (int c = 0; c < 32; c += 2) {
+                        for (int c = 0; c < 16; c += 2) {
                             float a0, a1;
                             f2_split(ffma2(f2(x[c0 + c], x[c0 + c + 1]), mul2, nm2), a0, a1);
                             const float p0 = ex2(a0), p1 = ex2(a1);
                             ls[(c >> 1) & 3] = fadd2(ls[(c >> 1) & 3], f2(p0, p1));
                             pk[c / 2] = E::pack(p0, p1);
                         }
-                        tmem_st_x16(tS + c0 / 2, pk);
+                        tmem_st_x8(tS + c0 / 2, pk);
                     }
                     float s0, s1;
                     f2_split(fadd2(fadd2(ls[0], ls[1]), fadd2(ls[2], ls[3])), s0, s1);
@@ -354,12 +369,12 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
                 if (lane == 0) mbar_arrive(bar(L::P_FULL + w));
             }
             // ------------------------------------------------------------ epilogue
-            if (first < i0 + g.count) wait(L::O_FULL + w, n_o++ & 1, 0x702);
+            if (first < behind) wait(L::O_FULL + w, n_o++ & 1, 0x702);
             ml[w * L::RT + lr] = dead ? make_float2(-INFINITY, 0.f) : make_float2(m, l);
             tc_fence_before();
             named_bar_sync(1, 32 * L::NSW);
             tc_fence_after();
-            if (g.first == 0 && threadIdx.x == 0) describe_unit(p, sched, g, pos, begin);
+            if (g.first == 0 && threadIdx.x == 0) describe_unit(p, sched, g, begin);
             if (!aborted && !*abort_flag && !__all_sync(0xffffffffu, r >= p.rows)) {
                 const float2 a = ml[lr], c = ml[L::RT + lr];
                 const float M = fmaxf(a.x, c.x);
@@ -367,7 +382,7 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
                 const float lsum = fa * a.y + fc * c.y;
                 const bool whole = g.count == g.s.n;
                 const float inv = whole ? (lsum == 0.f ? 0.f : 1.f / lsum) : 1.f;
-                float* slot = partial_slot(p, segment_slot(g, pos, begin));
+                float* slot = partial_slot(p, segment_slot(g, begin));
                 const int t = p.by_G.div(r);
                 uint16_t* out = p.o + g.b * p.osb + (g.kvh * p.G + r - t * p.G) * p.osh + t * p.oss;
                 for (int c0 = w * (DP / 2); c0 < (w + 1) * (DP / 2); c0 += 32) {
@@ -404,8 +419,7 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
             tc_fence_before();
             named_bar_sync(1, 32 * L::NSW);  // Q, O, the mask and (m, l) areas are free again
             tc_fence_after();
-            i0 += g.count;
-            pos += g.count;
+            i0 = behind;
         }
         zero_empty_units(p, threadIdx.x, 32 * L::NSW);
     }

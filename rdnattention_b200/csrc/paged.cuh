@@ -110,9 +110,16 @@ struct Rows {  // [B, Hkv, T, D] view
     const uint16_t* p;
     int64_t sb, sh, ss;
 };
-struct Cache {  // [num_pages, Hkv, P, D] view
-    uint16_t* p;
-    int64_t sp, sh, ss;
+struct Cache {  // [num_pages, Hkv, P, D] view, strides in bytes
+    char* p;
+    int64_t sh;
+    uint32_t sp, ss;  // (32 bits: one multiply-add for each part of an address)
+
+    __device__ __forceinline__ char* head(int h, int ch) const { return p + h * sh + ch * 16; }
+    __device__ __forceinline__ char* at(char* head, int page, int row) const {
+        return head + static_cast<uint64_t>(static_cast<uint32_t>(page)) * sp +
+               static_cast<uint64_t>(static_cast<uint32_t>(row)) * ss;
+    }
 };
 
 // ------------------------------------------------------------------- append
@@ -153,8 +160,8 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
         k = rotate4<E>(k, __ldg(reinterpret_cast<const float4*>(p.cos + at)),
                        __ldg(reinterpret_cast<const float4*>(p.sin + at)));
     }
-    *reinterpret_cast<uint4*>(p.kc.p + page * p.kc.sp + h * p.kc.sh + row * p.kc.ss + ch * 8) = k;
-    *reinterpret_cast<uint4*>(p.vc.p + page * p.vc.sp + h * p.vc.sh + row * p.vc.ss + ch * 8) = v;
+    *reinterpret_cast<uint4*>(p.kc.at(p.kc.head(h, ch), page, row)) = k;
+    *reinterpret_cast<uint4*>(p.vc.at(p.vc.head(h, ch), page, row)) = v;
 }
 
 // ------------------------------------------------------------------- accept
@@ -181,7 +188,7 @@ __global__ void accept_kernel(const __grid_constant__ AcceptParams p) {
     const int nch = p.D / 8;
     const int ch = col % nch, h = col / nch % p.Hkv;
     const Cache& c = col / nch / p.Hkv == 0 ? p.kc : p.vc;
-    uint16_t* base = c.p + h * c.sh + ch * 8;
+    char* base = c.head(h, ch);
     const int64_t len = p.t.len(b);
     const int n = p.accepted_lens == nullptr ? p.A : min(max(p.accepted_lens[b], 0), p.A);
     const int* acc = p.accepted + static_cast<int64_t>(b) * p.A;
@@ -192,12 +199,12 @@ __global__ void accept_kernel(const __grid_constant__ AcceptParams p) {
     for (int i = 0; i < n; ++i) {
         int page, row;
         if (source(i, page, row))
-            stage[i * blockDim.x + threadIdx.x] = *reinterpret_cast<const uint4*>(base + page * c.sp + row * c.ss);
+            stage[i * blockDim.x + threadIdx.x] = *reinterpret_cast<const uint4*>(c.at(base, page, row));
     }
     for (int i = 0; i < n; ++i) {
         int page, row, dpage, drow;
         if (source(i, page, row) && p.t.locate(b, len + i, dpage, drow))
-            *reinterpret_cast<uint4*>(base + dpage * c.sp + drow * c.ss) = stage[i * blockDim.x + threadIdx.x];
+            *reinterpret_cast<uint4*>(c.at(base, dpage, drow)) = stage[i * blockDim.x + threadIdx.x];
     }
 }
 

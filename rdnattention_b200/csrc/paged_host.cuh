@@ -22,8 +22,7 @@ const char* check_strides(int64_t s0, int64_t s1, int64_t s2, uint64_t n0, uint6
         if (n[i] <= 1) continue;
         if (s[i] <= 0) return "strides must be positive";
         if (s[i] % 8 != 0) return "strides must be multiples of 16 bytes";
-        // what a tensor map can hold (40 bits of bytes)
-        if (s[i] >= (int64_t(1) << 39)) return "stride too large";
+        if (s[i] >= (int64_t(1) << 46)) return "stride too large";
     }
     return nullptr;
 }
@@ -46,6 +45,9 @@ const char* check_cache(const PagedCacheParams& c) {
     if (c.batchSize > 1 && c.tableStride < 0) return "strides must be positive";
     if (const char* e = check_strides(c.kcStrideP, c.kcStrideH, c.kcStrideS, c.numPages, c.numKvHeads, c.pageSize))
         return e;
+    // the kernels hold the page and slot strides as 32 bits of bytes
+    for (int64_t s : {c.kcStrideP, c.kcStrideS, c.vcStrideP, c.vcStrideS})
+        if (s >= (int64_t(1) << 31)) return "cache page or slot stride too large";
     return check_strides(c.vcStrideP, c.vcStrideH, c.vcStrideS, c.numPages, c.numKvHeads, c.pageSize);
 }
 
@@ -77,7 +79,7 @@ paged::Table make_table(const PagedCacheParams& c, const void* new_lens, uint32_
 }
 
 paged::Cache cache_view(void* p, int64_t sp, int64_t sh, int64_t ss) {
-    return paged::Cache{static_cast<uint16_t*>(p), sp, sh, ss};
+    return paged::Cache{static_cast<char*>(p), 2 * sh, static_cast<uint32_t>(2 * sp), static_cast<uint32_t>(2 * ss)};
 }
 
 int sm_count() {
@@ -242,6 +244,7 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
     p.n_rt = f.n_rt;
     p.tpp = f.tpp;
     p.by_G.set(static_cast<uint32_t>(p.G));
+    p.by_Hkv.set(c.numKvHeads);
     p.by_P.set(c.pageSize);
     p.by_tpp.set(f.tpp == 0 ? 1 : static_cast<uint32_t>(f.tpp));
     p.window = a.windowSize > 0 ? a.windowSize : 0;
@@ -252,11 +255,12 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
     p.ws = static_cast<float*>(workspace);
     p.units = reinterpret_cast<int2*>(static_cast<char*>(workspace) + f.partials);
     p.grid = f.grid;
+    p.W = f.mma ? paged::kLeadMma : paged::kLead;
 
     // the list positions of one launch are 32-bit: as many sequences per launch as surely fit
     const int64_t tiles = f.tpp == 0 ? (static_cast<int64_t>(c.maxPages) * c.pageSize + paged::KT - 1) / paged::KT
                                      : static_cast<int64_t>(c.maxPages) * f.tpp;
-    const int64_t per_seq = tiles * p.n_rt * p.Hkv;
+    const int64_t per_seq = (tiles + p.W) * p.n_rt * p.Hkv;
     const int64_t join_blocks = static_cast<int64_t>(p.Hkv) * p.n_rt * ((f.RT + paged::kJoinRows - 1) / paged::kJoinRows);
     const int64_t fit = INT32_MAX / (per_seq > join_blocks ? per_seq : join_blocks);
     if (fit == 0) return pfail("problem too large for one launch");
@@ -319,8 +323,9 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
         if (ce == cudaSuccess) ce = cudaGetLastError();
         if (ce != cudaSuccess) return fail(g_err_paged, "%s", cudaGetErrorString(ce));
         cfg.gridDim = dim3(static_cast<unsigned>(s.B * join_blocks));
-        cfg.blockDim = dim3(paged::kJoinRows * (c.headDim / 8));
-        cfg.dynamicSmemBytes = 0;
+        const unsigned width = 2 * c.headDim, shares = paged::kJoinThreads / width;
+        cfg.blockDim = dim3(shares * width);
+        cfg.dynamicSmemBytes = (shares - 1) * 10 * width * sizeof(float);
         ce = c.dtype == paged::DT_F16 ? cudaLaunchKernelEx(&cfg, paged::join_kernel<paged::F16>, s)
                                       : cudaLaunchKernelEx(&cfg, paged::join_kernel<paged::BF16>, s);
         if (ce == cudaSuccess) ce = cudaGetLastError();
