@@ -13,7 +13,8 @@
 // Work: a unit = (sequence, KV head, tile of RT rows) times the key tiles that
 // some row of it sees.  The tiles of all units, each unit's led by W positions for
 // what starting a unit costs, form one list, and CTA c takes the c-th equal part of
-// it: every CTA has the same time's work whatever the lengths are, and the lengths
+// it (row tiles slowest, so that the CTAs that read the same keys for other rows do so
+// at the same time and find them in L2): every CTA has the same time's work whatever the lengths are, and the lengths
 // stay on the device (a captured graph replays with new ones).  A unit that lies inside one CTA is finished there; the parts
 // of the others go to a workspace as (O, m, l) in fp32 and the combine kernel
 // joins them in list order, so results do not depend on timing.
@@ -28,9 +29,9 @@ namespace rdna {
 namespace paged {
 
 constexpr int kMaxTree = 256;          // drafted tokens under a mask
-constexpr int kMaxBatch = 1024;        // sequences per launch (the host splits larger batches)
+constexpr int kMaxList = 2048;         // sequences x row tiles per launch (the host splits larger batches)
 constexpr int KT = 64;                 // keys per tile
-constexpr int kLead = 3, kLeadMma = 4; // AttnParams::W of the two kernels
+constexpr int kLead = 4, kLeadMma = 8; // AttnParams::W of the two kernels
 
 // n / d for n < 2^31 by a multiplication: with l = ceil(log2 d) and m =
 // floor(2^(31 + l) / d) + 1, m d exceeds 2^(31 + l) by at most 2^l, so the error
@@ -60,7 +61,7 @@ struct AttnParams {
     const float *cos, *sin;
     int rope_rows;
     int B, H, Hkv, G, D;
-    FastDiv by_G, by_Hkv;
+    FastDiv by_G, by_B;
     int rows;    // T * G
     int RT;      // rows per tile
     int n_rt;    // row tiles
@@ -113,21 +114,18 @@ __device__ __forceinline__ Span row_tile_span(const AttnParams& p, int L, int n,
     return s;
 }
 
-// The list of a launch: pre[b] (shared memory) = list position behind sequence b.
+// The list of a launch: entry e = rt * B + b, pre[e] (shared memory) = position behind it.
 struct Sched {
     int total;  // positions of the launch
     int ctas;   // CTAs that take part
     int q, r;   // the first r of them take q + 1 positions, the others q
 };
 
-// Positions of one KV head of a sequence.
-__device__ __forceinline__ int head_cost(const AttnParams& p, int L, int n) {
-    int w = 0;
-    for (int rt = 0; rt < p.n_rt; ++rt) {
-        const int tiles = row_tile_span(p, L, n, rt).n;
-        w += tiles > 0 ? p.W + tiles : 0;
-    }
-    return w;
+// Positions of an entry: all KV heads of a row tile of a sequence.
+__device__ __forceinline__ int entry_cost(const AttnParams& p, int e) {
+    const int rt = p.by_B.div(e), b = e - rt * p.B;
+    const int tiles = row_tile_span(p, p.t.len(b), p.t.news(b), rt).n;
+    return tiles > 0 ? (p.W + tiles) * p.Hkv : 0;
 }
 
 __device__ __forceinline__ int warp_scan(int v, int lane) {
@@ -139,34 +137,31 @@ __device__ __forceinline__ int warp_scan(int v, int lane) {
     return v;
 }
 
-// All threads of the block.  Up to 32 sequences every warp computes the whole list and
+// All threads of the block.  Up to 32 entries every warp computes the whole list and
 // writes the same values, so that no barrier stands between the lengths and the first
 // key tile.
 __device__ __forceinline__ Sched make_sched(const AttnParams& p, int* pre) {
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, n = p.B * p.n_rt;
     Sched s;
-    if (p.B <= 32) {
-        int v = 0;
-        if (lane < p.B) v = head_cost(p, p.t.len(lane), p.t.news(lane)) * p.Hkv;
-        v = warp_scan(v, lane);
-        if (lane < p.B) pre[lane] = v;
+    if (n <= 32) {
+        const int v = warp_scan(lane < n ? entry_cost(p, lane) : 0, lane);
+        if (lane < n) pre[lane] = v;
         s.total = __shfl_sync(0xffffffffu, v, 31);
         __syncwarp();
     } else {
-        for (int b = threadIdx.x; b < p.B; b += blockDim.x)
-            pre[b] = head_cost(p, p.t.len(b), p.t.news(b)) * p.Hkv;
+        for (int e = threadIdx.x; e < n; e += blockDim.x) pre[e] = entry_cost(p, e);
         __syncthreads();
         if (threadIdx.x < 32) {
             int carry = 0;
-            for (int b0 = 0; b0 < p.B; b0 += 32) {
-                const int b = b0 + lane;
-                const int v = warp_scan(b < p.B ? pre[b] : 0, lane) + carry;
-                if (b < p.B) pre[b] = v;
+            for (int e0 = 0; e0 < n; e0 += 32) {
+                const int e = e0 + lane;
+                const int v = warp_scan(e < n ? pre[e] : 0, lane) + carry;
+                if (e < n) pre[e] = v;
                 carry = __shfl_sync(0xffffffffu, v, 31);
             }
         }
         __syncthreads();
-        s.total = pre[p.B - 1];
+        s.total = pre[n - 1];
     }
     s.ctas = min(p.grid, max(1, s.total));
     s.q = s.total / s.ctas;
@@ -191,31 +186,26 @@ struct Segment {
     int next;  // list position behind the segment
 };
 
-// The segment at list position pos < total (a whole warp; b: a sequence at or
-// before it, kept from call to call).
-__device__ __forceinline__ Segment segment_at(const AttnParams& p, const int* pre, int pos, int end, int& b) {
+// The segment at list position pos < total (a whole warp; e: an entry at or before it,
+// kept from call to call).
+__device__ __forceinline__ Segment segment_at(const AttnParams& p, const int* pre, int pos, int end, int& e) {
     const int lane = threadIdx.x & 31;
-    for (;; b += 32) {
-        const uint32_t past = __ballot_sync(0xffffffffu, b + lane < p.B && pre[b + lane] > pos);
+    for (;; e += 32) {
+        const uint32_t past = __ballot_sync(0xffffffffu, e + lane < p.B * p.n_rt && pre[e + lane] > pos);
         if (past != 0) {
-            b += __ffs(past) - 1;
+            e += __ffs(past) - 1;
             break;
         }
     }
     Segment g;
-    g.b = b;
-    g.L = p.t.len(b);
-    g.n = p.t.news(b);
-    const int start = b > 0 ? pre[b - 1] : 0, head = p.by_Hkv.div(pre[b] - start);
-    int off = pos - start;
-    g.kvh = off / head;
-    off -= g.kvh * head;
-    for (g.rt = 0;; ++g.rt) {
-        g.s = row_tile_span(p, g.L, g.n, g.rt);
-        const int cost = g.s.n > 0 ? p.W + g.s.n : 0;
-        if (off < cost) break;
-        off -= cost;
-    }
+    g.rt = p.by_B.div(e);
+    g.b = e - g.rt * p.B;
+    g.L = p.t.len(g.b);
+    g.n = p.t.news(g.b);
+    g.s = row_tile_span(p, g.L, g.n, g.rt);
+    int off = pos - (e > 0 ? pre[e - 1] : 0);
+    g.kvh = off / (p.W + g.s.n);
+    off -= g.kvh * (p.W + g.s.n);
     g.pos0 = pos - off + p.W;
     g.first = max(0, off - p.W);
     g.count = max(0, min(g.s.n - g.first, end - g.pos0 - g.first));
@@ -431,7 +421,7 @@ struct Layout {
     static constexpr int MASK_BYTES = MAX_RT * (kMaxTree / 32) * 4 + MAX_RT * 4 + MAX_RT * 8;  // limits [RT]
     static constexpr int OFF_PRE = OFF_MASK + NQ * MASK_BYTES;
     static constexpr int Q_FULL = 2 * NST, Q_EMPTY = Q_FULL + NQ, OFF_ABORT = 8 * (Q_EMPTY + NQ);  // barriers
-    static constexpr int SMEM_BYTES = OFF_PRE + kMaxBatch * 4 + 1024;  // + alignment slack
+    static constexpr int SMEM_BYTES = OFF_PRE + kMaxList * 4 + 1024;  // + alignment slack
     static_assert(!ALIAS || NCW * 16 * PSTR * 4 >= 2 * Q_BYTES, "Q fits below the partials");
     static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
 };
@@ -677,9 +667,9 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
     float* part = reinterpret_cast<float*>(smem + L::OFF_PART);
     const float sl2 = p.scale_log2;
     bool aborted = false;    // consumers: a wait expired
-    int i0 = 0, b = 0, nseg = 0;  // running tile number of the segment's first tile; segments so far
+    int i0 = 0, e = 0, nseg = 0;  // running tile number of the segment's first tile; segments so far
     for (int pos = begin; pos < end;) {
-        const Segment g = segment_at(p, pre, pos, end, b);
+        const Segment g = segment_at(p, pre, pos, end, e);
         pos = g.next;
         if (g.count == 0) continue;
         const int row0 = g.rt * p.RT, ta = p.by_G.div(row0);

@@ -7,17 +7,21 @@
 // softmax keeps up; more row tiles read the same keys again, mostly from L2.
 //
 //   warps 0..3, 4..7   two softmax groups (thread = row = TMEM lane); key tile i of
-//                      the CTA goes to group i & 1, each with its own S, O, m and l,
-//                      so one group's softmax runs while the other's products do
+//                      the CTA goes to group i & 1
 //   warps 8..11        producers (produce(), as in the few-rows kernel)
-//   warps 12, 13       one MMA-issuing lane for each group
+//   warp 12, warp 13   one lane issues S = Q K^T, one lane O += P V
 //
 // TMEM (512 columns at head_dim 128): Q hi and lo as the A operand of S = Q K^T
 // (hi + lo, see the few-rows kernel: a query in shared memory would be read again by
-// every product, 256 cycles each, and take 64 KB from the ring), S_0, S_1 (P over S
-// in place, the A operand of O += P V), O_0, O_1.
-// At the end of a segment the two groups' (O, m, l) join in the epilogue, each group
-// taking half of the columns.
+// every product and keep them at 48 cycles instead of 31 for 64 keys), four S (P over
+// S in place, the A operand of O += P V), one O.  S = Q K^T runs up to four tiles ahead
+// of the softmax, so the products of one tile and the exponentials of two others
+// overlap.
+//
+// The groups share O and with it each row's reference maximum: tile i's group takes the
+// reference that tile i - 1's left in shared memory (a token per warp pair orders
+// them), and where its own maximum is more than 2^8 above it, waits for P V of tile
+// i - 1, rescales O and leaves the new one.
 #pragma once
 
 #include "fa_paged.cuh"
@@ -30,33 +34,30 @@ struct MmaLayout {
     static constexpr int NPW = 4;
     static constexpr int NSW = 8;                       // softmax warps
     static constexpr int THREADS = 32 * (NSW + NPW + 4);
-    // Registers: launched with LAUNCH_REGS per thread (16 warps fill the register file),
-    // moved to the softmax warps, which hold 64 scores each.
-    static constexpr int LAUNCH_REGS = 128, SOFTMAX_REGS = 160, OTHER_REGS = 96;
-    static_assert(NSW * SOFTMAX_REGS + (NPW + 4) * OTHER_REGS <= (NSW + NPW + 4) * LAUNCH_REGS,
-                  "register split exceeds the launch allocation");
     static constexpr int NBOX = DP / 64;
     static constexpr int BOX_BYTES = KT * 128;
     static constexpr int TILE = NBOX * BOX_BYTES;
     static constexpr int STAGE = 2 * TILE;
     static constexpr int NST = 6;
-    static_assert(NST % 2 == 0, "a ring slot belongs to one softmax group");
+    static constexpr int NSB = 4;  // S buffers
     static constexpr int RT = 128;
     static constexpr int NW = kMaxTree / 32;
     // barriers (8 bytes each): full [NST], empty [NST], then
-    static constexpr int S_FULL = 2 * NST, P_FULL = S_FULL + 2, O_FULL = P_FULL + 2, Q_FULL = O_FULL + 2,
-                         DRAIN = Q_FULL + 2, N_BARS = DRAIN + 2;
+    static constexpr int S_FULL = 2 * NST, P_FULL = S_FULL + NSB, PV_DONE = P_FULL + NSB,  // [NSB] each
+        TOKEN = PV_DONE + NSB,                                                             // [2 groups][4 warps]
+        O_FULL = TOKEN + 8, Q_FULL = O_FULL + 1, DRAIN = Q_FULL + 1, N_BARS = DRAIN + 2;
     static constexpr int OFF_TMEM = 8 * N_BARS, OFF_ABORT = OFF_TMEM + 4;
     static constexpr int OFF_RING = 1024;
-    static constexpr int OFF_MASK = OFF_RING + NST * STAGE;  // [RT][NW + 2] (two words of padding), then [RT]
-    static constexpr int OFF_ML = OFF_MASK + RT * NW * 4 + RT * 4;  // [2][RT] (m, l)
-    static constexpr int OFF_SEG = OFF_ML + 2 * RT * 8;  // [NSW] Segment
+    static constexpr int OFF_MASK = OFF_RING + NST * STAGE;  // [RT][NW], then [RT]
+    static constexpr int OFF_M = OFF_MASK + RT * NW * 4 + RT * 4;  // [RT] reference maxima
+    static constexpr int OFF_L = OFF_M + RT * 4;                   // [2][RT] row sums
+    static constexpr int OFF_SEG = OFF_L + 2 * RT * 4;             // [NSW] Segment
     static constexpr int OFF_PRE = OFF_SEG + NSW * 64;
     static_assert(sizeof(Segment) <= 64, "a segment's slot");
-    static constexpr int SMEM_BYTES = OFF_PRE + kMaxBatch * 4 + 1024;  // + alignment slack
+    static constexpr int SMEM_BYTES = OFF_PRE + kMaxList * 4 + 1024;  // + alignment slack
     static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
     // TMEM columns
-    static constexpr int QHI = 0, QLO = DP / 2, S0 = DP, O0 = S0 + 2 * KT, TMEM_USED = O0 + 2 * DP;
+    static constexpr int QHI = 0, QLO = DP / 2, S0 = DP, O0 = S0 + NSB * KT, TMEM_USED = O0 + DP;
     static constexpr int TMEM_COLS = 512;
     static_assert(TMEM_USED <= TMEM_COLS, "TMEM budget");
 };
@@ -72,15 +73,13 @@ struct AbFormat<BF16> {
     static constexpr uint32_t value = 1;
 };
 
-// Row max of 64 values: 8 chains of three-input max.
-__device__ __forceinline__ float max64(const float* x) {
+// Row max of 32 values: 8 chains of three-input max.
+__device__ __forceinline__ float max32(const float* x) {
     float m[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m[i] = fmaxf(x[i], x[i + 8]);
+    for (int i = 0; i < 8; ++i) m[i] = fmax3(x[i], x[i + 8], x[i + 16]);
 #pragma unroll
-    for (int c = 16; c < 64; c += 16)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m[i] = fmax3(m[i], x[c + i], x[c + 8 + i]);
+    for (int i = 0; i < 8; ++i) m[i] = fmaxf(m[i], x[i + 24]);
     return fmax3(fmax3(m[0], m[1], m[2]), fmax3(m[3], m[4], m[5]), fmaxf(m[6], m[7]));
 }
 
@@ -119,13 +118,16 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
             mbar_init(bar(s), 32 * L::NPW);
             mbar_init(bar(L::NST + s), 1);
         }
-        for (int w = 0; w < 2; ++w) {
-            mbar_init(bar(L::S_FULL + w), 1);
-            mbar_init(bar(L::P_FULL + w), 4);
-            mbar_init(bar(L::O_FULL + w), 1);
-            mbar_init(bar(L::Q_FULL + w), L::NSW);
-            mbar_init(bar(L::DRAIN + w), 1);
+        for (int k = 0; k < L::NSB; ++k) {
+            mbar_init(bar(L::S_FULL + k), 1);
+            mbar_init(bar(L::P_FULL + k), 4);
+            mbar_init(bar(L::PV_DONE + k), 1);
         }
+        for (int k = 0; k < 8; ++k) mbar_init(bar(L::TOKEN + k), 1);
+        mbar_init(bar(L::O_FULL), 1);
+        mbar_init(bar(L::Q_FULL), L::NSW);
+        mbar_init(bar(L::DRAIN), 1);
+        mbar_init(bar(L::DRAIN + 1), 1);
         fence_barrier_init();
     }
     // columns behind head_dim are never copied: zero for good
@@ -156,11 +158,10 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
     tc_fence_after();
     const uint32_t tmem = producer ? 0 : *reinterpret_cast<volatile uint32_t*>(smem + L::OFF_TMEM);
 
-    int i0 = 0, b = 0;  // running tile number of the segment's first tile
+    int i0 = 0, e = 0;  // running tile number of the segment's first tile
     if (producer) {
-        regs_decrease<L::OTHER_REGS>();
         for (int pos = begin; pos < end;) {
-            const Segment g = segment_at(p, pre, pos, end, b);
+            const Segment g = segment_at(p, pre, pos, end, e);
             if (!produce<L>(p, g, i0, bars, smem_u32(ring), ab, threadIdx.x - 32 * L::NSW)) break;
             i0 += g.count;
             pos = g.next;
@@ -168,55 +169,62 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
         cp_async_wait_all();  // after an expired wait too, no copy outlives the CTA
     } else if (warp >= L::NSW + L::NPW) {
         // ------------------------------------------------------------ MMA issuers
-        regs_decrease<L::OTHER_REGS>();
-        const int w = warp - (L::NSW + L::NPW);
+        const int w = warp - (L::NSW + L::NPW);  // 0: S = Q K^T, 1: O += P V, others: idle
         if (w < 2) {
             constexpr uint32_t IDESC_QK = instr_desc(1u, AbFormat<E>::value, 0u, 128, KT);
             constexpr uint32_t IDESC_PV = instr_desc(1u, AbFormat<E>::value, 1u, 128, DP);
-            const uint32_t tS = tmem + L::S0 + w * KT, tO = tmem + L::O0 + w * DP;
             const uint64_t kd = smem_desc(smem_u32(ring), 16, 1024, 2);
             const uint64_t vd = smem_desc(smem_u32(ring + L::TILE), L::BOX_BYTES, 1024, 2);
-            int seg = 0, n = 0;  // segments with a tile of this group, and its tiles, so far
-            int ok = 1;
+            const int halves = p.cos != nullptr ? 2 : 1;  // a query that is not turned has no lo
+            int seg = 0, ok = 1;
             for (int pos = begin; pos < end && ok;) {
-                const Segment g = segment_at(p, pre, pos, end, b);
-                const int first = i0 + ((w - i0) & 1);
-                if (lane == 0 && first < i0 + g.count) {
-                    // (signalled only for segments with a tile of this group: no phase passes
-                    // that this thread does not see)
-                    ok = mbar_wait(bar(L::Q_FULL + w), seg++ & 1, ab, 0x711);
-                    tc_fence_after();
-                    for (int i = first; ok && i < i0 + g.count; i += 2, ++n) {
-                        const int s = i % L::NST;
-                        const uint32_t slot = static_cast<uint32_t>(s * L::STAGE) >> 4;
-                        ok = mbar_wait(bar(s), i / L::NST & 1, ab, 0x712);
-                        if (!ok) break;
-                        // the copies were written through the generic proxy, the products read
-                        // through the async one
-                        fence_proxy_async_smem();
+                const Segment g = segment_at(p, pre, pos, end, e);
+                pos = g.next;
+                if (g.count == 0) continue;
+                if (lane == 0) {
+                    if (w == 0) {
+                        ok = mbar_wait(bar(L::Q_FULL), seg++ & 1, ab, 0x711);
                         tc_fence_after();
+                    }
+                    for (int i = i0; ok && i < i0 + g.count; ++i) {
+                        const int s = i % L::NST, sb = i % L::NSB;
+                        const uint32_t slot = static_cast<uint32_t>(s * L::STAGE) >> 4, tS = tmem + L::S0 + sb * KT;
+                        if (w == 0) {
+                            // the buffer's last P has been multiplied, the keys are there
+                            ok = mbar_wait(bar(L::PV_DONE + sb), (i / L::NSB & 1) ^ 1, ab, 0x712) &&
+                                 mbar_wait(bar(s), i / L::NST & 1, ab, 0x713);
+                            if (!ok) break;
+                            // the copies were written through the generic proxy, the products
+                            // read through the async one
+                            fence_proxy_async_smem();
+                            tc_fence_after();
+                            for (int half = 0; half < halves; ++half)
 #pragma unroll
-                        for (int half = 0; half < 2; ++half)
+                                for (int kk = 0; kk < DP / 16; ++kk)
+                                    mma_f16_ts(tS, tmem + (half ? L::QLO : L::QHI) + kk * 8,
+                                               kd + slot +
+                                                   static_cast<uint32_t>((kk / 4 * L::BOX_BYTES + kk % 4 * 32) >> 4),
+                                               IDESC_QK, half > 0 || kk > 0);
+                            tc_commit(bar(L::S_FULL + sb));
+                        } else {
+                            ok = mbar_wait(bar(s), i / L::NST & 1, ab, 0x714) &&
+                                 mbar_wait(bar(L::P_FULL + sb), i / L::NSB & 1, ab, 0x715);
+                            if (!ok) break;
+                            fence_proxy_async_smem();
+                            tc_fence_after();
 #pragma unroll
-                            for (int kk = 0; kk < DP / 16; ++kk)
-                                mma_f16_ts(tS, tmem + (half ? L::QLO : L::QHI) + kk * 8,
-                                           kd + slot + static_cast<uint32_t>((kk / 4 * L::BOX_BYTES + kk % 4 * 32) >> 4),
-                                           IDESC_QK, half || kk > 0);
-                        tc_commit(bar(L::S_FULL + w));
-                        ok = mbar_wait(bar(L::P_FULL + w), n & 1, ab, 0x713);
-                        if (!ok) break;
-                        tc_fence_after();
-#pragma unroll
-                        for (int kk = 0; kk < KT / 16; ++kk)
-                            mma_f16_ts(tO, tS + kk * 8, vd + slot + static_cast<uint32_t>((kk * 16 * 128) >> 4), IDESC_PV,
-                                       kk > 0 || i > first);
-                        tc_commit(bar(L::NST + s));
-                        if (i + 2 >= i0 + g.count) tc_commit(bar(L::O_FULL + w));
+                            for (int kk = 0; kk < KT / 16; ++kk)
+                                mma_f16_ts(tmem + L::O0, tS + kk * 8, vd + slot + static_cast<uint32_t>((kk * 16 * 128) >> 4),
+                                           IDESC_PV, kk > 0 || i > i0);
+                            // (S of this tile came first: its keys have been read too)
+                            tc_commit(bar(L::NST + s));
+                            tc_commit(bar(L::PV_DONE + sb));
+                            if (i == i0 + g.count - 1) tc_commit(bar(L::O_FULL));
+                        }
                     }
                 }
                 ok = __shfl_sync(0xffffffffu, ok, 0);
                 i0 += g.count;
-                pos = g.next;
             }
             if (lane == 0) {
                 // nothing of this thread's is in flight when the TMEM goes
@@ -227,17 +235,17 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
         }
     } else {
         // ---------------------------------------------------------------- softmax
-        regs_increase<L::SOFTMAX_REGS>();
         const int w = warp / 4, quad = warp % 4, lr = quad * 32 + lane;  // row of the tile
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
-        const uint32_t tS = tmem + lanes + L::S0 + w * KT, tO = tmem + lanes + L::O0;
+        const uint32_t tO = tmem + lanes + L::O0;
         uint32_t* words = reinterpret_cast<uint32_t*>(smem + L::OFF_MASK);
         int* ctx_lo = reinterpret_cast<int*>(smem + L::OFF_MASK + L::RT * L::NW * 4);
-        float2* ml = reinterpret_cast<float2*>(smem + L::OFF_ML);
+        volatile float* ref = reinterpret_cast<volatile float*>(smem + L::OFF_M);
+        float* sums = reinterpret_cast<float*>(smem + L::OFF_L);
         const int nw = (p.t.T + 31) / 32;
         const float sl2 = p.scale_log2;
         bool aborted = false;
-        int n = 0, n_o = 0;  // tiles, and segments with a tile, of this group so far
+        int seg = 0;  // segments so far
         auto wait = [&](int i, int parity, int site) {
             if (!aborted && !__all_sync(0xffffffffu, mbar_wait(bar(i), parity, ab, site))) aborted = true;
             return !aborted;
@@ -246,7 +254,7 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
             // (each warp keeps its segment in shared memory: registers are for the scores)
             Segment& g = reinterpret_cast<Segment*>(smem + L::OFF_SEG)[warp];
             {
-                const Segment found = segment_at(p, pre, pos, end, b);
+                const Segment found = segment_at(p, pre, pos, end, e);
                 if (lane == 0) g = found;
                 __syncwarp();
                 pos = found.next;
@@ -274,15 +282,14 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
                         lo[4 * c + 2] = l.z;
                         lo[4 * c + 3] = l.w;
                     }
+                    __syncwarp();
                     tmem_st_x16(tmem + lanes + L::QHI + 4 * c0, hi);
                     tmem_st_x16(tmem + lanes + L::QLO + 4 * c0, lo);
                 }
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0)
-                    for (int k = 0; k < 2; ++k)
-                        if (((k - i0) & 1) < g.count) mbar_arrive(bar(L::Q_FULL + k));
+                if (lane == 0) mbar_arrive(bar(L::Q_FULL));
             }
             if (p.mask != nullptr) {
                 build_mask(p, g, words, ctx_lo, threadIdx.x, 32 * L::NSW);
@@ -300,64 +307,97 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
             float m = -INFINITY, l = 0.f;
             const int behind = i0 + g.count, tile0 = g.s.t0 + g.first - i0, L0 = g.L;
             const int first = i0 + ((w - i0) & 1);
-            for (int i = first; i < behind; i += 2, ++n) {
-                if (!wait(L::S_FULL + w, n & 1, 0x701)) continue;
+            for (int i = first; i < behind; i += 2) {
+                const int sb = i % L::NSB;
+                const uint32_t tS = tmem + lanes + L::S0 + sb * KT;
+                if (!wait(L::S_FULL + sb, i / L::NSB & 1, 0x701)) continue;
+                tc_fence_after();
+                // 32 scores at a time, so that the row fits the 128 registers of 512 threads: the
+                // upper half for the maximum, then the lower half, which stays for its exponentials;
+                // the upper half is read once more
+                float mx = -INFINITY;
+                uint32_t raw[32];
+                float* x = reinterpret_cast<float*>(raw);
+                uint32_t see[2] = {~0u, ~0u};
+                bool edge = false;
+                auto load_half = [&](int h) {
+                    tmem_ld_x32(tS + 32 * h, raw);
+                    if (edge) {
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            if (!(see[h] >> c & 1u)) x[c] = -INFINITY;
+                    }
+                };
                 if (!idle) {
-                    tc_fence_after();
                     int k0, valid;
                     tile_keys(p, tile0 + i, k0, valid);
-                    uint32_t raw[KT];
-                    tmem_ld_x64(tS, raw);
-                    float* x = reinterpret_cast<float*>(raw);
-                    if (valid < KT || k0 < all_lo || k0 + KT > all_hi) {
-                        uint64_t see = bits_between(rlo - k0, min(rhi - k0, valid));
+                    edge = valid < KT || k0 < all_lo || k0 + KT > all_hi;
+                    if (edge) {
+                        uint64_t bits = bits_between(rlo - k0, min(rhi - k0, valid));
                         if (p.mask != nullptr && k0 + KT > L0)
-                            see &= bits_between(0, L0 - k0) | draft_bits(words + rw, nw, k0 - L0);
-                        const uint32_t see0 = static_cast<uint32_t>(see), see1 = static_cast<uint32_t>(see >> 32);
-#pragma unroll
-                        for (int c = 0; c < 32; ++c) {
-                            if (!(see0 >> c & 1u)) x[c] = -INFINITY;
-                            if (!(see1 >> c & 1u)) x[32 + c] = -INFINITY;
-                        }
+                            bits &= bits_between(0, L0 - k0) | draft_bits(words + rw, nw, k0 - L0);
+                        see[0] = static_cast<uint32_t>(bits);
+                        see[1] = static_cast<uint32_t>(bits >> 32);
                     }
-                    const float mx = max64(x) * sl2;
-                    // O is rescaled only when the maximum grows by more than 2^8: the row's final
-                    // 1 / l uses the same reference, and p stays below 2^8
-                    const bool grow = fmaxf(m, mx) > m + 8.f;
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float corr = grow ? ex2(m - fmaxf(m, mx)) : 1.f;
-                        if (grow) {
-                            m = fmaxf(m, mx);
-                            l *= corr;
-                        }
-                        // (S of this tile was committed after the group's previous P V)
-                        if (i > first)
+                    load_half(1);
+                    mx = max32(x);
+                    load_half(0);
+                    mx = fmaxf(mx, max32(x)) * sl2;
+                }
+                // the reference that the tile before left (the first tile of a segment has none)
+                if (i > i0 && !wait(L::TOKEN + (w ^ 1) * 4 + quad, (i - 1) / 2 & 1, 0x703)) continue;
+                const float old = i > i0 ? ref[lr] : -INFINITY;
+                float now = old;
+                const bool grow = fmaxf(old, mx) > old + 8.f;
+                if (grow) now = fmaxf(old, mx);
+                if (__any_sync(0xffffffffu, grow) && i > i0) {
+                    // O is rescaled only when a maximum grows by more than 2^8: the row's final 1 / l
+                    // uses the same reference, and p stays below 2^8
+                    if (!wait(L::PV_DONE + (i - 1) % L::NSB, (i - 1) / L::NSB & 1, 0x704)) continue;
+                    tc_fence_after();
+                    const float corr = grow ? ex2(old - now) : 1.f;
 #pragma unroll 1
-                            for (int c0 = 0; c0 < DP; c0 += 16) {
-                                uint32_t o[16];
-                                tmem_ld_x16(tO + w * DP + c0, o);
+                    for (int c0 = 0; c0 < DP; c0 += 16) {
+                        uint32_t o[16];
+                        tmem_ld_x16(tO + c0, o);
 #pragma unroll
-                                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                                tmem_st_x16(tO + w * DP + c0, o);
-                            }
+                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * corr);
+                        tmem_st_x16(tO + c0, o);
                     }
+                    tmem_wait_st();
+                    tc_fence_before();
+                }
+                ref[lr] = now;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(L::TOKEN + w * 4 + quad));
+                if (now != m) {
+                    l *= ex2(m - now);  // (the other group may have moved it)
+                    m = now;
+                }
+                __syncwarp();  // the TMEM accesses below are warp-wide
+                if (!idle) {
                     // P is rounded to the cache's type, the operand type of the second product;
                     // the row sums take it unrounded
                     const float nm = m == -INFINITY ? 0.f : -m;
                     const uint64_t mul2 = f2(sl2, sl2), nm2 = f2(nm, nm);
                     uint64_t ls[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
-                    for (int c0 = 0; c0 < KT; c0 += 16) {
-                        uint32_t pk[8];
+                    for (int h = 0; h < 2; ++h) {
+                        if (h == 1) load_half(1);
 #pragma unroll
-                        for (int c = 0; c < 16; c += 2) {
-                            float a0, a1;
-                            f2_split(ffma2(f2(x[c0 + c], x[c0 + c + 1]), mul2, nm2), a0, a1);
-                            const float p0 = ex2(a0), p1 = ex2(a1);
-                            ls[(c >> 1) & 3] = fadd2(ls[(c >> 1) & 3], f2(p0, p1));
-                            pk[c / 2] = E::pack(p0, p1);
+                        for (int c0 = 0; c0 < 32; c0 += 16) {
+                            uint32_t pk[8];
+#pragma unroll
+                            for (int c = 0; c < 16; c += 2) {
+                                float a0, a1;
+                                f2_split(ffma2(f2(x[c0 + c], x[c0 + c + 1]), mul2, nm2), a0, a1);
+                                const float p0 = ex2(a0), p1 = ex2(a1);
+                                ls[(c >> 1) & 3] = fadd2(ls[(c >> 1) & 3], f2(p0, p1));
+                                pk[c / 2] = E::pack(p0, p1);
+                            }
+                            // (columns whose scores have been read already)
+                            tmem_st_x8(tS + 16 * h + c0 / 2, pk);
                         }
-                        tmem_st_x8(tS + c0 / 2, pk);
                     }
                     float s0, s1;
                     f2_split(fadd2(fadd2(ls[0], ls[1]), fadd2(ls[2], ls[3])), s0, s1);
@@ -366,47 +406,48 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
                     tc_fence_before();
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar(L::P_FULL + w));
+                if (lane == 0) mbar_arrive(bar(L::P_FULL + sb));
             }
             // ------------------------------------------------------------ epilogue
-            if (first < behind) wait(L::O_FULL + w, n_o++ & 1, 0x702);
-            ml[w * L::RT + lr] = dead ? make_float2(-INFINITY, 0.f) : make_float2(m, l);
-            tc_fence_before();
-            named_bar_sync(1, 32 * L::NSW);
+            wait(L::O_FULL, seg++ & 1, 0x702);
             tc_fence_after();
+            // this group's sum against the segment's last reference
+            {
+                const int last = behind - 1;
+                if ((last & 1) != w) wait(L::TOKEN + (w ^ 1) * 4 + quad, last / 2 & 1, 0x705);
+                const float end_m = ref[lr];
+                sums[w * L::RT + lr] = m == end_m ? l : l * ex2(m - end_m);
+                m = end_m;
+            }
+            named_bar_sync(1, 32 * L::NSW);
             if (g.first == 0 && threadIdx.x == 0) describe_unit(p, sched, g, begin);
             if (!aborted && !*abort_flag && !__all_sync(0xffffffffu, r >= p.rows)) {
-                const float2 a = ml[lr], c = ml[L::RT + lr];
-                const float M = fmaxf(a.x, c.x);
-                const float fa = a.x == -INFINITY ? 0.f : ex2(a.x - M), fc = c.x == -INFINITY ? 0.f : ex2(c.x - M);
-                const float lsum = fa * a.y + fc * c.y;
+                const float M = dead ? -INFINITY : m;
+                const float lsum = dead ? 0.f : sums[lr] + sums[L::RT + lr];
                 const bool whole = g.count == g.s.n;
                 const float inv = whole ? (lsum == 0.f ? 0.f : 1.f / lsum) : 1.f;
                 float* slot = partial_slot(p, segment_slot(g, begin));
                 const int t = p.by_G.div(r);
                 uint16_t* out = p.o + g.b * p.osb + (g.kvh * p.G + r - t * p.G) * p.osh + t * p.oss;
                 for (int c0 = w * (DP / 2); c0 < (w + 1) * (DP / 2); c0 += 32) {
-                    uint32_t oa[32], oc[32];
-                    tmem_ld_x32(tO + c0, oa);
-                    tmem_ld_x32(tO + DP + c0, oc);
-                    // (a group without a tile, or a row without a key, left its O undefined)
+                    uint32_t raw[32];
+                    __syncwarp();
+                    tmem_ld_x32(tO + c0, raw);
                     float o[32];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e)
-                        o[e] = ((a.x == -INFINITY ? 0.f : fa * __uint_as_float(oa[e])) +
-                                (c.x == -INFINITY ? 0.f : fc * __uint_as_float(oc[e]))) * inv;
+                    for (int k = 0; k < 32; ++k) o[k] = M == -INFINITY ? 0.f : __uint_as_float(raw[k]) * inv;
                     if (r < p.rows) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            if (c0 + e >= p.D) break;
+                        for (int k = 0; k < 32; k += 8) {
+                            if (c0 + k >= p.D) break;
                             if (whole) {
-                                *reinterpret_cast<uint4*>(out + c0 + e) =
-                                    uint4{E::pack(o[e], o[e + 1]), E::pack(o[e + 2], o[e + 3]),
-                                          E::pack(o[e + 4], o[e + 5]), E::pack(o[e + 6], o[e + 7])};
+                                *reinterpret_cast<uint4*>(out + c0 + k) =
+                                    uint4{E::pack(o[k], o[k + 1]), E::pack(o[k + 2], o[k + 3]),
+                                          E::pack(o[k + 4], o[k + 5]), E::pack(o[k + 6], o[k + 7])};
                             } else {
-                                float4* d = reinterpret_cast<float4*>(slot) + (c0 + e) / 4 * p.RT + lr;
-                                d[0] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                                d[p.RT] = make_float4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]);
+                                float4* d = reinterpret_cast<float4*>(slot) + (c0 + k) / 4 * p.RT + lr;
+                                d[0] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                                d[p.RT] = make_float4(o[k + 4], o[k + 5], o[k + 6], o[k + 7]);
                             }
                         }
                     }

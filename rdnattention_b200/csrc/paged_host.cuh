@@ -2,6 +2,7 @@
 // translation unit that holds every kernel): checks, tensor maps, launches.
 #pragma once
 
+#include <algorithm>
 #include <cmath>
 
 namespace rdna {
@@ -112,8 +113,9 @@ PagedPlan paged_plan(uint32_t B, uint32_t H, uint32_t Hkv, uint32_t T, uint32_t 
     f.tpp = static_cast<int>(P) >= paged::KT ? (static_cast<int>(P) + paged::KT - 1) / paged::KT : 0;
     f.grid = sm_count();
     f.partials = align_up(static_cast<size_t>(2) * f.grid * f.RT * (D + 2) * sizeof(float));
-    const size_t seqs = B < static_cast<uint32_t>(paged::kMaxBatch) ? B : paged::kMaxBatch;
-    f.bytes = f.partials + align_up(seqs * Hkv * f.n_rt * sizeof(int2));
+    // units of a launch: at most kMaxList (sequence, row tile) pairs
+    const int64_t seqs = std::max<int64_t>(1, std::min<int64_t>(B, paged::kMaxList / f.n_rt));
+    f.bytes = f.partials + align_up(static_cast<size_t>(seqs) * Hkv * f.n_rt * sizeof(int2));
     return f;
 }
 
@@ -244,7 +246,6 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
     p.n_rt = f.n_rt;
     p.tpp = f.tpp;
     p.by_G.set(static_cast<uint32_t>(p.G));
-    p.by_Hkv.set(c.numKvHeads);
     p.by_P.set(c.pageSize);
     p.by_tpp.set(f.tpp == 0 ? 1 : static_cast<uint32_t>(f.tpp));
     p.window = a.windowSize > 0 ? a.windowSize : 0;
@@ -263,13 +264,14 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
     const int64_t per_seq = (tiles + p.W) * p.n_rt * p.Hkv;
     const int64_t join_blocks = static_cast<int64_t>(p.Hkv) * p.n_rt * ((f.RT + paged::kJoinRows - 1) / paged::kJoinRows);
     const int64_t fit = INT32_MAX / (per_seq > join_blocks ? per_seq : join_blocks);
-    if (fit == 0) return pfail("problem too large for one launch");
-    const int64_t step = fit < paged::kMaxBatch ? fit : paged::kMaxBatch;
+    const int64_t step = std::min<int64_t>(fit, paged::kMaxList / p.n_rt);
+    if (step == 0) return pfail("problem too large for one launch");
 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     for (int64_t b0 = 0; b0 < c.batchSize; b0 += step) {
         paged::AttnParams s = p;
         s.B = static_cast<int>(c.batchSize - b0 < step ? c.batchSize - b0 : step);
+        s.by_B.set(static_cast<uint32_t>(s.B));
         s.q += b0 * p.qsb;
         s.o += b0 * p.osb;
         s.t.pages += b0 * p.t.stride;
@@ -288,17 +290,9 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
         cfg.numAttrs = 1;
         cfg.stream = st;
         cfg.gridDim = dim3(static_cast<unsigned>(f.grid));
-        // regs != 0: the kernel moves registers between its warps and must have been given
-        // exactly that many per thread (an increase waits for registers the CTA has)
-        auto launch = [&](auto kern, int threads, int smem, int regs) {
+        auto launch = [&](auto kern, int threads, int smem) {
             cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
             if (ce != cudaSuccess) return ce;
-            if (regs != 0) {
-                cudaFuncAttributes fa{};
-                ce = cudaFuncGetAttributes(&fa, kern);
-                if (ce != cudaSuccess) return ce;
-                if (fa.numRegs != regs) return cudaErrorInvalidKernelImage;
-            }
             cfg.blockDim = dim3(threads);
             cfg.dynamicSmemBytes = smem;
             return launch_timed(st, [&] { return cudaLaunchKernelEx(&cfg, kern, s); });
@@ -311,12 +305,12 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
             using M64 = paged::MmaLayout<64>;
             using M128 = paged::MmaLayout<128>;
             if (f.mma)
-                return f.dp == 64 ? launch(paged::fa_paged_mma_kernel<T, 64>, M64::THREADS, M64::SMEM_BYTES, M64::LAUNCH_REGS)
-                                  : launch(paged::fa_paged_mma_kernel<T, 128>, M128::THREADS, M128::SMEM_BYTES, M128::LAUNCH_REGS);
+                return f.dp == 64 ? launch(paged::fa_paged_mma_kernel<T, 64>, M64::THREADS, M64::SMEM_BYTES)
+                                  : launch(paged::fa_paged_mma_kernel<T, 128>, M128::THREADS, M128::SMEM_BYTES);
             switch (f.dp) {
-                case 64: return launch(paged::fa_paged_kernel<T, 64>, L64::THREADS, L64::SMEM_BYTES, 0);
-                case 128: return launch(paged::fa_paged_kernel<T, 128>, L128::THREADS, L128::SMEM_BYTES, 0);
-                default: return launch(paged::fa_paged_kernel<T, 256>, L256::THREADS, L256::SMEM_BYTES, 0);
+                case 64: return launch(paged::fa_paged_kernel<T, 64>, L64::THREADS, L64::SMEM_BYTES);
+                case 128: return launch(paged::fa_paged_kernel<T, 128>, L128::THREADS, L128::SMEM_BYTES);
+                default: return launch(paged::fa_paged_kernel<T, 256>, L256::THREADS, L256::SMEM_BYTES);
             }
         };
         cudaError_t ce = c.dtype == paged::DT_F16 ? by_width(paged::F16{}) : by_width(paged::BF16{});
