@@ -20,6 +20,7 @@
 // joins them in list order, so results do not depend on timing.
 #pragma once
 
+#include <cuda.h>
 #include <limits.h>
 #include <math.h>
 
@@ -52,7 +53,6 @@ struct FastDiv {
 struct AttnParams {
     const uint16_t* q;
     uint16_t* o;
-    Cache kc, vc;
     int64_t qsb, qsh, qss, osb, osh, oss;
     Table t;
     const uint8_t* mask;  // [B][T][T] bool or null: chain
@@ -184,6 +184,7 @@ struct Segment {
     int first, count;
     int pos0;  // list position of the unit's tile 0
     int next;  // list position behind the segment
+    int e;     // its list entry
 };
 
 // The segment at list position pos < total (a whole warp; e: an entry at or before it,
@@ -198,6 +199,7 @@ __device__ __forceinline__ Segment segment_at(const AttnParams& p, const int* pr
         }
     }
     Segment g;
+    g.e = e;
     g.rt = p.by_B.div(e);
     g.b = e - g.rt * p.B;
     g.L = p.t.len(g.b);
@@ -259,42 +261,46 @@ __device__ __forceinline__ void zero_empty_units(const AttnParams& p, int tid, i
     }
 }
 
-// Bits of the drafted tokens that the tokens of a row tile see: words[i * nw + w]
-// for token ta + i, mask bytes to bits by ballot; then the window drops the
-// lowest.  rlo_ctx[i] = first context slot token ta + i sees.  Threads
-// tid .. of `nthreads` (whole warps) take part; the caller synchronises them.
-__device__ __forceinline__ void build_mask(const AttnParams& p, const Segment& g, uint32_t* words, int* ctx_lo,
-                                           int tid, int nthreads) {
-    const int nw = (p.t.T + 31) / 32;
-    const int ta = p.by_G.div(g.rt * p.RT);
-    const int nt = min(p.by_G.div(min((g.rt + 1) * p.RT, p.rows) - 1), g.n - 1) - ta + 1;
-    const int lane = tid & 31;
-    for (int i = tid / 32; i < nt; i += nthreads / 32) {
-        const uint8_t* row = p.mask + g.b * p.msb + (ta + i) * p.mst;
-        uint32_t mine = 0;  // lane w holds word w
+// Bits of the drafted tokens that the tokens of a row tile see: words[i * nw + w] for
+// token ta + i, mask bytes to bits by ballot, four words' loads in flight.  Threads tid ..
+// of `nthreads` (whole warps) take part; the caller synchronises them, and with a window
+// calls trim_mask() then and synchronises again.
+__device__ __forceinline__ int tile_tokens(const AttnParams& p, const Segment& g) {
+    return min(p.by_G.div(min((g.rt + 1) * p.RT, p.rows) - 1), g.n - 1) - p.by_G.div(g.rt * p.RT) + 1;
+}
+__device__ __forceinline__ void build_mask(const AttnParams& p, const Segment& g, uint32_t* words, int tid,
+                                           int nthreads) {
+    const int nw = (p.t.T + 31) / 32, total = tile_tokens(p, g) * nw;
+    const int lane = tid & 31, warps = nthreads / 32;
+    const uint8_t* base = p.mask + g.b * p.msb + p.by_G.div(g.rt * p.RT) * p.mst;
+    for (int j0 = tid / 32; j0 < total; j0 += 4 * warps) {
+        uint32_t see[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int j = j0 + k * warps, i = j / nw, u = 32 * (j - i * nw) + lane;
+            see[k] = j < total && u < g.n ? base[i * p.mst + u] : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t bits = __ballot_sync(0xffffffffu, see[k] != 0);
+            if (lane == 0 && j0 + k * warps < total) words[j0 + k * warps] = bits;
+        }
+    }
+}
+// The window: a token keeps its newest drafted tokens, at most w, and sees the newest w
+// less those of the context, from ctx_lo[i] on.
+__device__ __forceinline__ void trim_mask(const AttnParams& p, const Segment& g, uint32_t* words, int* ctx_lo, int tid,
+                                          int nthreads) {
+    const int nw = (p.t.T + 31) / 32, nt = tile_tokens(p, g);
+    for (int i = tid; i < nt; i += nthreads) {
         int seen = 0;
-        for (int w = 0; w < nw; ++w) {
-            const int u = 32 * w + lane;
-            const uint32_t bits = __ballot_sync(0xffffffffu, u < g.n && row[u] != 0);
-            seen += __popc(bits);
-            if (lane == w) mine = bits;
+        for (int w = 0; w < nw; ++w) seen += __popc(words[i * nw + w]);
+        for (int w = 0, drop = seen - p.window; drop > 0; ++w) {
+            uint32_t bits = words[i * nw + w];
+            for (; drop > 0 && bits != 0; --drop) bits &= bits - 1;
+            words[i * nw + w] = bits;
         }
-        int keep = seen;
-        if (p.window > 0 && seen > p.window) {
-            // drop the lowest seen - window bits
-            int drop = seen - p.window;
-            keep = p.window;
-            for (int w = 0; w < nw; ++w) {
-                uint32_t bits = __shfl_sync(0xffffffffu, mine, w);
-                while (drop > 0 && bits != 0) {
-                    bits &= bits - 1;
-                    --drop;
-                }
-                if (lane == w) mine = bits;
-            }
-        }
-        if (lane < nw) words[i * nw + lane] = mine;
-        if (lane == 0) ctx_lo[i] = p.window > 0 ? max(0, g.L - (p.window - keep)) : 0;
+        ctx_lo[i] = max(0, g.L - max(0, p.window - seen));
     }
 }
 
@@ -303,15 +309,16 @@ __device__ __forceinline__ void build_mask(const AttnParams& p, const Segment& g
 // the same order.  A block takes 16 rows; a thread one row (lanes side by side, so the
 // partials are read in whole lines), 8 columns and every n-th part, n = blockDim / (2 D)
 // (2 D threads cover the rows and columns); the n shares join in shared memory.  Bound
-// by the latency of dependent reads (the unit, its parts), so eight parts' loads are in
-// flight at a time.
+// by the latency of dependent reads (the unit, its parts) while there are few units of
+// many parts: the WIDE form has 512 threads and eight parts' loads in flight.  With more
+// blocks than SMs (many units, of few parts) the narrow form keeps four blocks on an SM
+// (256 row tiles of 128 over 8192 keys: 24 us wide).
 constexpr int kJoinRows = 16;
-constexpr int kJoinThreads = 512;
-constexpr int kJoinFlight = 8;
 
-template <class E>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttnParams p) {
+template <class E, bool WIDE>
+__global__ void __launch_bounds__(512, WIDE ? 1 : 2) join_kernel(const __grid_constant__ AttnParams p) {
     extern __shared__ float joined[];  // [n - 1][10][2 D]
+    constexpr int kJoinFlight = WIDE ? 8 : 3;
     const int groups = (p.RT + kJoinRows - 1) / kJoinRows;
     const int unit = blockIdx.x / groups;
     const int width = 2 * p.D, n = blockDim.x / width, split = threadIdx.x / width, tid = threadIdx.x - split * width;
@@ -388,7 +395,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 
 // -------------------------------------------------------- the few-rows kernel
 // Row groups of 16 (the M = 16 of m16n8k16), NRG of them per tile.
-//   warps NCW..     producers: 64-key tiles of K and V through an NST-stage ring
+//   warps NCW..     prepare the next segment: turned queries, mask bits, rows' limits
+//   last warp       TMA producer: 64-key tiles of K and V through an NST-stage ring
 //   warps 0..NCW-1  consumers: the 32-key halves of the tiles go round the NCW /
 //                   NRG warps of each row group: S = Q K^T and O += P V on mma.sync
 //                   with the online softmax in registers
@@ -399,8 +407,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 template <int DP>
 struct Layout {
     static constexpr int NCW = DP <= 128 ? 8 : 4;
-    static constexpr int NPW = 4;
-    static constexpr int THREADS = 32 * (NCW + NPW);
+    // warps NCW .. that prepare segments; the last one of all is the producer
+    static constexpr int NPREP = 3;
+    static_assert(32 * NPREP % (DP / 8) == 0, "whole rows between a thread's chunks");
+    static constexpr int THREADS = 32 * (NCW + NPREP + 1);
     static constexpr int NBOX = DP / 64;  // 64-element boxes (128 B, SWIZZLE_128B)
     static constexpr int BOX_BYTES = KT * 128;
     static constexpr int TILE = NBOX * BOX_BYTES;
@@ -463,48 +473,68 @@ __device__ __forceinline__ void mma16816<BF16>(float* c, const uint32_t* a, uint
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Loads 16 bytes of row r of a row tile and turns them; hi + lo (see above).
-// Zeros for rows that are padding or whose position lies outside the tables.
-template <class E>
-__device__ __forceinline__ void load_q_chunk(const AttnParams& p, const Segment& g, int r, int ch, uint4& hi, uint4& lo) {
+// Position of row r, -1 for a row that sees nothing: padding, or a position outside the
+// tables.  (Without tables the position does not matter.)
+__device__ __forceinline__ int row_position(const AttnParams& p, const Segment& g, int r) {
     const int t = p.by_G.div(r);
-    hi = lo = uint4{0u, 0u, 0u, 0u};
-    if (r >= p.rows || t >= g.n || ch * 8 >= p.D) return;
-    int pos = 0;
-    if (p.cos != nullptr) {
-        pos = p.positions != nullptr ? p.positions[static_cast<int64_t>(g.b) * p.t.T + t] : g.L + t;
-        if (static_cast<unsigned>(pos) >= static_cast<unsigned>(p.rope_rows)) return;
+    if (r >= p.rows || t >= g.n) return -1;
+    if (p.cos == nullptr) return 0;
+    const int pos = p.positions != nullptr ? p.positions[static_cast<int64_t>(g.b) * p.t.T + t] : g.L + t;
+    return static_cast<unsigned>(pos) < static_cast<unsigned>(p.rope_rows) ? pos : -1;
+}
+
+// Loads chunk ch (16 bytes) of N rows of Q, r0, r0 + STEP, .. at positions pos[k], and turns
+// them; hi + lo (see above).  Zeros for rows that see nothing.  All loads are issued before
+// the first is used: one by one each would wait for two reads in turn.
+template <class E, int N, int STEP>
+__device__ __forceinline__ void load_q(const AttnParams& p, const Segment& g, int r0, const int* pos, int ch,
+                                       uint4* hi, uint4* lo) {
+    const uint16_t* base = p.q + g.b * p.qsb + g.kvh * p.G * p.qsh + ch * 8;
+    const bool col = ch * 8 < p.D;
+    float4 c[N], s[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const int r = r0 + k * STEP, t = p.by_G.div(r);
+        hi[k] = lo[k] = uint4{0u, 0u, 0u, 0u};
+        if (pos[k] >= 0 && col) hi[k] = *reinterpret_cast<const uint4*>(base + (r - t * p.G) * p.qsh + t * p.qss);
     }
-    hi = *reinterpret_cast<const uint4*>(p.q + g.b * p.qsb + (g.kvh * p.G + r - t * p.G) * p.qsh + t * p.qss + ch * 8);
-    hi.x ^= p.flip;
-    hi.y ^= p.flip;
-    hi.z ^= p.flip;
-    hi.w ^= p.flip;
-    if (p.cos == nullptr) return;
-    const int64_t at = static_cast<int64_t>(pos) * (p.D / 2) + ch * 4;
-    const float4 c = __ldg(reinterpret_cast<const float4*>(p.cos + at));
-    const float4 s = __ldg(reinterpret_cast<const float4*>(p.sin + at));
-    turn_split<E>(hi.x, lo.x, c.x, s.x);
-    turn_split<E>(hi.y, lo.y, c.y, s.y);
-    turn_split<E>(hi.z, lo.z, c.z, s.z);
-    turn_split<E>(hi.w, lo.w, c.w, s.w);
+    if (p.cos != nullptr) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int64_t at = pos[k] >= 0 && col ? static_cast<int64_t>(pos[k]) * (p.D / 2) + ch * 4 : 0;
+            c[k] = __ldg(reinterpret_cast<const float4*>(p.cos + at));
+            s[k] = __ldg(reinterpret_cast<const float4*>(p.sin + at));
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        hi[k].x ^= p.flip;
+        hi[k].y ^= p.flip;
+        hi[k].z ^= p.flip;
+        hi[k].w ^= p.flip;
+    }
+    if (p.cos != nullptr) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            turn_split<E>(hi[k].x, lo[k].x, c[k].x, s[k].x);
+            turn_split<E>(hi[k].y, lo[k].y, c[k].y, s[k].y);
+            turn_split<E>(hi[k].z, lo[k].z, c[k].z, s[k].z);
+            turn_split<E>(hi[k].w, lo[k].w, c[k].w, s[k].w);
+        }
+    }
 }
 
 // Keys row r sees: [lo, hi), and with a mask the drafted slots from L on by bit.
-// A row that is padding, or whose position lies outside the tables, sees none.
-__device__ __forceinline__ void row_limits(const AttnParams& p, const Segment& g, int r, int ta, const int* ctx_lo,
+__device__ __forceinline__ void row_limits(const AttnParams& p, const Segment& g, int r, int pos, const int* ctx_lo,
                                            int& lo, int& hi) {
-    const int t = p.by_G.div(r);
-    bool ok = r < p.rows && t < g.n;
-    if (ok && p.cos != nullptr) {
-        const int pos = p.positions != nullptr ? p.positions[static_cast<int64_t>(g.b) * p.t.T + t] : g.L + t;
-        ok = static_cast<unsigned>(pos) < static_cast<unsigned>(p.rope_rows);
-    }
-    if (!ok) {
+    if (pos < 0) {
         lo = 1;
         hi = 0;
-    } else if (p.mask != nullptr) {
-        lo = ctx_lo[t - ta];
+        return;
+    }
+    const int t = p.by_G.div(r);
+    if (p.mask != nullptr) {
+        lo = p.window > 0 ? ctx_lo[t - p.by_G.div(g.rt * p.RT)] : 0;
         hi = g.s.hi;
     } else {
         lo = p.window > 0 ? max(0, g.L + t + 1 - p.window) : 0;
@@ -512,99 +542,67 @@ __device__ __forceinline__ void row_limits(const AttnParams& p, const Segment& g
     }
 }
 
-// 16 bytes to shared memory.
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint64_t pol) {
-    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(pol)
-                 : "memory");
+// One lane of the (converged) warp, always the same.  The work it is elected for stays in a
+// warp-uniform loop, and values that are the same in all lanes pass through a shuffle, so
+// that the compiler keeps them in uniform registers, where TMA and MMA instructions take
+// their operands: issued by `if (lane == 0)` a TMA box cost 180 cycles instead of 30 to 65
+// and an MMA 87 instead of 38.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t leader;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(leader)
+        :
+        : "memory");
+    return leader != 0;
 }
-// The same, or 16 zero bytes (src is then not read).
-__device__ __forceinline__ void cp_async16_or_zero(uint32_t dst, const void* src, bool real) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
-// Arrives on `bar` (once per thread) when the thread's copies so far have landed.
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
-// The producers' part of a segment (NPW warps, ptid = thread among them): its tiles
-// into the ring by 16-byte asynchronous copies, thread -> one chunk column and every
-// (32 NPW / chunks)-th row.  Rows that are not keys of the unit (behind a page's end,
-// outside what its rows see, on a page outside the cache) become zeros, so that
-// whatever lies there cannot reach the products.  Copies by TMA boxes were bound by
-// the engine's rate for pages below 64 slots: about 180 cycles a box, 16 boxes per
-// tile at 16 slots (ragged decode batch of 552 MB: 173 us).  i: running tile number.
-// False when a wait expired.
+// The producer's part of a segment (one warp): its tiles into the ring by TMA boxes of one
+// page's rows (at most KT) x 64 columns; rows behind a page's end, columns behind head_dim
+// and pages outside the cache are zero fill.  A copy alone reaches 6.7 TB/s with boxes of
+// any height from 8 rows.  i: running tile number; `filled`, `issued`: for drain().  False
+// when a wait expired.
 template <class L>
-__device__ __forceinline__ bool produce(const AttnParams& p, const Segment& g, int i, uint32_t bars, uint32_t ring,
-                                        const Abort& ab, int ptid) {
-    constexpr int NCH = L::NBOX * 8;            // 16-byte chunks per row
-    constexpr int RSTEP = 32 * L::NPW / NCH;    // rows between a thread's copies
+__device__ __forceinline__ bool produce(const AttnParams& p, const CUtensorMap* tmK, const CUtensorMap* tmV,
+                                        const Segment& g, int i, uint32_t bars, uint32_t ring, uint32_t& filled,
+                                        int& issued, const Abort& ab, int lane) {
     const uint64_t pol = policy_evict_first();
-    const int lane = ptid & 31, ch = ptid % NCH, r0 = ptid / NCH;
-    const bool col = ch * 8 < p.D;              // the columns behind head_dim stay zero
+    const int ppt = uniform(p.tpp == 0 ? KT >> p.t.Pshift : 1), box = min(p.t.P, KT) * 128;  // pages per tile
     const int* pages = p.t.pages + g.b * p.t.stride;
-    char* const kbase = p.kc.head(g.kvh, ch);
-    char* const vbase = p.vc.head(g.kvh, ch);
-    const uint32_t dst0 = chunk_off(KT, r0, ch);  // (8 rows further the swizzle is the same)
-    const int shift = p.tpp == 0 ? p.t.Pshift : 31;           // row of the tile -> page of the tile
-    const int mask = p.tpp == 0 ? p.t.Pmask : KT - 1;          // and row within it
-    const int ppt = p.tpp == 0 ? KT >> p.t.Pshift : 1;         // pages per tile
-    const int tile0 = g.s.t0 + g.first;
-    int lp = p.tpp == 0 ? tile0 * ppt : p.by_tpp.div(tile0);   // logical page, first row in it
-    int sub = p.tpp == 0 ? 0 : (tile0 - lp * p.tpp) * KT;
+    const int tile0 = g.s.t0 + g.first, count = uniform(g.count), kvh = uniform(g.kvh);
+    i = uniform(i);
+    int lp = uniform(p.tpp == 0 ? tile0 * ppt : p.by_tpp.div(tile0));  // logical page, first row in it
+    int sub = uniform(p.tpp == 0 ? 0 : (tile0 - lp * p.tpp) * KT);
     int win = -1, ids = -1;  // 32 consecutive page table entries, one per lane
-    uint32_t bad = 0;        // of these, the ones outside the cache
-    for (int k = 0; k < g.count; ++k, ++i) {
+    for (int k = 0; k < count; ++k, ++i) {
         if (lp / 32 != win) {
             win = lp / 32;
             const int e = win * 32 + lane;
             ids = e < p.t.max_pages ? __ldg(pages + e) : -1;
-            bad = __ballot_sync(0xffffffffu, static_cast<unsigned>(ids) >= static_cast<unsigned>(p.t.num_pages));
+            if (static_cast<unsigned>(ids) >= static_cast<unsigned>(p.t.num_pages)) ids = -1;  // zero fill
         }
-        const int k0 = lp * p.t.P + sub;  // the tile's rows are the keys k0 ..
-        const int lo = g.s.lo - k0, hi = min(g.s.hi - k0, p.tpp == 0 ? KT : min(KT, p.t.P - sub));
-        const uint32_t here = (bad >> (lp & 31)) & ((1u << ppt) - 1u);
         const int s = i % L::NST;
-        bool ok = mbar_wait(bars + 8u * (L::NST + s), (i / L::NST & 1) ^ 1, ab, 0x601);
-        if (!__all_sync(0xffffffffu, ok)) return false;
-        const uint32_t dst = ring + s * L::STAGE;
-        const bool inner = lo <= 0 && hi == KT && here == 0;
-        if (inner && p.tpp != 0) {
-            // a tile inside one page
-            const int page = __shfl_sync(0xffffffffu, ids, lp & 31);
-            const char* ks = p.kc.at(kbase, page, sub + r0);
-            const char* vs = p.vc.at(vbase, page, sub + r0);
-            if (col) {
+        const uint32_t full = bars + 8u * s, dst = ring + s * L::STAGE;
+        if (!__all_sync(0xffffffffu, mbar_wait(bars + 8u * (L::NST + s), (i / L::NST & 1) ^ 1, ab, 0x601))) return false;
+        filled |= 1u << s;
+        issued = i;
+        if (elect_one()) mbar_arrive_expect_tx(full, L::STAGE);
+        __syncwarp();
+        for (int j = 0; j < ppt; ++j) {
+            const int page = uniform(__shfl_sync(0xffffffffu, ids, (lp + j) & 31));
+            if (elect_one()) {
 #pragma unroll
-                for (int r = r0, j = 0; j < KT / RSTEP; r += RSTEP, ++j) {
-                    const uint32_t d = dst + (RSTEP % 8 == 0 ? dst0 + j * RSTEP * 128 : chunk_off(KT, r, ch));
-                    cp_async16(d, ks, pol);
-                    cp_async16(d + L::TILE, vs, pol);
-                    ks += static_cast<uint64_t>(p.kc.ss) * RSTEP;
-                    vs += static_cast<uint64_t>(p.vc.ss) * RSTEP;
-                }
+                for (int bx = 0; bx < L::NBOX; ++bx)
+                    tma_load_4d(dst + bx * L::BOX_BYTES + j * box, tmK, full, bx * 64, sub, kvh, page, pol);
+#pragma unroll
+                for (int bx = 0; bx < L::NBOX; ++bx)
+                    tma_load_4d(dst + L::TILE + bx * L::BOX_BYTES + j * box, tmV, full, bx * 64, sub, kvh, page, pol);
             }
-        } else {
-#pragma unroll 4
-            for (int r = r0, j = 0; j < KT / RSTEP; r += RSTEP, ++j) {
-                const int page = __shfl_sync(0xffffffffu, ids, (lp + (r >> shift)) & 31);
-                const uint32_t d = dst + (RSTEP % 8 == 0 ? dst0 + j * RSTEP * 128 : chunk_off(KT, r, ch));
-                const int row = sub + (r & mask);
-                const char* ks = p.kc.at(kbase, page, row);
-                const char* vs = p.vc.at(vbase, page, row);
-                if (!col) continue;
-                if (inner) {
-                    cp_async16(d, ks, pol);
-                    cp_async16(d + L::TILE, vs, pol);
-                } else {
-                    const bool real = r >= lo && r < hi && !(here >> (r >> shift) & 1u);
-                    cp_async16_or_zero(d, real ? ks : kbase, real);
-                    cp_async16_or_zero(d + L::TILE, real ? vs : vbase, real);
-                }
-            }
+            __syncwarp();
         }
-        cp_async_arrive(bars + 8u * s);
         if (p.tpp == 0) {
             lp += ppt;
         } else if ((sub += KT) >= p.t.P) {
@@ -615,8 +613,32 @@ __device__ __forceinline__ bool produce(const AttnParams& p, const Segment& g, i
     return true;
 }
 
+// After an expired wait: the copies in flight land before the CTA leaves.  Slot s last
+// received tile j, the largest j <= issued with j % NST == s.
+template <class L>
+__device__ __forceinline__ void drain(uint32_t bars, uint32_t filled, int issued) {
+    for (int s = 0; s < L::NST; ++s)
+        if (filled >> s & 1u) {
+            const int j = issued - ((issued - s) % L::NST + L::NST) % L::NST;
+            mbar_wait_drain(bars + 8u * s, j / L::NST & 1);
+        }
+}
+
+// Slots no row of the unit sees may hold anything (0 * NaN): zeros over the V rows of a tile
+// whose keys k0 + r lie outside the unit's, rows r0 .. r0 + rows - 1, by n threads.
+template <int DP>
+__device__ __forceinline__ void zero_unseen_v(uint8_t* v, const Span& s, int k0, int r0, int rows, int tid, int n) {
+    for (int idx = tid; idx < rows * (DP / 8); idx += n) {
+        const int r = r0 + idx / (DP / 8);
+        if (k0 + r < s.lo || k0 + r >= s.hi)
+            *reinterpret_cast<uint4*>(v + chunk_off(KT, r, idx % (DP / 8))) = uint4{0u, 0u, 0u, 0u};
+    }
+    fence_proxy_async_smem();  // before the tensor core's reads, or the slot's next copy
+}
+
 template <class E, int DP>
 __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
+    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
     const __grid_constant__ AttnParams p) {
     using L = Layout<DP>;
     constexpr int NCW = L::NCW;
@@ -635,21 +657,17 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int s = 0; s < L::NST; ++s) {
-            mbar_init(full_bar(s), 32 * L::NPW);
+            mbar_init(full_bar(s), 1);
             mbar_init(empty_bar(s), NRG * min(2, NTG));
         }
         for (int k = 0; k < L::NQ; ++k) {
-            mbar_init(bars + 8u * (L::Q_FULL + k), 32 * L::NPW);
+            mbar_init(bars + 8u * (L::Q_FULL + k), 32 * L::NPREP);
             mbar_init(bars + 8u * (L::Q_EMPTY + k), 1);
         }
         fence_barrier_init();
+        prefetch_tmap(&tmK);
+        prefetch_tmap(&tmV);
     }
-    // columns behind head_dim are never copied: zero for good
-    if (p.D < DP)
-    for (int idx = threadIdx.x; idx < 2 * L::NST * KT * (DP / 8); idx += L::THREADS)
-        if (idx % (DP / 8) * 8 >= p.D)
-            *reinterpret_cast<uint4*>(ring + idx / (DP / 8) / KT * L::TILE +
-                                      chunk_off(KT, idx / (DP / 8) % KT, idx % (DP / 8))) = uint4{0u, 0u, 0u, 0u};
     warm_params(p);
     __syncthreads();
     grid_dependency_wait();
@@ -667,6 +685,8 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
     float* part = reinterpret_cast<float*>(smem + L::OFF_PART);
     const float sl2 = p.scale_log2;
     bool aborted = false;    // consumers: a wait expired
+    uint32_t filled = 0;     // producer: slots that received a copy, last tile issued
+    int issued = -1;
     int i0 = 0, e = 0, nseg = 0;  // running tile number of the segment's first tile; segments so far
     for (int pos = begin; pos < end;) {
         const Segment g = segment_at(p, pre, pos, end, e);
@@ -679,25 +699,45 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
         uint32_t* words = reinterpret_cast<uint32_t*>(smem + L::OFF_MASK + qb * L::MASK_BYTES);
         int* ctx_lo = reinterpret_cast<int*>(words + L::MAX_RT * (kMaxTree / 32));
         int2* limits = reinterpret_cast<int2*>(ctx_lo + L::MAX_RT);
+        if (warp == NCW + L::NPREP) {
+            if (!produce<L>(p, &tmK, &tmV, g, i0, bars, smem_u32(ring), filled, issued, ab, lane)) {
+                drain<L>(bars, filled, issued);
+                break;
+            }
+            i0 += g.count;
+            continue;
+        }
         if (warp >= NCW) {
-            // Q of the row tile (turned, hi and lo), the mask bits and the rows' limits, then the tiles
+            // Q of the row tile (turned, hi and lo), the mask bits and the rows' limits
             const int ptid = threadIdx.x - 32 * NCW;
             if (!__all_sync(0xffffffffu, mbar_wait(bars + 8u * (L::Q_EMPTY + qb), (qn & 1) ^ 1, ab, 0x603))) break;
-            for (int idx = ptid; idx < p.RT * (DP / 8); idx += 32 * L::NPW) {
-                const int r = idx / (DP / 8), ch = idx % (DP / 8);
-                uint4 hi, lo;
-                load_q_chunk<E>(p, g, row0 + r, ch, hi, lo);
-                *reinterpret_cast<uint4*>(qmem + chunk_off(p.RT, r, ch)) = hi;
-                *reinterpret_cast<uint4*>(qmem + L::Q_BYTES + chunk_off(p.RT, r, ch)) = lo;
+            constexpr int STEP = 32 * L::NPREP / (DP / 8);  // rows between a thread's chunks
+            for (int lr = ptid / (DP / 8); lr < p.RT; lr += 2 * STEP) {
+                const int ch = ptid % (DP / 8);
+                int pos[2];
+                uint4 hi[2], lo[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    pos[k] = lr + k * STEP < p.RT ? row_position(p, g, row0 + lr + k * STEP) : -1;
+                load_q<E, 2, STEP>(p, g, row0 + lr, pos, ch, hi, lo);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    if (lr + k * STEP >= p.RT) continue;
+                    *reinterpret_cast<uint4*>(qmem + chunk_off(p.RT, lr + k * STEP, ch)) = hi[k];
+                    *reinterpret_cast<uint4*>(qmem + L::Q_BYTES + chunk_off(p.RT, lr + k * STEP, ch)) = lo[k];
+                }
             }
             if (p.mask != nullptr) {
-                build_mask(p, g, words, ctx_lo, ptid, 32 * L::NPW);
-                named_bar_sync(2, 32 * L::NPW);
+                build_mask(p, g, words, ptid, 32 * L::NPREP);
+                if (p.window > 0) {
+                    named_bar_sync(2, 32 * L::NPREP);
+                    trim_mask(p, g, words, ctx_lo, ptid, 32 * L::NPREP);
+                    named_bar_sync(2, 32 * L::NPREP);
+                }
             }
-            if (ptid < p.RT) row_limits(p, g, row0 + ptid, ta, ctx_lo, limits[ptid].x, limits[ptid].y);
+            if (ptid < p.RT)
+                row_limits(p, g, row0 + ptid, row_position(p, g, row0 + ptid), ctx_lo, limits[ptid].x, limits[ptid].y);
             mbar_arrive(bars + 8u * (L::Q_FULL + qb));
-            if (!produce<L>(p, g, i0, bars, smem_u32(ring), ab, ptid)) break;
-            i0 += g.count;
             continue;
         }
         // ------------------------------------------------------------ consumers
@@ -747,6 +787,11 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
             const bool none = valid <= 0 || k0 >= g.s.hi || k0 + 32 <= g.s.lo;
             const uint32_t kb = smem_u32(ring) + s * L::STAGE, vb = kb + L::TILE;
             const bool edge = valid < 32 || k0 < all_lo || k0 + 32 > all_hi;
+            const bool dirty = !none && (k0 < g.s.lo || k0 + 32 > g.s.hi);
+            if (dirty) {
+                zero_unseen_v<DP>(ring + s * L::STAGE + L::TILE, g.s, k0 - kh, kh, 32, lane, 32);
+                __syncwarp();
+            }
             if (!none) {
                 float sc[4][4];
 #pragma unroll
@@ -915,10 +960,7 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
         if (threadIdx.x == 0) mbar_arrive(bars + 8u * (L::Q_EMPTY + qb));
         i0 += g.count;
     }
-    if (warp >= NCW)
-        cp_async_wait_all();  // after an expired wait too, no copy outlives the CTA
-    else
-        zero_empty_units(p, threadIdx.x, 32 * NCW);
+    if (warp < NCW) zero_empty_units(p, threadIdx.x, 32 * NCW);
 }
 
 }  // namespace paged

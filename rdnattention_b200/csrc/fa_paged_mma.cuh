@@ -8,8 +8,8 @@
 //
 //   warps 0..3, 4..7   two softmax groups (thread = row = TMEM lane); key tile i of
 //                      the CTA goes to group i & 1
-//   warps 8..11        producers (produce(), as in the few-rows kernel)
-//   warp 12, warp 13   one lane issues S = Q K^T, one lane O += P V
+//   warp 8             TMA producer, as in the few-rows kernel (warp 9: none)
+//   warps 10, 11       issue S = Q K^T and O += P V, each for every other tile
 //
 // TMEM (512 columns at head_dim 128): Q hi and lo as the A operand of S = Q K^T
 // (hi + lo, see the few-rows kernel: a query in shared memory would be read again by
@@ -31,28 +31,34 @@ namespace paged {
 
 template <int DP>
 struct MmaLayout {
-    static constexpr int NPW = 4;
     static constexpr int NSW = 8;                       // softmax warps
-    static constexpr int THREADS = 32 * (NSW + NPW + 4);
+    static constexpr int THREADS = 32 * (NSW + 4);
+    // Registers: LAUNCH_REGS are the most that 12 warps can have each; a few move from the
+    // other four warps, which need far fewer, to the softmax warps.
+    static constexpr int LAUNCH_REGS = 168, SOFTMAX_REGS = 184, OTHER_REGS = 136;
+    static_assert(NSW * SOFTMAX_REGS + 4 * OTHER_REGS <= (NSW + 4) * LAUNCH_REGS,
+                  "register split exceeds the launch allocation");
     static constexpr int NBOX = DP / 64;
     static constexpr int BOX_BYTES = KT * 128;
     static constexpr int TILE = NBOX * BOX_BYTES;
     static constexpr int STAGE = 2 * TILE;
-    static constexpr int NST = 6;
+    static constexpr int NST = DP == 64 ? 12 : 6;  // 192 KB
     static constexpr int NSB = 4;  // S buffers
     static constexpr int RT = 128;
     static constexpr int NW = kMaxTree / 32;
     // barriers (8 bytes each): full [NST], empty [NST], then
     static constexpr int S_FULL = 2 * NST, P_FULL = S_FULL + NSB, PV_DONE = P_FULL + NSB,  // [NSB] each
         TOKEN = PV_DONE + NSB,                                                             // [2 groups][4 warps]
-        O_FULL = TOKEN + 8, Q_FULL = O_FULL + 1, DRAIN = Q_FULL + 1, N_BARS = DRAIN + 2;
-    static constexpr int OFF_TMEM = 8 * N_BARS, OFF_ABORT = OFF_TMEM + 4;
+        O_FULL = TOKEN + 8, Q_FULL = O_FULL + 1, DRAIN = Q_FULL + 2, N_BARS = DRAIN + 2;  // Q_FULL [2 issuers]
+    static constexpr int OFF_TMEM = 8 * N_BARS, OFF_ABORT = OFF_TMEM + 4, OFF_KEPT = OFF_ABORT + 4;
     static constexpr int OFF_RING = 1024;
     static constexpr int OFF_MASK = OFF_RING + NST * STAGE;  // [RT][NW], then [RT]
     static constexpr int OFF_M = OFF_MASK + RT * NW * 4 + RT * 4;  // [RT] reference maxima
     static constexpr int OFF_L = OFF_M + RT * 4;                   // [2][RT] row sums
     static constexpr int OFF_SEG = OFF_L + 2 * RT * 4;             // [NSW] Segment
-    static constexpr int OFF_PRE = OFF_SEG + NSW * 64;
+    static constexpr int OFF_STAGE = OFF_SEG + NSW * 64;  // [NSW] 32 rows of 64 bytes (see row_chunk)
+    static constexpr int STAGE_BYTES = 32 * 64;
+    static constexpr int OFF_PRE = OFF_STAGE + NSW * STAGE_BYTES;
     static_assert(sizeof(Segment) <= 64, "a segment's slot");
     static constexpr int SMEM_BYTES = OFF_PRE + kMaxList * 4 + 1024;  // + alignment slack
     static_assert(SMEM_BYTES <= 232448, "shared memory of one CTA");
@@ -73,14 +79,25 @@ struct AbFormat<BF16> {
     static constexpr uint32_t value = 1;
 };
 
-// Row max of 32 values: 8 chains of three-input max.
-__device__ __forceinline__ float max32(const float* x) {
+// Row max of N values: 8 chains of three-input max.
+template <int N>
+__device__ __forceinline__ float row_max(const float* x) {
     float m[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m[i] = fmax3(x[i], x[i + 8], x[i + 16]);
+    for (int i = 0; i < 8; ++i) m[i] = fmaxf(x[i], x[i + 8]);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m[i] = fmaxf(m[i], x[i + 24]);
+    for (int c = 16; c < N; c += 16)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m[i] = fmax3(m[i], x[c + i], x[c + 8 + i]);
     return fmax3(fmax3(m[0], m[1], m[2]), fmax3(m[3], m[4], m[5]), fmaxf(m[6], m[7]));
+}
+
+// A warp's exchange between rows held by lanes (TMEM) and rows in global memory: 32 rows of
+// four 16-byte chunks, placed so that both orders of access are free of bank conflicts.
+// Four lanes side by side take one row's 64 bytes of global memory; a lane on its own per
+// row would touch 32 lines with every access (the query's load took 7000 cycles so).
+__device__ __forceinline__ uint4* row_chunk(uint8_t* stage, int row, int c) {
+    return reinterpret_cast<uint4*>(stage + row * 64 + ((c ^ (row >> 1 & 3)) << 4));
 }
 
 // Bits lo .. hi - 1 (clamped to 0 .. 64).
@@ -101,7 +118,9 @@ __device__ __forceinline__ uint64_t draft_bits(const uint32_t* words, int nw, in
 }
 
 template <class E, int DP>
-__global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel(
+    const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+    const __grid_constant__ AttnParams p) {
     using L = MmaLayout<DP>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = smem_raw + (-smem_u32(smem_raw) & 1023u);  // (an offset keeps the address space known)
@@ -115,7 +134,7 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
     if (threadIdx.x == 0) {
         *abort_flag = 0;
         for (int s = 0; s < L::NST; ++s) {
-            mbar_init(bar(s), 32 * L::NPW);
+            mbar_init(bar(s), 1);
             mbar_init(bar(L::NST + s), 1);
         }
         for (int k = 0; k < L::NSB; ++k) {
@@ -126,17 +145,13 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
         for (int k = 0; k < 8; ++k) mbar_init(bar(L::TOKEN + k), 1);
         mbar_init(bar(L::O_FULL), 1);
         mbar_init(bar(L::Q_FULL), L::NSW);
+        mbar_init(bar(L::Q_FULL + 1), L::NSW);
         mbar_init(bar(L::DRAIN), 1);
         mbar_init(bar(L::DRAIN + 1), 1);
         fence_barrier_init();
+        prefetch_tmap(&tmK);
+        prefetch_tmap(&tmV);
     }
-    // columns behind head_dim are never copied: zero for good
-    if (p.D < DP)
-    for (int idx = threadIdx.x; idx < 2 * L::NST * KT * (DP / 8); idx += L::THREADS)
-        if (idx % (DP / 8) * 8 >= p.D)
-            *reinterpret_cast<uint4*>(ring + idx / (DP / 8) / KT * L::TILE +
-                                      chunk_off(KT, idx / (DP / 8) % KT, idx % (DP / 8))) = uint4{0u, 0u, 0u, 0u};
-    fence_proxy_async_smem();
     warm_params(p);
     __syncthreads();
     grid_dependency_wait();
@@ -147,94 +162,123 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
         return;
     }
     const int begin = cta_begin(sched, blockIdx.x), end = cta_begin(sched, blockIdx.x + 1);
+    if (threadIdx.x == 0) {
+        volatile int* k = reinterpret_cast<volatile int*>(smem + L::OFF_KEPT);
+        k[0] = begin;
+        k[1] = end;
+        k[2] = sched.q;
+        k[3] = sched.r;
+    }
     if (warp == 0) {
         tmem_alloc(smem_u32(smem + L::OFF_TMEM), L::TMEM_COLS);
         tmem_relinquish();
     }
     tc_fence_before();
-    // the producers need no TMEM: they start on the ring while the rest waits for it
-    const bool producer = warp >= L::NSW && warp < L::NSW + L::NPW;
-    if (!producer) named_bar_sync(2, L::THREADS - 32 * L::NPW);
+    // the producer needs no TMEM: it starts on the ring while the rest waits for it
+    const bool producer = warp == L::NSW;
+    if (!producer) named_bar_sync(2, L::THREADS - 32);
     tc_fence_after();
     const uint32_t tmem = producer ? 0 : *reinterpret_cast<volatile uint32_t*>(smem + L::OFF_TMEM);
 
+    // (the softmax warps read these again where they need them: registers are for the scores)
+    volatile int* const kept = reinterpret_cast<volatile int*>(smem + L::OFF_KEPT);
+
     int i0 = 0, e = 0;  // running tile number of the segment's first tile
-    if (producer) {
-        for (int pos = begin; pos < end;) {
-            const Segment g = segment_at(p, pre, pos, end, e);
-            if (!produce<L>(p, g, i0, bars, smem_u32(ring), ab, threadIdx.x - 32 * L::NSW)) break;
-            i0 += g.count;
-            pos = g.next;
-        }
-        cp_async_wait_all();  // after an expired wait too, no copy outlives the CTA
-    } else if (warp >= L::NSW + L::NPW) {
-        // ------------------------------------------------------------ MMA issuers
-        const int w = warp - (L::NSW + L::NPW);  // 0: S = Q K^T, 1: O += P V, others: idle
-        if (w < 2) {
+    if (warp >= L::NSW) {
+        regs_decrease<L::OTHER_REGS>();
+        if (producer) {
+            uint32_t filled = 0;
+            int issued = -1;
+            for (int pos = begin; pos < end;) {
+                const Segment g = segment_at(p, pre, pos, end, e);
+                if (!produce<L>(p, &tmK, &tmV, g, i0, bars, smem_u32(ring), filled, issued, ab, lane)) {
+                    drain<L>(bars, filled, issued);
+                    break;
+                }
+                i0 += g.count;
+                pos = g.next;
+            }
+        } else if (warp >= L::NSW + 2) {
+            // ------------------------------------------------------------ MMA issuers
+            // Warp w issues both products of the tiles i with i & 1 == w: O += P V of tile i, then
+            // S = Q K^T of tile i + 4 into the buffer that P V has just read (one thread's products
+            // run in the order of their issue), so that one warp's waits fall into the other's
+            // products.  The whole warp runs the loop and one elected lane issues: operands that are
+            // the same in all lanes (the shuffles tell the compiler) stay in uniform registers, where
+            // the MMA takes them; issued by a lane in a branch of its own, each cost 87 cycles.
+            const int w = warp - (L::NSW + 2);
             constexpr uint32_t IDESC_QK = instr_desc(1u, AbFormat<E>::value, 0u, 128, KT);
             constexpr uint32_t IDESC_PV = instr_desc(1u, AbFormat<E>::value, 1u, 128, DP);
             const uint64_t kd = smem_desc(smem_u32(ring), 16, 1024, 2);
             const uint64_t vd = smem_desc(smem_u32(ring + L::TILE), L::BOX_BYTES, 1024, 2);
-            const int halves = p.cos != nullptr ? 2 : 1;  // a query that is not turned has no lo
-            int seg = 0, ok = 1;
+            const bool split = p.cos != nullptr;  // a query that is not turned has no lo
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            int seg = 0;
+            bool ok = true;
+            auto wait = [&](int i, int parity, int site) {
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(bar(i), parity, ab, site));
+                return ok;
+            };
+            auto issue_qk = [&](int i) {
+                const int s = i % L::NST, sb = i % L::NSB;
+                if (!wait(s, i / L::NST & 1, 0x713)) return;
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t at = kd + (static_cast<uint32_t>(s * L::STAGE) >> 4);
+                    const uint32_t tS = tm + L::S0 + sb * KT;
+#pragma unroll
+                    for (int kk = 0; kk < DP / 16; ++kk)
+                        mma_f16_ts(tS, tm + L::QHI + kk * 8, at + ((kk / 4 * L::BOX_BYTES + kk % 4 * 32) >> 4), IDESC_QK,
+                                   kk > 0);
+                    if (split) {
+#pragma unroll
+                        for (int kk = 0; kk < DP / 16; ++kk)
+                            mma_f16_ts(tS, tm + L::QLO + kk * 8, at + ((kk / 4 * L::BOX_BYTES + kk % 4 * 32) >> 4),
+                                       IDESC_QK, 1);
+                    }
+                    tc_commit(bar(L::S_FULL + sb));
+                }
+                __syncwarp();
+            };
             for (int pos = begin; pos < end && ok;) {
                 const Segment g = segment_at(p, pre, pos, end, e);
                 pos = g.next;
                 if (g.count == 0) continue;
-                if (lane == 0) {
-                    if (w == 0) {
-                        ok = mbar_wait(bar(L::Q_FULL), seg++ & 1, ab, 0x711);
-                        tc_fence_after();
-                    }
-                    for (int i = i0; ok && i < i0 + g.count; ++i) {
-                        const int s = i % L::NST, sb = i % L::NSB;
-                        const uint32_t slot = static_cast<uint32_t>(s * L::STAGE) >> 4, tS = tmem + L::S0 + sb * KT;
-                        if (w == 0) {
-                            // the buffer's last P has been multiplied, the keys are there
-                            ok = mbar_wait(bar(L::PV_DONE + sb), (i / L::NSB & 1) ^ 1, ab, 0x712) &&
-                                 mbar_wait(bar(s), i / L::NST & 1, ab, 0x713);
-                            if (!ok) break;
-                            // the copies were written through the generic proxy, the products
-                            // read through the async one
-                            fence_proxy_async_smem();
-                            tc_fence_after();
-                            for (int half = 0; half < halves; ++half)
+                const int behind = __shfl_sync(0xffffffffu, i0 + g.count, 0), start = __shfl_sync(0xffffffffu, i0, 0);
+                const int first = start + ((w - start) & 1);
+                // (signalled for segments with a tile of this warp only: no phase passes unseen)
+                if (first < behind && !wait(L::Q_FULL + w, seg++ & 1, 0x711)) break;
+                tc_fence_after();
+                for (int i = first; i < behind && i < first + L::NSB; i += 2) issue_qk(i);
+                for (int i = first; ok && i < behind; i += 2) {
+                    const int s = i % L::NST, sb = i % L::NSB;
+                    // both warps add to O: the tile before must have been added
+                    if (!wait(L::P_FULL + sb, i / L::NSB & 1, 0x715)) break;
+                    if (i > start && !wait(L::PV_DONE + (i - 1) % L::NSB, (i - 1) / L::NSB & 1, 0x712)) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+                        const uint64_t at = vd + (static_cast<uint32_t>(s * L::STAGE) >> 4);
 #pragma unroll
-                                for (int kk = 0; kk < DP / 16; ++kk)
-                                    mma_f16_ts(tS, tmem + (half ? L::QLO : L::QHI) + kk * 8,
-                                               kd + slot +
-                                                   static_cast<uint32_t>((kk / 4 * L::BOX_BYTES + kk % 4 * 32) >> 4),
-                                               IDESC_QK, half > 0 || kk > 0);
-                            tc_commit(bar(L::S_FULL + sb));
-                        } else {
-                            ok = mbar_wait(bar(s), i / L::NST & 1, ab, 0x714) &&
-                                 mbar_wait(bar(L::P_FULL + sb), i / L::NSB & 1, ab, 0x715);
-                            if (!ok) break;
-                            fence_proxy_async_smem();
-                            tc_fence_after();
-#pragma unroll
-                            for (int kk = 0; kk < KT / 16; ++kk)
-                                mma_f16_ts(tmem + L::O0, tS + kk * 8, vd + slot + static_cast<uint32_t>((kk * 16 * 128) >> 4),
-                                           IDESC_PV, kk > 0 || i > i0);
-                            // (S of this tile came first: its keys have been read too)
-                            tc_commit(bar(L::NST + s));
-                            tc_commit(bar(L::PV_DONE + sb));
-                            if (i == i0 + g.count - 1) tc_commit(bar(L::O_FULL));
-                        }
+                        for (int kk = 0; kk < KT / 16; ++kk)
+                            mma_f16_ts(tm + L::O0, tm + L::S0 + sb * KT + kk * 8, at + ((kk * 16 * 128) >> 4), IDESC_PV,
+                                       kk > 0 || i > start);
+                        tc_commit(bar(L::NST + s));
+                        tc_commit(bar(L::PV_DONE + sb));
+                        if (i == behind - 1) tc_commit(bar(L::O_FULL));
                     }
+                    __syncwarp();
+                    if (i + L::NSB < behind) issue_qk(i + L::NSB);
                 }
-                ok = __shfl_sync(0xffffffffu, ok, 0);
-                i0 += g.count;
+                i0 = behind;
             }
-            if (lane == 0) {
-                // nothing of this thread's is in flight when the TMEM goes
-                tc_commit(bar(L::DRAIN + w));
-                mbar_wait_drain(bar(L::DRAIN + w), 0);
-            }
+            // nothing of this warp's is in flight when the TMEM goes
+            if (elect_one()) tc_commit(bar(L::DRAIN + w));
+            mbar_wait_drain(bar(L::DRAIN + w), 0);
             __syncwarp();
         }
     } else {
         // ---------------------------------------------------------------- softmax
+        regs_increase<L::SOFTMAX_REGS>();
         const int w = warp / 4, quad = warp % 4, lr = quad * 32 + lane;  // row of the tile
         const uint32_t lanes = static_cast<uint32_t>(quad * 32) << 16;
         const uint32_t tO = tmem + lanes + L::O0;
@@ -242,6 +286,7 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
         int* ctx_lo = reinterpret_cast<int*>(smem + L::OFF_MASK + L::RT * L::NW * 4);
         volatile float* ref = reinterpret_cast<volatile float*>(smem + L::OFF_M);
         float* sums = reinterpret_cast<float*>(smem + L::OFF_L);
+        uint8_t* stage = smem + L::OFF_STAGE + warp * L::STAGE_BYTES;
         const int nw = (p.t.T + 31) / 32;
         const float sl2 = p.scale_log2;
         bool aborted = false;
@@ -250,53 +295,66 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
             if (!aborted && !__all_sync(0xffffffffu, mbar_wait(bar(i), parity, ab, site))) aborted = true;
             return !aborted;
         };
-        for (int pos = begin; pos < end;) {
-            // (each warp keeps its segment in shared memory: registers are for the scores)
-            Segment& g = reinterpret_cast<Segment*>(smem + L::OFF_SEG)[warp];
+        // each warp keeps its segment in shared memory
+        Segment& g = reinterpret_cast<Segment*>(smem + L::OFF_SEG)[warp];
+        if (lane == 0) {
+            g.next = kept[0];
+            g.e = 0;
+        }
+        __syncwarp();
+        while (g.next < kept[1]) {
             {
-                const Segment found = segment_at(p, pre, pos, end, e);
+                int from = g.e;
+                const Segment found = segment_at(p, pre, g.next, kept[1], from);
+                __syncwarp();
                 if (lane == 0) g = found;
                 __syncwarp();
-                pos = found.next;
             }
             if (g.count == 0) {
                 __syncwarp();
                 continue;
             }
             const int row0 = g.rt * p.RT, ta = p.by_G.div(row0), r = row0 + lr;
+            const int qpos = row_position(p, g, r);
             {
-                // this row's Q, half of the columns each group, turned and split, into TMEM
-#pragma unroll 1
-                for (int c0 = w * (DP / 16); c0 < (w + 1) * (DP / 16); c0 += 4) {
-                    uint32_t hi[16], lo[16];
+                // the rows' Q, half of the columns each group, turned and split, into TMEM
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint4 h, l;
-                        load_q_chunk<E>(p, g, r, c0 + c, h, l);
-                        hi[4 * c] = h.x;
-                        hi[4 * c + 1] = h.y;
-                        hi[4 * c + 2] = h.z;
-                        hi[4 * c + 3] = h.w;
-                        lo[4 * c] = l.x;
-                        lo[4 * c + 1] = l.y;
-                        lo[4 * c + 2] = l.z;
-                        lo[4 * c + 3] = l.w;
+                for (int c0 = 0; c0 < DP / 16; c0 += 4) {
+                    uint4 hi[4], lo[4];
+                    int pos[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) pos[k] = __shfl_sync(0xffffffffu, qpos, 8 * k + lane / 4);
+                    load_q<E, 4, 8>(p, g, row0 + quad * 32 + lane / 4, pos, w * (DP / 16) + c0 + lane % 4, hi, lo);
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) *row_chunk(stage, 8 * k + lane / 4, lane % 4) = half ? lo[k] : hi[k];
+                        __syncwarp();
+                        uint4 mine[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mine[k] = *row_chunk(stage, lane, k);
+                        tmem_st_x16(tmem + lanes + (half ? L::QLO : L::QHI) + w * (DP / 4) + 4 * c0,
+                                    reinterpret_cast<const uint32_t*>(mine));
                     }
-                    __syncwarp();
-                    tmem_st_x16(tmem + lanes + L::QHI + 4 * c0, hi);
-                    tmem_st_x16(tmem + lanes + L::QLO + 4 * c0, lo);
                 }
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar(L::Q_FULL));
+                if (lane == 0)
+                    for (int k = 0; k < 2; ++k)
+                        if (((k - i0) & 1) < g.count) mbar_arrive(bar(L::Q_FULL + k));
             }
             if (p.mask != nullptr) {
-                build_mask(p, g, words, ctx_lo, threadIdx.x, 32 * L::NSW);
+                build_mask(p, g, words, threadIdx.x, 32 * L::NSW);
                 named_bar_sync(1, 32 * L::NSW);
+                if (p.window > 0) {
+                    trim_mask(p, g, words, ctx_lo, threadIdx.x, 32 * L::NSW);
+                    named_bar_sync(1, 32 * L::NSW);
+                }
             }
             int rlo, rhi;
-            row_limits(p, g, r, ta, ctx_lo, rlo, rhi);
+            row_limits(p, g, r, qpos, ctx_lo, rlo, rhi);
             const bool dead = rlo >= rhi;
             const int rw = dead ? 0 : (p.by_G.div(r) - ta) * nw;
             const bool idle = __all_sync(0xffffffffu, dead);  // no row of this warp sees a key
@@ -312,37 +370,41 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
                 const uint32_t tS = tmem + lanes + L::S0 + sb * KT;
                 if (!wait(L::S_FULL + sb, i / L::NSB & 1, 0x701)) continue;
                 tc_fence_after();
-                // 32 scores at a time, so that the row fits the 128 registers of 512 threads: the
-                // upper half for the maximum, then the lower half, which stays for its exponentials;
-                // the upper half is read once more
+                // the first 32 scores stay in registers from the maximum to the exponentials, the last
+                // 32 are read twice (64 leave the compiler too few of its 168 registers)
                 float mx = -INFINITY;
-                uint32_t raw[32];
-                float* x = reinterpret_cast<float*>(raw);
-                uint32_t see[2] = {~0u, ~0u};
+                uint32_t raw[32], last[32];
+                float *x = reinterpret_cast<float*>(raw), *y = reinterpret_cast<float*>(last);
+                uint64_t see = ~0ull;
                 bool edge = false;
-                auto load_half = [&](int h) {
-                    tmem_ld_x32(tS + 32 * h, raw);
+                auto load_last = [&] {
+                    tmem_ld_x32(tS + 32, last);
                     if (edge) {
+                        const uint32_t bits = static_cast<uint32_t>(see >> 32);
 #pragma unroll
                         for (int c = 0; c < 32; ++c)
-                            if (!(see[h] >> c & 1u)) x[c] = -INFINITY;
+                            if (!(bits >> c & 1u)) y[c] = -INFINITY;
                     }
                 };
+                int k0, valid;
+                tile_keys(p, tile0 + i, k0, valid);
                 if (!idle) {
-                    int k0, valid;
-                    tile_keys(p, tile0 + i, k0, valid);
                     edge = valid < KT || k0 < all_lo || k0 + KT > all_hi;
                     if (edge) {
-                        uint64_t bits = bits_between(rlo - k0, min(rhi - k0, valid));
+                        see = bits_between(rlo - k0, min(rhi - k0, valid));
                         if (p.mask != nullptr && k0 + KT > L0)
-                            bits &= bits_between(0, L0 - k0) | draft_bits(words + rw, nw, k0 - L0);
-                        see[0] = static_cast<uint32_t>(bits);
-                        see[1] = static_cast<uint32_t>(bits >> 32);
+                            see &= bits_between(0, L0 - k0) | draft_bits(words + rw, nw, k0 - L0);
                     }
-                    load_half(1);
-                    mx = max32(x);
-                    load_half(0);
-                    mx = fmaxf(mx, max32(x)) * sl2;
+                    load_last();
+                    mx = row_max<32>(y);
+                    tmem_ld_x32(tS, raw);
+                    if (edge) {
+                        const uint32_t bits = static_cast<uint32_t>(see);
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            if (!(bits >> c & 1u)) x[c] = -INFINITY;
+                    }
+                    mx = fmaxf(mx, row_max<32>(x)) * sl2;
                 }
                 // the reference that the tile before left (the first tile of a segment has none)
                 if (i > i0 && !wait(L::TOKEN + (w ^ 1) * 4 + quad, (i - 1) / 2 & 1, 0x703)) continue;
@@ -381,30 +443,31 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
                     const float nm = m == -INFINITY ? 0.f : -m;
                     const uint64_t mul2 = f2(sl2, sl2), nm2 = f2(nm, nm);
                     uint64_t ls[4] = {0ull, 0ull, 0ull, 0ull};
+                    auto exponentials = [&](const float* v, int c0) {
+                        uint32_t pk[8];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (h == 1) load_half(1);
-#pragma unroll
-                        for (int c0 = 0; c0 < 32; c0 += 16) {
-                            uint32_t pk[8];
-#pragma unroll
-                            for (int c = 0; c < 16; c += 2) {
-                                float a0, a1;
-                                f2_split(ffma2(f2(x[c0 + c], x[c0 + c + 1]), mul2, nm2), a0, a1);
-                                const float p0 = ex2(a0), p1 = ex2(a1);
-                                ls[(c >> 1) & 3] = fadd2(ls[(c >> 1) & 3], f2(p0, p1));
-                                pk[c / 2] = E::pack(p0, p1);
-                            }
-                            // (columns whose scores have been read already)
-                            tmem_st_x8(tS + 16 * h + c0 / 2, pk);
+                        for (int c = 0; c < 16; c += 2) {
+                            float a0, a1;
+                            f2_split(ffma2(f2(v[c], v[c + 1]), mul2, nm2), a0, a1);
+                            const float p0 = ex2(a0), p1 = ex2(a1);
+                            ls[(c >> 1) & 3] = fadd2(ls[(c >> 1) & 3], f2(p0, p1));
+                            pk[c / 2] = E::pack(p0, p1);
                         }
-                    }
+                        tmem_st_x8(tS + c0 / 2, pk);  // (over scores that have been read)
+                    };
+#pragma unroll
+                    for (int c0 = 0; c0 < 32; c0 += 16) exponentials(x + c0, c0);
+                    load_last();
+#pragma unroll
+                    for (int c0 = 0; c0 < 32; c0 += 16) exponentials(y + c0, 32 + c0);
                     float s0, s1;
                     f2_split(fadd2(fadd2(ls[0], ls[1]), fadd2(ls[2], ls[3])), s0, s1);
                     l += s0 + s1;
                     tmem_wait_st();
                     tc_fence_before();
                 }
+                if (k0 < g.s.lo || k0 + KT > g.s.hi)
+                    zero_unseen_v<DP>(ring + i % L::NST * L::STAGE + L::TILE, g.s, k0, quad * (KT / 4), KT / 4, lane, 32);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(L::P_FULL + sb));
             }
@@ -420,36 +483,42 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
                 m = end_m;
             }
             named_bar_sync(1, 32 * L::NSW);
-            if (g.first == 0 && threadIdx.x == 0) describe_unit(p, sched, g, begin);
+            if (g.first == 0 && threadIdx.x == 0) describe_unit(p, Sched{0, 0, kept[2], kept[3]}, g, kept[0]);
             if (!aborted && !*abort_flag && !__all_sync(0xffffffffu, r >= p.rows)) {
                 const float M = dead ? -INFINITY : m;
                 const float lsum = dead ? 0.f : sums[lr] + sums[L::RT + lr];
                 const bool whole = g.count == g.s.n;
                 const float inv = whole ? (lsum == 0.f ? 0.f : 1.f / lsum) : 1.f;
-                float* slot = partial_slot(p, segment_slot(g, begin));
-                const int t = p.by_G.div(r);
-                uint16_t* out = p.o + g.b * p.osb + (g.kvh * p.G + r - t * p.G) * p.osh + t * p.oss;
-                for (int c0 = w * (DP / 2); c0 < (w + 1) * (DP / 2); c0 += 32) {
-                    uint32_t raw[32];
+                float* slot = partial_slot(p, segment_slot(g, kept[0]));
+#pragma unroll 1
+                for (int c0 = w * (DP / 2); c0 < (w + 1) * (DP / 2); c0 += 16) {
+                    uint32_t raw[16];
                     __syncwarp();
-                    tmem_ld_x32(tO + c0, raw);
-                    float o[32];
+                    tmem_ld_x16(tO + c0, raw);
+                    float* o = reinterpret_cast<float*>(raw);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) o[k] = M == -INFINITY ? 0.f : __uint_as_float(raw[k]) * inv;
-                    if (r < p.rows) {
+                    for (int k = 0; k < 16; ++k) o[k] = M == -INFINITY ? 0.f : o[k] * inv;
+                    if (whole) {
 #pragma unroll
-                        for (int k = 0; k < 32; k += 8) {
-                            if (c0 + k >= p.D) break;
-                            if (whole) {
-                                *reinterpret_cast<uint4*>(out + c0 + k) =
-                                    uint4{E::pack(o[k], o[k + 1]), E::pack(o[k + 2], o[k + 3]),
-                                          E::pack(o[k + 4], o[k + 5]), E::pack(o[k + 6], o[k + 7])};
-                            } else {
-                                float4* d = reinterpret_cast<float4*>(slot) + (c0 + k) / 4 * p.RT + lr;
-                                d[0] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-                                d[p.RT] = make_float4(o[k + 4], o[k + 5], o[k + 6], o[k + 7]);
-                            }
+                        for (int k = 0; k < 2; ++k)
+                            *row_chunk(stage, lane, k) =
+                                uint4{E::pack(o[8 * k], o[8 * k + 1]), E::pack(o[8 * k + 2], o[8 * k + 3]),
+                                      E::pack(o[8 * k + 4], o[8 * k + 5]), E::pack(o[8 * k + 6], o[8 * k + 7])};
+                        __syncwarp();
+                        const int c = c0 + lane % 2 * 8;
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int row = row0 + quad * 32 + 16 * k + lane / 2, t = p.by_G.div(row);
+                            if (row < p.rows && c < p.D)
+                                *reinterpret_cast<uint4*>(p.o + g.b * p.osb + (g.kvh * p.G + row - t * p.G) * p.osh +
+                                                          t * p.oss + c) = *row_chunk(stage, 16 * k + lane / 2, lane % 2);
                         }
+                    } else if (r < p.rows) {
+#pragma unroll
+                        for (int k = 0; k < 16; k += 4)
+                            if (c0 + k < p.D)
+                                reinterpret_cast<float4*>(slot)[(c0 + k) / 4 * p.RT + lr] =
+                                    make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
                     }
                 }
                 if (!whole && w == 0) {

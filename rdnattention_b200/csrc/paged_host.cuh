@@ -23,7 +23,7 @@ const char* check_strides(int64_t s0, int64_t s1, int64_t s2, uint64_t n0, uint6
         if (n[i] <= 1) continue;
         if (s[i] <= 0) return "strides must be positive";
         if (s[i] % 8 != 0) return "strides must be multiples of 16 bytes";
-        if (s[i] >= (int64_t(1) << 46)) return "stride too large";
+        if (s[i] >= (int64_t(1) << 39)) return "stride too large";  // 40 bits of bytes, a tensor map's limit
     }
     return nullptr;
 }
@@ -227,8 +227,6 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
     p.osb = a.oStrideB;
     p.osh = a.oStrideH;
     p.oss = a.oStrideS;
-    p.kc = cache_view(c.kCache, c.kcStrideP, c.kcStrideH, c.kcStrideS);
-    p.vc = cache_view(c.vCache, c.vcStrideP, c.vcStrideH, c.vcStrideS);
     p.t = make_table(c, a.newLens, a.seqLen);
     p.mask = static_cast<const uint8_t*>(a.treeMask);
     p.msb = a.maskStrideB;
@@ -267,6 +265,17 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
     const int64_t step = std::min<int64_t>(fit, paged::kMaxList / p.n_rt);
     if (step == 0) return pfail("problem too large for one launch");
 
+    CUtensorMap tmK, tmV;
+    const uint32_t box_rows = std::min<uint32_t>(c.pageSize, paged::KT);
+    const CUtensorMapDataType dt =
+        c.dtype == paged::DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const View4 vk{c.kCache, {c.headDim, c.pageSize, c.numKvHeads, c.numPages}, {c.kcStrideS, c.kcStrideH, c.kcStrideP}};
+    const View4 vv{c.vCache, {c.headDim, c.pageSize, c.numKvHeads, c.numPages}, {c.vcStrideS, c.vcStrideH, c.vcStrideP}};
+    const char* e = nullptr;
+    if ((e = make_map(&tmK, vk, dt, 2, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B)) ||
+        (e = make_map(&tmV, vv, dt, 2, 64, box_rows, CU_TENSOR_MAP_SWIZZLE_128B)))
+        return pfail(e);
+
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     for (int64_t b0 = 0; b0 < c.batchSize; b0 += step) {
         paged::AttnParams s = p;
@@ -290,12 +299,20 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
         cfg.numAttrs = 1;
         cfg.stream = st;
         cfg.gridDim = dim3(static_cast<unsigned>(f.grid));
-        auto launch = [&](auto kern, int threads, int smem) {
+        // regs != 0: the kernel moves registers between its warps and must have been given
+        // exactly that many per thread (an increase waits for registers the CTA has)
+        auto launch = [&](auto kern, int threads, int smem, int regs) {
             cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
             if (ce != cudaSuccess) return ce;
+            if (regs != 0) {
+                cudaFuncAttributes fa{};
+                ce = cudaFuncGetAttributes(&fa, kern);
+                if (ce != cudaSuccess) return ce;
+                if (fa.numRegs != regs) return cudaErrorInvalidKernelImage;
+            }
             cfg.blockDim = dim3(threads);
             cfg.dynamicSmemBytes = smem;
-            return launch_timed(st, [&] { return cudaLaunchKernelEx(&cfg, kern, s); });
+            return launch_timed(st, [&] { return cudaLaunchKernelEx(&cfg, kern, tmK, tmV, s); });
         };
         auto by_width = [&](auto E) {
             using T = decltype(E);
@@ -305,23 +322,28 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
             using M64 = paged::MmaLayout<64>;
             using M128 = paged::MmaLayout<128>;
             if (f.mma)
-                return f.dp == 64 ? launch(paged::fa_paged_mma_kernel<T, 64>, M64::THREADS, M64::SMEM_BYTES)
-                                  : launch(paged::fa_paged_mma_kernel<T, 128>, M128::THREADS, M128::SMEM_BYTES);
+                return f.dp == 64 ? launch(paged::fa_paged_mma_kernel<T, 64>, M64::THREADS, M64::SMEM_BYTES, M64::LAUNCH_REGS)
+                                  : launch(paged::fa_paged_mma_kernel<T, 128>, M128::THREADS, M128::SMEM_BYTES, M128::LAUNCH_REGS);
             switch (f.dp) {
-                case 64: return launch(paged::fa_paged_kernel<T, 64>, L64::THREADS, L64::SMEM_BYTES);
-                case 128: return launch(paged::fa_paged_kernel<T, 128>, L128::THREADS, L128::SMEM_BYTES);
-                default: return launch(paged::fa_paged_kernel<T, 256>, L256::THREADS, L256::SMEM_BYTES);
+                case 64: return launch(paged::fa_paged_kernel<T, 64>, L64::THREADS, L64::SMEM_BYTES, 0);
+                case 128: return launch(paged::fa_paged_kernel<T, 128>, L128::THREADS, L128::SMEM_BYTES, 0);
+                default: return launch(paged::fa_paged_kernel<T, 256>, L256::THREADS, L256::SMEM_BYTES, 0);
             }
         };
         cudaError_t ce = c.dtype == paged::DT_F16 ? by_width(paged::F16{}) : by_width(paged::BF16{});
         if (ce == cudaSuccess) ce = cudaGetLastError();
         if (ce != cudaSuccess) return fail(g_err_paged, "%s", cudaGetErrorString(ce));
         cfg.gridDim = dim3(static_cast<unsigned>(s.B * join_blocks));
-        const unsigned width = 2 * c.headDim, shares = paged::kJoinThreads / width;
+        const bool wide = s.B * join_blocks <= f.grid;
+        const unsigned width = 2 * c.headDim, shares = wide ? 512 / width : 1;
         cfg.blockDim = dim3(shares * width);
         cfg.dynamicSmemBytes = (shares - 1) * 10 * width * sizeof(float);
-        ce = c.dtype == paged::DT_F16 ? cudaLaunchKernelEx(&cfg, paged::join_kernel<paged::F16>, s)
-                                      : cudaLaunchKernelEx(&cfg, paged::join_kernel<paged::BF16>, s);
+        auto join = [&](auto E) {
+            using T = decltype(E);
+            return wide ? cudaLaunchKernelEx(&cfg, paged::join_kernel<T, true>, s)
+                        : cudaLaunchKernelEx(&cfg, paged::join_kernel<T, false>, s);
+        };
+        ce = c.dtype == paged::DT_F16 ? join(paged::F16{}) : join(paged::BF16{});
         if (ce == cudaSuccess) ce = cudaGetLastError();
         if (ce != cudaSuccess) return fail(g_err_paged, "%s", cudaGetErrorString(ce));
     }
