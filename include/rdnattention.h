@@ -291,7 +291,8 @@ RDNA_API int32_t rdna_peer_barrier(int32_t world, int32_t rank, void* const* pee
 
 /* ---------------------------------------------------------------------------
  * Paged KV cache (extension; no counterpart in the reference): append, attention,
- * accept.  Element type `dtype`: 0 = fp16, 1 = bf16, for every tensor of a call.
+ * accept.  Arguments come in structs (a binding fills one in a single step; calls of a
+ * few microseconds would otherwise wait for forty conversions).  Element type `dtype`: 0 = fp16, 1 = bf16, for every tensor of a call.
  *
  * k_cache / v_cache: [num_pages, num_kv_heads, page_size, head_dim], head_dim
  * contiguous, strides in elements (16-byte multiples) for the page / head / slot
@@ -311,44 +312,69 @@ RDNA_API int32_t rdna_peer_barrier(int32_t world, int32_t rank, void* const* pee
  * cache_lens[b] + t.  new_lens: int32 [batch], how many of the seq_len tokens of
  * each sequence count, or null for all. */
 
+/* A cache and the batch that uses it; part of every call's arguments. */
+typedef struct rdna_paged_cache {
+    void* k_cache;
+    void* v_cache;
+    const void* page_table;
+    const void* cache_lens;
+    int64_t k_stride[3]; /* page, head, slot */
+    int64_t v_stride[3];
+    int64_t table_stride;
+    uint32_t batch_size, num_kv_heads, head_dim, num_pages, page_size, max_pages;
+    int32_t dtype;
+    uint32_t reserved; /* 0 */
+} rdna_paged_cache;
+
 /* Writes token t < new_lens[b] of key / value ([batch, num_kv_heads, seq_len,
- * head_dim], head_dim contiguous, strides in elements) to slot cache_lens[b] + t,
- * the key turned to its position; keys are kept rotated. */
-RDNA_API int32_t rdna_paged_kv_append(
-    const void* key, const void* value, void* k_cache, void* v_cache,
-    const void* page_table, const void* cache_lens, const void* new_lens, const void* positions,
-    const void* rot_cos, const void* rot_sin,
-    int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
-    int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_s,
-    int64_t kc_stride_p, int64_t kc_stride_h, int64_t kc_stride_s,
-    int64_t vc_stride_p, int64_t vc_stride_h, int64_t vc_stride_s, int64_t table_stride,
-    uint32_t batch_size, uint32_t num_kv_heads, uint32_t seq_len, uint32_t head_dim,
-    uint32_t num_pages, uint32_t page_size, uint32_t max_pages, uint32_t rope_rows,
-    int32_t dtype, void* stream);
+ * head_dim], head_dim contiguous, strides in elements for the batch / head / token
+ * axes) to slot cache_lens[b] + t, the key turned to its position; keys are kept
+ * rotated. */
+typedef struct rdna_paged_append_args {
+    rdna_paged_cache cache;
+    const void* key;
+    const void* value;
+    const void* new_lens;
+    const void* positions;
+    const void* rot_cos;
+    const void* rot_sin;
+    int64_t key_stride[3];
+    int64_t value_stride[3];
+    uint32_t seq_len, rope_rows;
+} rdna_paged_append_args;
+RDNA_API int32_t rdna_paged_kv_append(const rdna_paged_append_args* args, void* stream);
 
 /* Attention of seq_len new tokens per sequence, which are in the cache already
  * (slots cache_lens[b] + t).  tree_mask null: token t sees slots 0 ..
  * cache_lens[b] + t.  tree_mask (bytes, nonzero = sees, [batch, seq_len, seq_len]
- * with strides mask_stride_b, mask_stride_t and 1; seq_len <= 256): token t sees
+ * with strides mask_stride[0], mask_stride[1] and 1; seq_len <= 256): token t sees
  * the slots below cache_lens[b] and the new tokens u < new_lens[b] with
  * mask[b][t][u].  window_size > 0: only the newest window_size of these, the new
- * tokens (in index order: parents before children) counting first.  Query rows are
- * turned to their positions.  Output rows t >= new_lens[b] and rows that see
- * nothing are zero.  `workspace` (256-byte aligned, any content, for this call
- * alone until it has run) holds rdna_attention_paged_workspace_size() bytes. */
-RDNA_API int32_t rdna_attention_forward_paged(
-    const void* q, const void* k_cache, const void* v_cache, void* output,
-    const void* page_table, const void* cache_lens, const void* new_lens,
-    const void* tree_mask, const void* positions, const void* rot_cos, const void* rot_sin,
-    int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
-    int64_t kc_stride_p, int64_t kc_stride_h, int64_t kc_stride_s,
-    int64_t vc_stride_p, int64_t vc_stride_h, int64_t vc_stride_s,
-    int64_t o_stride_b, int64_t o_stride_h, int64_t o_stride_s,
-    int64_t mask_stride_b, int64_t mask_stride_t, int64_t table_stride,
-    uint32_t batch_size, uint32_t num_heads, uint32_t num_kv_heads, uint32_t seq_len, uint32_t head_dim,
-    uint32_t num_pages, uint32_t page_size, uint32_t max_pages, uint32_t rope_rows,
-    float scale, int32_t window_size, int32_t dtype,
-    void* workspace, uint64_t workspace_bytes, void* stream);
+ * tokens (in index order: parents before children) counting first.  Query rows
+ * ([batch, num_heads, seq_len, head_dim]) are turned to their positions.  Output
+ * rows t >= new_lens[b] and rows that see nothing are zero.  `workspace` (256-byte
+ * aligned, any content, for this call alone until it has run) holds
+ * rdna_attention_paged_workspace_size() bytes. */
+typedef struct rdna_paged_attention_args {
+    rdna_paged_cache cache;
+    const void* query;
+    void* output;
+    const void* new_lens;
+    const void* tree_mask;
+    const void* positions;
+    const void* rot_cos;
+    const void* rot_sin;
+    void* workspace;
+    uint64_t workspace_bytes;
+    int64_t query_stride[3];
+    int64_t output_stride[3];
+    int64_t mask_stride[2];
+    uint32_t num_heads, seq_len, rope_rows;
+    int32_t window_size;
+    float scale;
+    uint32_t reserved; /* 0 */
+} rdna_paged_attention_args;
+RDNA_API int32_t rdna_attention_forward_paged(const rdna_paged_attention_args* args, void* stream);
 RDNA_API uint64_t rdna_attention_paged_workspace_size(
     uint32_t batch_size, uint32_t num_heads, uint32_t num_kv_heads, uint32_t seq_len, uint32_t head_dim,
     uint32_t page_size, uint32_t max_pages);
@@ -358,13 +384,13 @@ RDNA_API uint64_t rdna_attention_paged_workspace_size(
  * and V, all rows as they were before the call.  accepted: int32 [batch,
  * max_accepted] contiguous, max_accepted <= 256; an entry that is negative or
  * behind the page table moves nothing. */
-RDNA_API int32_t rdna_paged_kv_accept(
-    void* k_cache, void* v_cache, const void* page_table, const void* cache_lens,
-    const void* accepted, const void* accepted_lens,
-    int64_t kc_stride_p, int64_t kc_stride_h, int64_t kc_stride_s,
-    int64_t vc_stride_p, int64_t vc_stride_h, int64_t vc_stride_s, int64_t table_stride,
-    uint32_t batch_size, uint32_t num_kv_heads, uint32_t head_dim,
-    uint32_t num_pages, uint32_t page_size, uint32_t max_pages, uint32_t max_accepted,
-    int32_t dtype, void* stream);
+typedef struct rdna_paged_accept_args {
+    rdna_paged_cache cache;
+    const void* accepted;
+    const void* accepted_lens;
+    uint32_t max_accepted;
+    uint32_t reserved; /* 0 */
+} rdna_paged_accept_args;
+RDNA_API int32_t rdna_paged_kv_accept(const rdna_paged_accept_args* args, void* stream);
 
 #endif /* RDNATTENTION_H_ */

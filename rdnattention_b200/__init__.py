@@ -109,14 +109,14 @@ def _lib_handle():
         lib.rdna_peer_barrier.restype = i32
         lib.rdna_debug_set_kernel_events.argtypes = [vp, vp]
         lib.rdna_debug_set_kernel_events.restype = i32
-        lib.rdna_paged_kv_append.argtypes = [vp] * 10 + [i64] * 13 + [u32] * 8 + [i32, vp]
+        # the paged calls take a packed struct (paged.py)
+        lib.rdna_paged_kv_append.argtypes = [ctypes.c_char_p, vp]
         lib.rdna_paged_kv_append.restype = i32
-        lib.rdna_attention_forward_paged.argtypes = ([vp] * 11 + [i64] * 15 + [u32] * 9 + [f32, i32, i32]
-                                                     + [vp, ctypes.c_uint64, vp])
+        lib.rdna_attention_forward_paged.argtypes = [ctypes.c_char_p, vp]
         lib.rdna_attention_forward_paged.restype = i32
         lib.rdna_attention_paged_workspace_size.argtypes = [u32] * 7
         lib.rdna_attention_paged_workspace_size.restype = ctypes.c_uint64
-        lib.rdna_paged_kv_accept.argtypes = [vp] * 6 + [i64] * 7 + [u32] * 7 + [i32, vp]
+        lib.rdna_paged_kv_accept.argtypes = [ctypes.c_char_p, vp]
         lib.rdna_paged_kv_accept.restype = i32
         _lib = lib
     return _lib

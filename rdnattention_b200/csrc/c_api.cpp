@@ -455,65 +455,52 @@ RDNA_API int32_t rdna_attention_forward_noalloc(
 
 namespace {
 
-rdna::PagedCacheParams paged_cache(
-    const void* k_cache, const void* v_cache, const void* page_table, const void* cache_lens,
-    int64_t kc_stride_p, int64_t kc_stride_h, int64_t kc_stride_s,
-    int64_t vc_stride_p, int64_t vc_stride_h, int64_t vc_stride_s, int64_t table_stride,
-    uint32_t batch_size, uint32_t num_kv_heads, uint32_t head_dim,
-    uint32_t num_pages, uint32_t page_size, uint32_t max_pages, int32_t dtype) {
+rdna::PagedCacheParams paged_cache(const rdna_paged_cache& a) {
     rdna::PagedCacheParams c{};
-    c.kCache = const_cast<void*>(k_cache);
-    c.vCache = const_cast<void*>(v_cache);
-    c.kcStrideP = kc_stride_p;
-    c.kcStrideH = kc_stride_h;
-    c.kcStrideS = kc_stride_s;
-    c.vcStrideP = vc_stride_p;
-    c.vcStrideH = vc_stride_h;
-    c.vcStrideS = vc_stride_s;
-    c.pageTable = page_table;
-    c.tableStride = table_stride;
-    c.cacheLens = cache_lens;
-    c.numPages = num_pages;
-    c.pageSize = page_size;
-    c.maxPages = max_pages;
-    c.batchSize = batch_size;
-    c.numKvHeads = num_kv_heads;
-    c.headDim = head_dim;
-    c.dtype = dtype;
+    c.kCache = a.k_cache;
+    c.vCache = a.v_cache;
+    c.kcStrideP = a.k_stride[0];
+    c.kcStrideH = a.k_stride[1];
+    c.kcStrideS = a.k_stride[2];
+    c.vcStrideP = a.v_stride[0];
+    c.vcStrideH = a.v_stride[1];
+    c.vcStrideS = a.v_stride[2];
+    c.pageTable = a.page_table;
+    c.tableStride = a.table_stride;
+    c.cacheLens = a.cache_lens;
+    c.numPages = a.num_pages;
+    c.pageSize = a.page_size;
+    c.maxPages = a.max_pages;
+    c.batchSize = a.batch_size;
+    c.numKvHeads = a.num_kv_heads;
+    c.headDim = a.head_dim;
+    c.dtype = a.dtype;
     return c;
 }
 
 }  // namespace
 
-RDNA_API int32_t rdna_paged_kv_append(
-    const void* key, const void* value, void* k_cache, void* v_cache,
-    const void* page_table, const void* cache_lens, const void* new_lens, const void* positions,
-    const void* rot_cos, const void* rot_sin,
-    int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_s,
-    int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_s,
-    int64_t kc_stride_p, int64_t kc_stride_h, int64_t kc_stride_s,
-    int64_t vc_stride_p, int64_t vc_stride_h, int64_t vc_stride_s, int64_t table_stride,
-    uint32_t batch_size, uint32_t num_kv_heads, uint32_t seq_len, uint32_t head_dim,
-    uint32_t num_pages, uint32_t page_size, uint32_t max_pages, uint32_t rope_rows,
-    int32_t dtype, void* stream) {
+RDNA_API int32_t rdna_paged_kv_append(const rdna_paged_append_args* args, void* stream) {
+    if (args == nullptr) {
+        set_error("Paged cache append failed: %s", "null arguments");
+        return -3;
+    }
     rdna::PagedAppendParams p{};
-    p.c = paged_cache(k_cache, v_cache, page_table, cache_lens, kc_stride_p, kc_stride_h, kc_stride_s, vc_stride_p,
-                      vc_stride_h, vc_stride_s, table_stride, batch_size, num_kv_heads, head_dim, num_pages,
-                      page_size, max_pages, dtype);
-    p.key = key;
-    p.value = value;
-    p.kStrideB = k_stride_b;
-    p.kStrideH = k_stride_h;
-    p.kStrideS = k_stride_s;
-    p.vStrideB = v_stride_b;
-    p.vStrideH = v_stride_h;
-    p.vStrideS = v_stride_s;
-    p.newLens = new_lens;
-    p.positions = positions;
-    p.rotCos = rot_cos;
-    p.rotSin = rot_sin;
-    p.seqLen = seq_len;
-    p.ropeRows = rope_rows;
+    p.c = paged_cache(args->cache);
+    p.key = args->key;
+    p.value = args->value;
+    p.kStrideB = args->key_stride[0];
+    p.kStrideH = args->key_stride[1];
+    p.kStrideS = args->key_stride[2];
+    p.vStrideB = args->value_stride[0];
+    p.vStrideH = args->value_stride[1];
+    p.vStrideS = args->value_stride[2];
+    p.newLens = args->new_lens;
+    p.positions = args->positions;
+    p.rotCos = args->rot_cos;
+    p.rotSin = args->rot_sin;
+    p.seqLen = args->seq_len;
+    p.ropeRows = args->rope_rows;
     if (rdna::pagedAppend(p, stream) != 0) {
         set_error("Paged cache append failed: %s", rdna::lastErrorPaged());
         return -3;
@@ -521,44 +508,34 @@ RDNA_API int32_t rdna_paged_kv_append(
     return 0;
 }
 
-RDNA_API int32_t rdna_attention_forward_paged(
-    const void* q, const void* k_cache, const void* v_cache, void* output,
-    const void* page_table, const void* cache_lens, const void* new_lens,
-    const void* tree_mask, const void* positions, const void* rot_cos, const void* rot_sin,
-    int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_s,
-    int64_t kc_stride_p, int64_t kc_stride_h, int64_t kc_stride_s,
-    int64_t vc_stride_p, int64_t vc_stride_h, int64_t vc_stride_s,
-    int64_t o_stride_b, int64_t o_stride_h, int64_t o_stride_s,
-    int64_t mask_stride_b, int64_t mask_stride_t, int64_t table_stride,
-    uint32_t batch_size, uint32_t num_heads, uint32_t num_kv_heads, uint32_t seq_len, uint32_t head_dim,
-    uint32_t num_pages, uint32_t page_size, uint32_t max_pages, uint32_t rope_rows,
-    float scale, int32_t window_size, int32_t dtype,
-    void* workspace, uint64_t workspace_bytes, void* stream) {
+RDNA_API int32_t rdna_attention_forward_paged(const rdna_paged_attention_args* args, void* stream) {
+    if (args == nullptr) {
+        set_error("Attention (paged) failed: %s", "null arguments");
+        return -3;
+    }
     rdna::PagedAttentionParams p{};
-    p.c = paged_cache(k_cache, v_cache, page_table, cache_lens, kc_stride_p, kc_stride_h, kc_stride_s, vc_stride_p,
-                      vc_stride_h, vc_stride_s, table_stride, batch_size, num_kv_heads, head_dim, num_pages,
-                      page_size, max_pages, dtype);
-    p.q = q;
-    p.o = output;
-    p.qStrideB = q_stride_b;
-    p.qStrideH = q_stride_h;
-    p.qStrideS = q_stride_s;
-    p.oStrideB = o_stride_b;
-    p.oStrideH = o_stride_h;
-    p.oStrideS = o_stride_s;
-    p.newLens = new_lens;
-    p.treeMask = tree_mask;
-    p.maskStrideB = mask_stride_b;
-    p.maskStrideT = mask_stride_t;
-    p.positions = positions;
-    p.rotCos = rot_cos;
-    p.rotSin = rot_sin;
-    p.numHeads = num_heads;
-    p.seqLen = seq_len;
-    p.ropeRows = rope_rows;
-    p.scale = scale;
-    p.windowSize = window_size;
-    if (rdna::pagedAttention(p, workspace, workspace_bytes, stream) != 0) {
+    p.c = paged_cache(args->cache);
+    p.q = args->query;
+    p.o = args->output;
+    p.qStrideB = args->query_stride[0];
+    p.qStrideH = args->query_stride[1];
+    p.qStrideS = args->query_stride[2];
+    p.oStrideB = args->output_stride[0];
+    p.oStrideH = args->output_stride[1];
+    p.oStrideS = args->output_stride[2];
+    p.newLens = args->new_lens;
+    p.treeMask = args->tree_mask;
+    p.maskStrideB = args->mask_stride[0];
+    p.maskStrideT = args->mask_stride[1];
+    p.positions = args->positions;
+    p.rotCos = args->rot_cos;
+    p.rotSin = args->rot_sin;
+    p.numHeads = args->num_heads;
+    p.seqLen = args->seq_len;
+    p.ropeRows = args->rope_rows;
+    p.scale = args->scale;
+    p.windowSize = args->window_size;
+    if (rdna::pagedAttention(p, args->workspace, args->workspace_bytes, stream) != 0) {
         set_error("Attention (paged) failed: %s", rdna::lastErrorPaged());
         return -3;
     }
@@ -579,21 +556,16 @@ RDNA_API uint64_t rdna_attention_paged_workspace_size(
     return rdna::pagedAttentionWorkspaceBytes(p);
 }
 
-RDNA_API int32_t rdna_paged_kv_accept(
-    void* k_cache, void* v_cache, const void* page_table, const void* cache_lens,
-    const void* accepted, const void* accepted_lens,
-    int64_t kc_stride_p, int64_t kc_stride_h, int64_t kc_stride_s,
-    int64_t vc_stride_p, int64_t vc_stride_h, int64_t vc_stride_s, int64_t table_stride,
-    uint32_t batch_size, uint32_t num_kv_heads, uint32_t head_dim,
-    uint32_t num_pages, uint32_t page_size, uint32_t max_pages, uint32_t max_accepted,
-    int32_t dtype, void* stream) {
+RDNA_API int32_t rdna_paged_kv_accept(const rdna_paged_accept_args* args, void* stream) {
+    if (args == nullptr) {
+        set_error("Paged cache accept failed: %s", "null arguments");
+        return -3;
+    }
     rdna::PagedAcceptParams p{};
-    p.c = paged_cache(k_cache, v_cache, page_table, cache_lens, kc_stride_p, kc_stride_h, kc_stride_s, vc_stride_p,
-                      vc_stride_h, vc_stride_s, table_stride, batch_size, num_kv_heads, head_dim, num_pages,
-                      page_size, max_pages, dtype);
-    p.accepted = accepted;
-    p.acceptedLens = accepted_lens;
-    p.maxAccepted = max_accepted;
+    p.c = paged_cache(args->cache);
+    p.accepted = args->accepted;
+    p.acceptedLens = args->accepted_lens;
+    p.maxAccepted = args->max_accepted;
     if (rdna::pagedAccept(p, stream) != 0) {
         set_error("Paged cache accept failed: %s", rdna::lastErrorPaged());
         return -3;

@@ -3,7 +3,9 @@
 #pragma once
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <type_traits>
 
 namespace rdna {
 namespace {
@@ -83,11 +85,44 @@ paged::Cache cache_view(void* p, int64_t sp, int64_t sh, int64_t ss) {
     return paged::Cache{static_cast<char*>(p), 2 * sh, static_cast<uint32_t>(2 * sp), static_cast<uint32_t>(2 * ss)};
 }
 
-int sm_count() {
-    int dev = 0, sms = 148;
+// What a launch needs to know of a device, asked for once: its SMs, and whether a kernel's
+// attributes have been set there.
+constexpr int kMaxPagedDevices = 64;
+
+int current_device() {
+    int dev = 0;
     cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return dev >= 0 && dev < kMaxPagedDevices ? dev : -1;
+}
+
+int sm_count() {
+    static std::atomic<int> known[kMaxPagedDevices];
+    const int dev = current_device();
+    int sms = dev >= 0 ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (sms == 0) {
+        sms = 148;
+        cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev >= 0 ? dev : 0);
+        if (dev >= 0) known[dev].store(sms, std::memory_order_relaxed);
+    }
     return sms;
+}
+
+// Lets `kern` use `smem` bytes on the current device.  regs != 0: the kernel moves registers
+// between its warps and must have been given exactly that many per thread (an increase
+// waits for registers the CTA has).
+template <auto kern>
+cudaError_t prepare_kernel(int smem, int regs) {
+    static std::atomic<bool> done[kMaxPagedDevices];
+    const int dev = current_device();
+    if (dev >= 0 && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+    cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (ce == cudaSuccess && regs != 0) {
+        cudaFuncAttributes fa{};
+        ce = cudaFuncGetAttributes(&fa, kern);
+        if (ce == cudaSuccess && fa.numRegs != regs) ce = cudaErrorInvalidKernelImage;
+    }
+    if (ce == cudaSuccess && dev >= 0) done[dev].store(true, std::memory_order_release);
+    return ce;
 }
 
 int launched() {
@@ -179,7 +214,7 @@ int pagedAccept(const PagedAcceptParams& a, void* stream) {
     // threads x rows x 16 bytes of staging: 128 threads up to 96 rows, else 32
     const int threads = p.A <= 96 ? 128 : 32;
     const int smem = threads * p.A * 16;
-    cudaError_t ce = cudaFuncSetAttribute(paged::accept_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 196608);
+    const cudaError_t ce = prepare_kernel<paged::accept_kernel>(196608, 0);
     if (ce != cudaSuccess) return fail(g_err_paged, "%s", cudaGetErrorString(ce));
     const dim3 grid((p.n + threads - 1) / threads, p.B);
     paged::accept_kernel<<<grid, threads, smem, static_cast<cudaStream_t>(stream)>>>(p);
@@ -299,36 +334,28 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
         cfg.numAttrs = 1;
         cfg.stream = st;
         cfg.gridDim = dim3(static_cast<unsigned>(f.grid));
-        // regs != 0: the kernel moves registers between its warps and must have been given
-        // exactly that many per thread (an increase waits for registers the CTA has)
-        auto launch = [&](auto kern, int threads, int smem, int regs) {
-            cudaError_t ce = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-            if (ce != cudaSuccess) return ce;
-            if (regs != 0) {
-                cudaFuncAttributes fa{};
-                ce = cudaFuncGetAttributes(&fa, kern);
-                if (ce != cudaSuccess) return ce;
-                if (fa.numRegs != regs) return cudaErrorInvalidKernelImage;
-            }
+        auto launch = [&](auto kern, cudaError_t ready, int threads, int smem) {
+            if (ready != cudaSuccess) return ready;
             cfg.blockDim = dim3(threads);
             cfg.dynamicSmemBytes = smem;
             return launch_timed(st, [&] { return cudaLaunchKernelEx(&cfg, kern, tmK, tmV, s); });
         };
         auto by_width = [&](auto E) {
             using T = decltype(E);
-            using L64 = paged::Layout<64>;
-            using L128 = paged::Layout<128>;
-            using L256 = paged::Layout<256>;
-            using M64 = paged::MmaLayout<64>;
-            using M128 = paged::MmaLayout<128>;
-            if (f.mma)
-                return f.dp == 64 ? launch(paged::fa_paged_mma_kernel<T, 64>, M64::THREADS, M64::SMEM_BYTES, M64::LAUNCH_REGS)
-                                  : launch(paged::fa_paged_mma_kernel<T, 128>, M128::THREADS, M128::SMEM_BYTES, M128::LAUNCH_REGS);
-            switch (f.dp) {
-                case 64: return launch(paged::fa_paged_kernel<T, 64>, L64::THREADS, L64::SMEM_BYTES, 0);
-                case 128: return launch(paged::fa_paged_kernel<T, 128>, L128::THREADS, L128::SMEM_BYTES, 0);
-                default: return launch(paged::fa_paged_kernel<T, 256>, L256::THREADS, L256::SMEM_BYTES, 0);
-            }
+            auto few = [&](auto W) {
+                using L = paged::Layout<decltype(W)::value>;
+                constexpr auto kern = paged::fa_paged_kernel<T, decltype(W)::value>;
+                return launch(kern, prepare_kernel<kern>(L::SMEM_BYTES, 0), L::THREADS, L::SMEM_BYTES);
+            };
+            auto many = [&](auto W) {
+                using L = paged::MmaLayout<decltype(W)::value>;
+                constexpr auto kern = paged::fa_paged_mma_kernel<T, decltype(W)::value>;
+                return launch(kern, prepare_kernel<kern>(L::SMEM_BYTES, L::LAUNCH_REGS), L::THREADS, L::SMEM_BYTES);
+            };
+            const std::integral_constant<int, 64> w64;
+            const std::integral_constant<int, 128> w128;
+            if (f.mma) return f.dp == 64 ? many(w64) : many(w128);
+            return f.dp == 64 ? few(w64) : f.dp == 128 ? few(w128) : few(std::integral_constant<int, 256>{});
         };
         cudaError_t ce = c.dtype == paged::DT_F16 ? by_width(paged::F16{}) : by_width(paged::BF16{});
         if (ce == cudaSuccess) ce = cudaGetLastError();

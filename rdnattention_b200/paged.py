@@ -27,6 +27,9 @@ clamped to the table's capacity; a page outside the cache is not written and rea
 as zeros; a token whose position lies outside the rotation tables is not appended,
 and its attention row is zero.
 """
+import functools
+import struct
+
 import torch
 
 from . import RDNAttentionError, _last_error, _lib_handle
@@ -36,6 +39,15 @@ MAX_TREE_TOKENS = 256
 MAX_ACCEPTED_TOKENS = 256
 
 _DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1}
+_HEAD_DIMS = frozenset(SUPPORTED_HEAD_DIMS_PAGED)
+
+# rdna_paged_cache and the argument structs that start with one (include/rdnattention.h).
+# One pack per call: converting the arguments one by one would take longer than the
+# smaller kernels.
+_CACHE = "4Q7q6IiI"
+_APPEND = struct.Struct("=" + _CACHE + "6Q6q2I")
+_ATTENTION = struct.Struct("=" + _CACHE + "9Q8q3IifI")
+_ACCEPT = struct.Struct("=" + _CACHE + "2Q2I")
 
 
 def _tensor(name, t, dtype, device, shape=None):
@@ -50,49 +62,77 @@ def _tensor(name, t, dtype, device, shape=None):
 
 
 def _optional_int32(name, t, device, shape):
-    """Address of a contiguous int32 tensor, or None."""
+    """Address of a contiguous int32 tensor, or 0."""
     if t is None:
-        return None
+        return 0
+    if (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.device == device and t.shape == shape
+            and t.is_contiguous()):
+        return t.data_ptr()
     _tensor(name, t, torch.int32, device, shape)
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous - call .contiguous() first")
     return t.data_ptr()
 
 
-def _cache_args(k_cache, v_cache, page_table, cache_lens):
-    """Checks what every call shares; returns (device, dtype code, cache shape, batch, max_pages)."""
+def _check_cache(k_cache, v_cache, page_table, cache_lens):
+    """Raises what is wrong with the cache's tensors."""
     if not isinstance(k_cache, torch.Tensor) or not isinstance(v_cache, torch.Tensor):
         raise TypeError("k_cache and v_cache must be torch.Tensors")
     device, dtype = k_cache.device, k_cache.dtype
     if not k_cache.is_cuda:
         raise ValueError("k_cache must be on a CUDA device")
-    code = _DTYPE_CODES.get(dtype)
-    if code is None:
+    if dtype not in _DTYPE_CODES:
         raise ValueError(f"k_cache must be float16 or bfloat16, got {dtype}")
     if k_cache.dim() != 4:
         raise ValueError(f"k_cache must be 4D [num_pages, kv_heads, page_size, head_dim], got {tuple(k_cache.shape)}")
-    shape = tuple(k_cache.shape)
-    _tensor("v_cache", v_cache, dtype, device, shape)
+    _tensor("v_cache", v_cache, dtype, device, tuple(k_cache.shape))
     if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
         raise ValueError("k_cache and v_cache must have a contiguous head_dim axis")
-    if shape[3] not in SUPPORTED_HEAD_DIMS_PAGED:
-        raise RDNAttentionError(f"head_dim {shape[3]} not supported (allowed: {list(SUPPORTED_HEAD_DIMS_PAGED)})")
+    if k_cache.shape[3] not in _HEAD_DIMS:
+        raise RDNAttentionError(
+            f"head_dim {k_cache.shape[3]} not supported (allowed: {list(SUPPORTED_HEAD_DIMS_PAGED)})")
     _tensor("page_table", page_table, torch.int32, device)
     if page_table.dim() != 2 or page_table.shape[1] > 1 and page_table.stride(1) != 1:
         raise ValueError("page_table must be 2D [batch, max_pages] with contiguous rows")
-    batch, max_pages = page_table.shape
-    _tensor("cache_lens", cache_lens, torch.int32, device, (batch,))
+    _tensor("cache_lens", cache_lens, torch.int32, device, (page_table.shape[0],))
     if not cache_lens.is_contiguous():
         raise ValueError("cache_lens must be contiguous - call .contiguous() first")
-    return device, code, shape, batch, max_pages
+
+
+def _cache_args(k_cache, v_cache, page_table, cache_lens):
+    """Checks what every call shares; returns (device, shape of the cache, batch, packed rdna_paged_cache values)."""
+    try:
+        device, dtype, shape, ks = k_cache.device, k_cache.dtype, k_cache.shape, k_cache.stride()
+        vs, ts, batch = v_cache.stride(), page_table.stride(), page_table.shape[0]
+        max_pages = page_table.shape[1]
+        # (all in one expression: these checks are half of a small call)
+        good = (device.type == "cuda" and dtype in _DTYPE_CODES and len(shape) == 4 and v_cache.dtype is dtype
+                and v_cache.device == device and v_cache.shape == shape and ks[3] == 1 and vs[3] == 1
+                and shape[3] in _HEAD_DIMS and page_table.dtype is torch.int32 and page_table.device == device
+                and len(ts) == 2 and (ts[1] == 1 or max_pages <= 1) and cache_lens.dtype is torch.int32
+                and cache_lens.device == device and cache_lens.shape == (batch,) and cache_lens.is_contiguous())
+    except (AttributeError, IndexError, TypeError):
+        good = False
+    if not good:
+        _check_cache(k_cache, v_cache, page_table, cache_lens)
+        raise ValueError("unsupported cache tensors")
+    return device, shape, batch, (
+        k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), cache_lens.data_ptr(), ks[0], ks[1], ks[2],
+        vs[0], vs[1], vs[2], ts[0], batch, shape[1], shape[3], shape[0], shape[2], max_pages, _DTYPE_CODES[dtype], 0)
 
 
 def _rope_tables(rot_cos, rot_sin, device, head_dim):
-    """(cos address, sin address, rows), or (None, None, 0)."""
+    """(cos address, sin address, rows), or (0, 0, 0)."""
     if rot_cos is None and rot_sin is None:
-        return None, None, 0
+        return 0, 0, 0
     if rot_cos is None or rot_sin is None:
         raise ValueError("pass both rot_cos and rot_sin, or neither")
+    if isinstance(rot_cos, torch.Tensor) and isinstance(rot_sin, torch.Tensor):
+        shape = rot_cos.shape
+        if (rot_cos.dtype is torch.float32 and rot_sin.dtype is torch.float32 and rot_cos.device == device
+                and rot_sin.device == device and len(shape) == 2 and rot_sin.shape == shape
+                and shape[1] == head_dim // 2 and rot_cos.is_contiguous() and rot_sin.is_contiguous()):
+            return rot_cos.data_ptr(), rot_sin.data_ptr(), shape[0]
     for name, t in (("rot_cos", rot_cos), ("rot_sin", rot_sin)):
         _tensor(name, t, torch.float32, device)
         if t.dim() != 2 or t.shape[1] != head_dim // 2:
@@ -104,24 +144,34 @@ def _rope_tables(rot_cos, rot_sin, device, head_dim):
     return rot_cos.data_ptr(), rot_sin.data_ptr(), rot_cos.shape[0]
 
 
-def _new_rows(name, t, k_cache, batch, heads):
-    """Checks a [batch, heads, tokens, head_dim] tensor of the cache's type; returns its number of tokens."""
+def _new_rows(name, t, k_cache, batch, heads, head_dim):
+    """Checks a [batch, heads, tokens, head_dim] tensor of the cache's type; returns (tokens, strides)."""
+    if isinstance(t, torch.Tensor) and t.dtype is k_cache.dtype and t.device == k_cache.device:
+        shape, stride = t.shape, t.stride()
+        if (len(shape) == 4 and shape[0] == batch and shape[3] == head_dim and (heads == 0 or shape[1] == heads)
+                and stride[3] == 1):
+            return shape[2], stride
     _tensor(name, t, k_cache.dtype, k_cache.device)
-    if t.dim() != 4 or t.shape[0] != batch or t.shape[3] != k_cache.shape[3] or heads and t.shape[1] != heads:
-        raise ValueError(f"{name} must be 4D [batch = {batch}, heads, tokens, head_dim = {k_cache.shape[3]}]"
+    if t.dim() != 4 or t.shape[0] != batch or t.shape[3] != head_dim or heads and t.shape[1] != heads:
+        raise ValueError(f"{name} must be 4D [batch = {batch}, heads, tokens, head_dim = {head_dim}]"
                          f"{f' with {heads} heads' if heads else ''}, got {tuple(t.shape)}")
-    if t.stride(3) != 1:
-        raise ValueError(f"{name} must have a contiguous head_dim axis")
-    return t.shape[2]
+    raise ValueError(f"{name} must have a contiguous head_dim axis")
 
 
-def _call(who, device, fn, *args):
+@functools.lru_cache(maxsize=1024)
+def _workspace_elements(device_index, *sizes):
+    """Workspace of an attention call, in 2-byte elements."""
+    with torch.cuda.device(device_index):
+        return (_lib_handle().rdna_attention_paged_workspace_size(*sizes) + 1) // 2
+
+
+def _call(who, device, fn, args):
     """Runs a library call on `device`'s current stream, with `device` current."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    if device.index == torch.cuda.current_device():
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(device.index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(device.index))
     if rc != 0:
         raise RDNAttentionError(f"{who} failed: {_last_error()}")
 
@@ -135,22 +185,19 @@ def paged_kv_append(key, value, k_cache, v_cache, page_table, cache_lens, new_le
     None: cache_lens[b] + t) by the float32 [positions, head_dim // 2] tables
     rot_cos / rot_sin as interleaved pairs (None: stored as it is).  No two tokens
     may go to the same row.  Returns (k_cache, v_cache)."""
-    device, code, (num_pages, heads, page_size, head_dim), batch, max_pages = _cache_args(
-        k_cache, v_cache, page_table, cache_lens)
-    tokens = _new_rows("key", key, k_cache, batch, heads)
-    if _new_rows("value", value, k_cache, batch, heads) != tokens:
+    device, (_, heads, _, head_dim), batch, cache = _cache_args(k_cache, v_cache, page_table, cache_lens)
+    tokens, ks = _new_rows("key", key, k_cache, batch, heads, head_dim)
+    value_tokens, vs = _new_rows("value", value, k_cache, batch, heads, head_dim)
+    if value_tokens != tokens:
         raise ValueError(f"key and value shapes must match: K={tuple(key.shape)}, V={tuple(value.shape)}")
     new_p = _optional_int32("new_lens", new_lens, device, (batch,))
     pos_p = _optional_int32("positions", positions, device, (batch, tokens))
     cos_p, sin_p, rows = _rope_tables(rot_cos, rot_sin, device, head_dim)
     if batch == 0 or tokens == 0:
         return k_cache, v_cache
-    ks, vs, kc, vc = key.stride(), value.stride(), k_cache.stride(), v_cache.stride()
     _call("paged_kv_append", device, _lib_handle().rdna_paged_kv_append,
-          key.data_ptr(), value.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
-          cache_lens.data_ptr(), new_p, pos_p, cos_p, sin_p, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-          kc[0], kc[1], kc[2], vc[0], vc[1], vc[2], page_table.stride(0), batch, heads, tokens, head_dim,
-          num_pages, page_size, max_pages, rows, code)
+          _APPEND.pack(*cache, key.data_ptr(), value.data_ptr(), new_p, pos_p, cos_p, sin_p, ks[0], ks[1], ks[2],
+                       vs[0], vs[1], vs[2], tokens, rows))
     return k_cache, v_cache
 
 
@@ -174,46 +221,41 @@ def flash_attn_paged(query, k_cache, v_cache, page_table, cache_lens, new_lens=N
     Softmax scale: ``scale``, None for 1/sqrt(head_dim).  Returns ``out`` (or a new
     tensor) shaped like query; rows t >= new_lens[b] and rows that see nothing are
     zero."""
-    device, code, (num_pages, kv_heads, page_size, head_dim), batch, max_pages = _cache_args(
-        k_cache, v_cache, page_table, cache_lens)
-    tokens = _new_rows("query", query, k_cache, batch, 0)
+    device, (_, kv_heads, page_size, head_dim), batch, cache = _cache_args(k_cache, v_cache, page_table, cache_lens)
+    tokens, qs = _new_rows("query", query, k_cache, batch, 0, head_dim)
     heads = query.shape[1]
     if kv_heads == 0 or heads == 0 or heads % kv_heads != 0:
         raise ValueError(f"Q heads ({heads}) must be a multiple of the cache's heads ({kv_heads})")
     new_p = _optional_int32("new_lens", new_lens, device, (batch,))
     pos_p = _optional_int32("positions", positions, device, (batch, tokens))
     cos_p, sin_p, rows = _rope_tables(rot_cos, rot_sin, device, head_dim)
-    mask_p, mask_b, mask_t = None, 0, 0
+    mask_p = mask_b = mask_t = 0
     if tree_mask is not None:
         _tensor("tree_mask", tree_mask, torch.bool, device)
-        shape = tuple(tree_mask.shape)
+        shape = tree_mask.shape
         if shape not in ((tokens, tokens), (1, tokens, tokens), (batch, tokens, tokens)):
-            raise ValueError(f"tree_mask must be [batch or 1, tokens, tokens] or [tokens, tokens], got {shape}")
+            raise ValueError(f"tree_mask must be [batch or 1, tokens, tokens] or [tokens, tokens], got {tuple(shape)}")
         if tokens > MAX_TREE_TOKENS:
             raise ValueError(f"tree_mask takes at most {MAX_TREE_TOKENS} tokens, got {tokens}")
-        if tokens > 1 and (tree_mask.stride(-1) != 1 or tree_mask.stride(-2) < 0):
+        ms = tree_mask.stride()
+        if tokens > 1 and (ms[-1] != 1 or ms[-2] < 0):
             raise ValueError("tree_mask must have contiguous rows")
-        mask_p = tree_mask.data_ptr()
-        mask_t = tree_mask.stride(-2)
-        mask_b = tree_mask.stride(0) if len(shape) == 3 and shape[0] > 1 else 0
+        mask_p, mask_t = tree_mask.data_ptr(), ms[-2]
+        mask_b = ms[0] if len(shape) == 3 and shape[0] > 1 else 0
     if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=device)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
     else:
         _tensor("out", out, query.dtype, device, tuple(query.shape))
         if out.stride(3) != 1:
             raise ValueError("out must have a contiguous head_dim axis")
     if batch == 0 or tokens == 0:
         return out
-    lib = _lib_handle()
-    ws_bytes = lib.rdna_attention_paged_workspace_size(batch, heads, kv_heads, tokens, head_dim, page_size, max_pages)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=device)
-    qs, kc, vc, os_ = query.stride(), k_cache.stride(), v_cache.stride(), out.stride()
-    _call("flash_attn_paged", device, lib.rdna_attention_forward_paged,
-          query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), page_table.data_ptr(),
-          cache_lens.data_ptr(), new_p, mask_p, pos_p, cos_p, sin_p, qs[0], qs[1], qs[2], kc[0], kc[1], kc[2],
-          vc[0], vc[1], vc[2], os_[0], os_[1], os_[2], mask_b, mask_t, page_table.stride(0), batch, heads, kv_heads,
-          tokens, head_dim, num_pages, page_size, max_pages, rows,
-          head_dim ** -0.5 if scale is None else float(scale), int(window_size), code, ws.data_ptr(), ws_bytes)
+    ws = query.new_empty(_workspace_elements(device.index, batch, heads, kv_heads, tokens, head_dim, page_size, cache[-3]))
+    os_ = out.stride()
+    _call("flash_attn_paged", device, _lib_handle().rdna_attention_forward_paged,
+          _ATTENTION.pack(*cache, query.data_ptr(), out.data_ptr(), new_p, mask_p, pos_p, cos_p, sin_p, ws.data_ptr(),
+                          2 * ws.numel(), qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], mask_b, mask_t, heads, tokens,
+                          rows, int(window_size), head_dim ** -0.5 if scale is None else float(scale), 0))
     return out
 
 
@@ -225,8 +267,7 @@ def paged_kv_accept(k_cache, v_cache, page_table, cache_lens, accepted, accepted
     MAX_ACCEPTED_TOKENS; a negative entry, or one behind the page table, moves nothing.
     The drafted slots' pages must belong to one sequence only.  Returns (k_cache,
     v_cache)."""
-    device, code, (num_pages, heads, page_size, head_dim), batch, max_pages = _cache_args(
-        k_cache, v_cache, page_table, cache_lens)
+    device, _, batch, cache = _cache_args(k_cache, v_cache, page_table, cache_lens)
     _tensor("accepted", accepted, torch.int32, device)
     if accepted.dim() != 2 or accepted.shape[0] != batch or not accepted.is_contiguous():
         raise ValueError(f"accepted must be contiguous [batch = {batch}, n], got {tuple(accepted.shape)}")
@@ -236,9 +277,6 @@ def paged_kv_accept(k_cache, v_cache, page_table, cache_lens, accepted, accepted
     lens_p = _optional_int32("accepted_lens", accepted_lens, device, (batch,))
     if batch == 0 or n == 0:
         return k_cache, v_cache
-    kc, vc = k_cache.stride(), v_cache.stride()
     _call("paged_kv_accept", device, _lib_handle().rdna_paged_kv_accept,
-          k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), cache_lens.data_ptr(), accepted.data_ptr(),
-          lens_p, kc[0], kc[1], kc[2], vc[0], vc[1], vc[2], page_table.stride(0), batch, heads, head_dim, num_pages,
-          page_size, max_pages, n, code)
+          _ACCEPT.pack(*cache, accepted.data_ptr(), lens_p, n, 0))
     return k_cache, v_cache

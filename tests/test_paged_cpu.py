@@ -1,11 +1,16 @@
 """Paged KV-cache operators without a GPU: what the C ABI and the Python entry
 points refuse before they touch a device, the workspace's size, and the oracle
 against a dense computation."""
+import struct
+import subprocess
+from pathlib import Path
+
 import pytest
 import torch
 
 import paged_oracle as O
 import rdnattention_b200 as R
+from rdnattention_b200 import paged
 
 CS = (8 * 64 * 128, 64 * 128, 128)  # page / head / slot strides of a [pages, 8, 64, 128] cache
 
@@ -14,14 +19,23 @@ def _message(rc):
     return rc, R._lib_handle().rdna_get_error().decode()
 
 
+def _pack(layout, *values):
+    """The struct's bytes; values beyond a field's range are the caller's mistake, None is a null pointer."""
+    return layout.pack(*(0 if v is None else v for v in values))
+
+
+def _cache(a):
+    return (a["kc"], a["vc"], a["table"], a["lens"], *a["kcs"], *a["vcs"], a["ts"], a["B"], a["Hkv"], a["D"],
+            a["pages"], a["P"], a["mp"], a["dt"], 0)
+
+
 def _append(**kw):
     a = dict(key=16, value=16, kc=16, vc=16, table=16, lens=16, news=None, pos=None, cos=None, sin=None, ks=CS, vs=CS,
              kcs=CS, vcs=CS, ts=4, B=2, Hkv=8, T=3, D=128, pages=8, P=64, mp=4, rows=0, dt=0)
     a.update(kw)
     return _message(R._lib_handle().rdna_paged_kv_append(
-        a["key"], a["value"], a["kc"], a["vc"], a["table"], a["lens"], a["news"], a["pos"], a["cos"], a["sin"],
-        *a["ks"], *a["vs"], *a["kcs"], *a["vcs"], a["ts"], a["B"], a["Hkv"], a["T"], a["D"], a["pages"], a["P"],
-        a["mp"], a["rows"], a["dt"], None))
+        _pack(paged._APPEND, *_cache(a), a["key"], a["value"], a["news"], a["pos"], a["cos"], a["sin"], *a["ks"],
+              *a["vs"], a["T"], a["rows"]), None))
 
 
 def _attend(**kw):
@@ -30,9 +44,9 @@ def _attend(**kw):
              scale=0.1, window=-1, dt=0, ws=256, wsb=1 << 40)
     a.update(kw)
     return _message(R._lib_handle().rdna_attention_forward_paged(
-        a["q"], a["kc"], a["vc"], a["o"], a["table"], a["lens"], a["news"], a["mask"], a["pos"], a["cos"], a["sin"],
-        *a["qs"], *a["kcs"], *a["vcs"], *a["os"], a["mb"], a["mt"], a["ts"], a["B"], a["H"], a["Hkv"], a["T"], a["D"],
-        a["pages"], a["P"], a["mp"], a["rows"], a["scale"], a["window"], a["dt"], a["ws"], a["wsb"], None))
+        _pack(paged._ATTENTION, *_cache(a), a["q"], a["o"], a["news"], a["mask"], a["pos"], a["cos"], a["sin"],
+              a["ws"], a["wsb"], *a["qs"], *a["os"], a["mb"], a["mt"], a["H"], a["T"], a["rows"], a["window"],
+              a["scale"], 0), None))
 
 
 def _accept(**kw):
@@ -40,8 +54,7 @@ def _accept(**kw):
              mp=4, A=4, dt=0)
     a.update(kw)
     return _message(R._lib_handle().rdna_paged_kv_accept(
-        a["kc"], a["vc"], a["table"], a["lens"], a["acc"], a["al"], *a["kcs"], *a["vcs"], a["ts"], a["B"], a["Hkv"],
-        a["D"], a["pages"], a["P"], a["mp"], a["A"], a["dt"], None))
+        _pack(paged._ACCEPT, *_cache(a), a["acc"], a["al"], a["A"], 0), None))
 
 
 COMMON = [
@@ -101,6 +114,35 @@ def test_accept_refusals(kw, needle):
 
 def test_nothing_to_do_is_not_an_error():
     assert _append(T=0)[0] == 0 and _attend(T=0)[0] == 0 and _accept(A=0)[0] == 0
+
+
+def test_argument_structs_match_the_header(tmp_path):
+    """Sizes and the offsets of each struct's last named field, as a C compiler lays them out."""
+    src = tmp_path / "layout.c"
+    src.write_text('''#include <stddef.h>
+#include <stdio.h>
+#include "rdnattention.h"
+int main(void) {
+    printf("%zu %zu %zu %zu\\n", sizeof(rdna_paged_cache), sizeof(rdna_paged_append_args),
+           sizeof(rdna_paged_attention_args), sizeof(rdna_paged_accept_args));
+    printf("%zu %zu %zu %zu\\n", offsetof(rdna_paged_cache, dtype), offsetof(rdna_paged_append_args, rope_rows),
+           offsetof(rdna_paged_attention_args, scale), offsetof(rdna_paged_accept_args, max_accepted));
+    return 0;
+}''')
+    exe = tmp_path / "layout"
+    include = Path(__file__).resolve().parents[1] / "include"
+    subprocess.run(["gcc", f"-I{include}", str(src), "-o", str(exe)], check=True)
+    sizes, offsets = ([int(x) for x in line.split()] for line in subprocess.check_output([str(exe)], text=True).splitlines())
+    cache = struct.Struct("=" + paged._CACHE)
+    assert sizes == [cache.size, paged._APPEND.size, paged._ATTENTION.size, paged._ACCEPT.size]
+    assert offsets == [cache.size - 8, paged._APPEND.size - 4, paged._ATTENTION.size - 8, paged._ACCEPT.size - 8]
+
+
+def test_null_arguments():
+    lib = R._lib_handle()
+    for call in (lib.rdna_paged_kv_append, lib.rdna_attention_forward_paged, lib.rdna_paged_kv_accept):
+        assert call(None, None) == -3
+        assert "null arguments" in lib.rdna_get_error().decode()
 
 
 def test_workspace_size():
