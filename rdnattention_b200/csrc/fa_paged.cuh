@@ -24,6 +24,7 @@
 #include <limits.h>
 #include <math.h>
 
+#include "fa_decode.cuh"
 #include "paged.cuh"
 
 namespace rdna {
@@ -75,6 +76,7 @@ struct AttnParams {
     int2* units; // per unit (b, kvh, rt): first partial's slot, number of parts (0 or 1: nothing to join)
     int grid;    // CTAs of the attention kernel
     int W;       // list positions that a unit costs besides its tiles
+    int join_shift;  // log2 of the join's rows per block
 };
 
 // Touches every line of the parameters once (one word per lane and 64 bytes), so that
@@ -306,24 +308,26 @@ __device__ __forceinline__ void trim_mask(const AttnParams& p, const Segment& g,
 
 // ------------------------------------------------------------- the join kernel
 // O = sum_i 2^(m_i - M) O_i / sum_i 2^(m_i - M) l_i over a split unit's parts, always in
-// the same order.  A block takes 16 rows; a thread one row (lanes side by side, so the
-// partials are read in whole lines), 8 columns and every n-th part, n = blockDim / (2 D)
-// (2 D threads cover the rows and columns); the n shares join in shared memory.  Bound
-// by the latency of dependent reads (the unit, its parts) while there are few units of
-// many parts: the WIDE form has 512 threads and eight parts' loads in flight.  With more
-// blocks than SMs (many units, of few parts) the narrow form keeps four blocks on an SM
-// (256 row tiles of 128 over 8192 keys: 24 us wide).
-constexpr int kJoinRows = 16;
+// the same order.  A thread takes one row (lanes side by side, so the partials are read in
+// runs of 64 or 256 bytes), 8 columns and every n-th part; the n shares of a block join in
+// shared memory.  Bound by the latency of dependent reads (the unit, its parts) while
+// there are few units of many parts: the WIDE form has blocks of 512 threads (n = 2 to 8 at
+// head_dim 128), one for each SM at most, and eight parts' loads in flight.  With more units
+// (of few parts then) the narrow form takes 16 rows with n = 1 and three parts in flight, four
+// blocks on an SM (256 row tiles of 128 over 8192 keys: 9 us, wide 24 us).
+constexpr int kJoinRows = 16, kJoinRowsWide = 4;  // rows of a block: 16; wide: 4, 8 or 16
+constexpr int kJoinThreads = 512;
 
 template <class E, bool WIDE>
-__global__ void __launch_bounds__(512, WIDE ? 1 : 2) join_kernel(const __grid_constant__ AttnParams p) {
-    extern __shared__ float joined[];  // [n - 1][10][2 D]
+__global__ void __launch_bounds__(kJoinThreads, WIDE ? 1 : 2) join_kernel(const __grid_constant__ AttnParams p) {
+    extern __shared__ float joined[];  // [n - 1][10][width]
     constexpr int kJoinFlight = WIDE ? 8 : 3;
-    const int groups = (p.RT + kJoinRows - 1) / kJoinRows;
+    const int rows = 1 << p.join_shift, groups = p.RT >> p.join_shift;
     const int unit = blockIdx.x / groups;
-    const int width = 2 * p.D, n = blockDim.x / width, split = threadIdx.x / width, tid = threadIdx.x - split * width;
-    const int lr = blockIdx.x % groups * kJoinRows + tid % kJoinRows;  // row of the tile
-    const int c = tid / kJoinRows * 8;                                 // first column
+    const int width = rows * (p.D / 8), n = blockDim.x / width, split = threadIdx.x / width,
+              tid = threadIdx.x - split * width;
+    const int lr = blockIdx.x % groups * rows + (tid & (rows - 1));  // row of the tile
+    const int c = (tid >> p.join_shift) * 8;                         // first column
     grid_dependency_wait();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int2 u = p.units[unit];
@@ -391,6 +395,94 @@ __global__ void __launch_bounds__(512, WIDE ? 1 : 2) join_kernel(const __grid_co
     *reinterpret_cast<uint4*>(p.o + b * p.osb + h * p.osh + t * p.oss + c) =
         uint4{E::pack(o[0] * inv, o[1] * inv), E::pack(o[2] * inv, o[3] * inv), E::pack(o[4] * inv, o[5] * inv),
               E::pack(o[6] * inv, o[7] * inv)};
+}
+
+// ------------------------------------------------------------- the cluster form
+// A single sequence's heads are equally long, so an even split needs no list: a cluster of
+// CTAs takes a unit, CTA `rank` the rank-th part of its tiles, and the parts are joined
+// over distributed shared memory.  That saves the second launch and two trips through L2;
+// the host's rule has the measurements.
+__device__ __forceinline__ Segment cluster_segment(const AttnParams& p) {
+    const int size = static_cast<int>(decode::cluster_size()), rank = static_cast<int>(decode::cluster_rank());
+    const int unit = blockIdx.x / size;
+    Segment g;
+    g.rt = unit % p.n_rt;
+    g.kvh = unit / p.n_rt % p.Hkv;
+    g.b = unit / p.n_rt / p.Hkv;
+    g.L = p.t.len(g.b);
+    g.n = p.t.news(g.b);
+    g.s = row_tile_span(p, g.L, g.n, g.rt);
+    g.first = g.s.n * rank / size;
+    g.count = g.s.n * (rank + 1) / size - g.first;
+    g.pos0 = 0;
+    g.next = 1;
+    g.e = 0;
+    return g;
+}
+
+__device__ __forceinline__ float4 ld_dsmem4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+// Joins the cluster's parts (at `part` in each CTA's shared memory: O [D / 4][RT] float4,
+// m [RT], l [RT]; a CTA without tiles has m = -inf) and writes the rows out; every thread of
+// every CTA takes part.
+template <class E>
+__device__ __forceinline__ void cluster_join(const AttnParams& p, const float* part, int tid, int nthreads) {
+    decode::cluster_sync_all();
+    const int size = static_cast<int>(decode::cluster_size()), rank = static_cast<int>(decode::cluster_rank());
+    const int unit = blockIdx.x / size, rt = unit % p.n_rt, kvh = unit / p.n_rt % p.Hkv, b = unit / p.n_rt / p.Hkv;
+    const uint32_t base = smem_u32(part);
+    for (int i = rank * nthreads + tid; i < p.RT * (p.D / 4); i += size * nthreads) {
+        const int lr = i & (p.RT - 1), c = i / p.RT, r = rt * p.RT + lr;
+        if (r >= p.rows) continue;
+        float M = -INFINITY, l = 0.f;
+        float4 o{};
+        for (int k0 = 0; k0 < size; k0 += 8) {
+            float m[8], li[8];
+            float4 x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                m[k] = -INFINITY;
+                if (k0 + k < size) {
+                    const uint32_t a = decode::map_to_rank(base, k0 + k);
+                    m[k] = decode::ld_dsmem(a + 4 * (p.RT * p.D + lr));
+                    li[k] = decode::ld_dsmem(a + 4 * (p.RT * p.D + p.RT + lr));
+                    x[k] = ld_dsmem4(a + 16 * (c * p.RT + lr));
+                }
+            }
+            float mx = M;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) mx = fmaxf(mx, m[k]);
+            const float g = M == -INFINITY ? 0.f : ex2(M - mx);
+            M = mx;
+            l *= g;
+            o.x *= g;
+            o.y *= g;
+            o.z *= g;
+            o.w *= g;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (m[k] != -INFINITY) {
+                    const float f = ex2(m[k] - mx);
+                    l += f * li[k];
+                    o.x += f * x[k].x;
+                    o.y += f * x[k].y;
+                    o.z += f * x[k].z;
+                    o.w += f * x[k].w;
+                }
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int t = p.by_G.div(r);
+        *reinterpret_cast<uint2*>(p.o + b * p.osb + (kvh * p.G + r - t * p.G) * p.osh + t * p.oss + 4 * c) =
+            uint2{E::pack(o.x * inv, o.y * inv), E::pack(o.z * inv, o.w * inv)};
+    }
+    decode::cluster_sync_all();  // no CTA leaves while others read its part
 }
 
 // -------------------------------------------------------- the few-rows kernel
@@ -636,7 +728,7 @@ __device__ __forceinline__ void zero_unseen_v(uint8_t* v, const Span& s, int k0,
     fence_proxy_async_smem();  // before the tensor core's reads, or the slot's next copy
 }
 
-template <class E, int DP>
+template <class E, int DP, bool CLUSTER>
 __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
     const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
     const __grid_constant__ AttnParams p) {
@@ -672,12 +764,17 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
     __syncthreads();
     grid_dependency_wait();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const Sched sched = make_sched(p, pre);
-    if (sched.total == 0 || static_cast<int>(blockIdx.x) >= sched.ctas) {
-        zero_empty_units(p, threadIdx.x, L::THREADS);
-        return;
+    Sched sched{};
+    int begin = 0, end = 1;
+    if constexpr (!CLUSTER) {
+        sched = make_sched(p, pre);
+        if (sched.total == 0 || static_cast<int>(blockIdx.x) >= sched.ctas) {
+            zero_empty_units(p, threadIdx.x, L::THREADS);
+            return;
+        }
+        begin = cta_begin(sched, blockIdx.x);
+        end = cta_begin(sched, blockIdx.x + 1);
     }
-    const int begin = cta_begin(sched, blockIdx.x), end = cta_begin(sched, blockIdx.x + 1);
 
     const int wrg = warp % NRG, wtg = warp / NRG;
     const int gq = lane >> 2, tq = lane & 3;
@@ -689,9 +786,13 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
     int issued = -1;
     int i0 = 0, e = 0, nseg = 0;  // running tile number of the segment's first tile; segments so far
     for (int pos = begin; pos < end;) {
-        const Segment g = segment_at(p, pre, pos, end, e);
+        const Segment g = CLUSTER ? cluster_segment(p) : segment_at(p, pre, pos, end, e);
         pos = g.next;
-        if (g.count == 0) continue;
+        if (g.count == 0) {
+            // (in a cluster: a part without weight)
+            if (CLUSTER && threadIdx.x < p.RT) reinterpret_cast<float*>(ring)[p.RT * p.D + threadIdx.x] = -INFINITY;
+            continue;
+        }
         const int row0 = g.rt * p.RT, ta = p.by_G.div(row0);
         const int qb = nseg % L::NQ, qn = nseg / L::NQ;
         ++nseg;
@@ -917,9 +1018,9 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
             }
         }
         named_bar_sync(1, 32 * NCW);
-        const bool whole = g.count == g.s.n;
-        float* slot = partial_slot(p, segment_slot(g, begin));
-        if (g.first == 0 && threadIdx.x == 0) describe_unit(p, sched, g, begin);
+        const bool whole = !CLUSTER && g.count == g.s.n;
+        float* slot = CLUSTER ? reinterpret_cast<float*>(ring) : partial_slot(p, segment_slot(g, begin));
+        if (!CLUSTER && g.first == 0 && threadIdx.x == 0) describe_unit(p, sched, g, begin);
         const int rows = min(p.RT, p.rows - row0);
         if (!*abort_flag) {
             // rows side by side: whole lines of the partial's [D / 4][RT] layout
@@ -960,7 +1061,12 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
         if (threadIdx.x == 0) mbar_arrive(bars + 8u * (L::Q_EMPTY + qb));
         i0 += g.count;
     }
-    if (warp < NCW) zero_empty_units(p, threadIdx.x, 32 * NCW);
+    if constexpr (CLUSTER) {
+        __syncwarp();
+        cluster_join<E>(p, reinterpret_cast<const float*>(ring), threadIdx.x, L::THREADS);
+    } else if (warp < NCW) {
+        zero_empty_units(p, threadIdx.x, 32 * NCW);
+    }
 }
 
 }  // namespace paged

@@ -107,11 +107,18 @@ int sm_count() {
     return sms;
 }
 
+template <auto K>
+struct Kernel {
+    static constexpr auto value = K;
+};
+constexpr int kMaxCluster = 16;
+constexpr int kMaxPagedUnits = 74;  // (two CTAs for each of more do not fit 148 SMs)
+
 // Lets `kern` use `smem` bytes on the current device.  regs != 0: the kernel moves registers
 // between its warps and must have been given exactly that many per thread (an increase
 // waits for registers the CTA has).
 template <auto kern>
-cudaError_t prepare_kernel(int smem, int regs) {
+cudaError_t prepare_kernel(int smem, int regs, bool cluster = false) {
     static std::atomic<bool> done[kMaxPagedDevices];
     const int dev = current_device();
     if (dev >= 0 && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
@@ -121,8 +128,36 @@ cudaError_t prepare_kernel(int smem, int regs) {
         ce = cudaFuncGetAttributes(&fa, kern);
         if (ce == cudaSuccess && fa.numRegs != regs) ce = cudaErrorInvalidKernelImage;
     }
+    if (ce == cudaSuccess && cluster) ce = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (ce == cudaSuccess && dev >= 0) done[dev].store(true, std::memory_order_release);
     return ce;
+}
+
+// Clusters of `size` CTAs that fit the current device at once (asked for once).
+template <auto kern>
+int max_clusters(int size, int threads, int smem) {
+    static std::atomic<int> known[kMaxPagedDevices][kMaxCluster + 1];
+    const int dev = current_device();
+    int n = dev >= 0 ? known[dev][size].load(std::memory_order_relaxed) : 0;
+    if (n == 0) {
+        cudaLaunchConfig_t cfg{};
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = size;
+        attr[0].val.clusterDim.y = 1;
+        attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        cfg.gridDim = dim3(size);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = smem;
+        if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            n = 0;
+        }
+        if (dev >= 0) known[dev][size].store(n > 0 ? n : -1, std::memory_order_relaxed);
+    }
+    return n > 0 ? n : 0;
 }
 
 int launched() {
@@ -327,30 +362,62 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
         // attention kernel waits for it before it reads or writes global memory, the join
         // waits for the attention kernel.
         cudaLaunchConfig_t cfg{};
-        cudaLaunchAttribute attr[1];
+        cudaLaunchAttribute attr[2];
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         cfg.stream = st;
         cfg.gridDim = dim3(static_cast<unsigned>(f.grid));
-        auto launch = [&](auto kern, cudaError_t ready, int threads, int smem) {
-            if (ready != cudaSuccess) return ready;
+        auto launch = [&](auto list, int threads, int smem, int regs) {
+            constexpr auto kern = decltype(list)::value;
             cfg.blockDim = dim3(threads);
             cfg.dynamicSmemBytes = smem;
+            cudaError_t ce = prepare_kernel<kern>(smem, regs);
+            if (ce != cudaSuccess) return ce;
+            return launch_timed(st, [&] { return cudaLaunchKernelEx(&cfg, kern, tmK, tmV, s); });
+        };
+        // The cluster form, where it fits; false: the list.  It takes a single sequence's units,
+        // each by the widest cluster of which enough fit the device at once (8 units: 10 CTAs
+        // each), and joins the parts itself.  Few rows, head_dim 128, 4096 slots: 12.1 us for 8 KV
+        // heads, 10.8 for one, against 13.9 and 17.4 with the list; its CTAs are fewer, though, and
+        // the list is ahead from about 28 key tiles per CTA on (16384 slots, 8 heads: 21.0 and
+        // 21.7 us; 32768: 34.3 and 31.2).  The page table bounds the tiles.
+        bool joined = false;
+        auto launch_cluster = [&](auto cluster, int threads, int smem) {
+            constexpr auto kern = decltype(cluster)::value;
+            const int units = p.Hkv * p.n_rt;
+            if (c.batchSize != 1 || units > kMaxPagedUnits) return cudaSuccess;
+            cudaError_t ce = prepare_kernel<kern>(smem, 0, true);
+            if (ce != cudaSuccess) return ce;
+            int size = kMaxCluster;
+            while (size > 1 && units > max_clusters<kern>(size, threads, smem)) --size;
+            if (size == 1 || tiles > 28 * size) return cudaSuccess;
+            attr[1].id = cudaLaunchAttributeClusterDimension;
+            attr[1].val.clusterDim.x = size;
+            attr[1].val.clusterDim.y = 1;
+            attr[1].val.clusterDim.z = 1;
+            cfg.numAttrs = 2;
+            cfg.gridDim = dim3(units * size);
+            cfg.blockDim = dim3(threads);
+            cfg.dynamicSmemBytes = smem;
+            joined = true;
             return launch_timed(st, [&] { return cudaLaunchKernelEx(&cfg, kern, tmK, tmV, s); });
         };
         auto by_width = [&](auto E) {
             using T = decltype(E);
             auto few = [&](auto W) {
-                using L = paged::Layout<decltype(W)::value>;
-                constexpr auto kern = paged::fa_paged_kernel<T, decltype(W)::value>;
-                return launch(kern, prepare_kernel<kern>(L::SMEM_BYTES, 0), L::THREADS, L::SMEM_BYTES);
+                constexpr int w = decltype(W)::value;
+                using L = paged::Layout<w>;
+                const cudaError_t ce =
+                    launch_cluster(Kernel<paged::fa_paged_kernel<T, w, true>>{}, L::THREADS, L::SMEM_BYTES);
+                if (ce != cudaSuccess || joined) return ce;
+                return launch(Kernel<paged::fa_paged_kernel<T, w, false>>{}, L::THREADS, L::SMEM_BYTES, 0);
             };
             auto many = [&](auto W) {
-                using L = paged::MmaLayout<decltype(W)::value>;
-                constexpr auto kern = paged::fa_paged_mma_kernel<T, decltype(W)::value>;
-                return launch(kern, prepare_kernel<kern>(L::SMEM_BYTES, L::LAUNCH_REGS), L::THREADS, L::SMEM_BYTES);
+                constexpr int w = decltype(W)::value;
+                using L = paged::MmaLayout<w>;
+                return launch(Kernel<paged::fa_paged_mma_kernel<T, w>>{}, L::THREADS, L::SMEM_BYTES, L::LAUNCH_REGS);
             };
             const std::integral_constant<int, 64> w64;
             const std::integral_constant<int, 128> w128;
@@ -360,9 +427,16 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
         cudaError_t ce = c.dtype == paged::DT_F16 ? by_width(paged::F16{}) : by_width(paged::BF16{});
         if (ce == cudaSuccess) ce = cudaGetLastError();
         if (ce != cudaSuccess) return fail(g_err_paged, "%s", cudaGetErrorString(ce));
-        cfg.gridDim = dim3(static_cast<unsigned>(s.B * join_blocks));
-        const bool wide = s.B * join_blocks <= f.grid;
-        const unsigned width = 2 * c.headDim, shares = wide ? 512 / width : 1;
+        if (joined) continue;
+        cfg.numAttrs = 1;
+        const int64_t join_rows = static_cast<int64_t>(s.B) * p.Hkv * p.n_rt * f.RT;
+        const bool wide = join_rows <= static_cast<int64_t>(f.grid) * paged::kJoinRows;
+        unsigned rows = wide ? paged::kJoinRowsWide : paged::kJoinRows;
+        while (wide && join_rows > static_cast<int64_t>(f.grid) * rows) rows *= 2;
+        for (s.join_shift = 0; (1u << s.join_shift) < rows; ++s.join_shift) {
+        }
+        const unsigned width = rows * (c.headDim / 8), shares = wide ? paged::kJoinThreads / width : 1;
+        cfg.gridDim = dim3(static_cast<unsigned>(join_rows / rows));
         cfg.blockDim = dim3(shares * width);
         cfg.dynamicSmemBytes = (shares - 1) * 10 * width * sizeof(float);
         auto join = [&](auto E) {

@@ -139,6 +139,30 @@ def test_attention(case):
     run_case(**case)
 
 
+@pytest.mark.parametrize("T,kind,window", [(1, "chain", -1), (4, "chain", 70), (5, "tree", -1), (16, "tree", 90),
+                                           (64, "tree", -1), (40, "chain", -1)])
+@pytest.mark.parametrize("length", [0, 1, 64, 700, 6001])
+@pytest.mark.parametrize("dtype,H,Hkv,D,P", [(F16, 32, 8, 128, 64), (BF16, 24, 12, 64, 16), (F16, 8, 8, 256, 72)])
+def test_single_sequence(T, kind, window, length, dtype, H, Hkv, D, P):
+    """One sequence with enough heads for the cluster form, from fewer key tiles than CTAs to many."""
+    run_case(dtype, H, Hkv, T, D, P, [length], kind=kind, window=window)
+
+
+def test_single_sequence_with_nothing_to_see():
+    """No key, no new token, masks that hide everything, NaN in the cache: zeros."""
+    g = torch.Generator().manual_seed(21)
+    for T, D in ((1, 128), (8, 128), (8, 256)):
+        kc, vc, table = make_cache(g, F16, [0], T, 8, 16, D)
+        kc.fill_(float("nan"))
+        vc.fill_(float("nan"))
+        q = torch.randn(1, 32, T, D, generator=g).to(F16)
+        assert (attend(q, kc, vc, table, [0], [0]) == 0).all()
+        assert (attend(q, kc, vc, table, [50], [0]) == 0).all()
+        vc.zero_()
+        kc.zero_()
+        assert (attend(q, kc, vc, table, [0], mask=torch.zeros(T, T, dtype=torch.bool)) == 0).all()
+
+
 def test_masks_that_leave_rows_empty():
     """Rows whose mask is all false see the context alone; over an empty context they are zero."""
     g = torch.Generator().manual_seed(3)
