@@ -176,35 +176,51 @@ struct AcceptParams {
     int n;                    // 2 * Hkv * (D / 8) columns of 16 bytes per sequence
 };
 
-// Row len + i takes row len + accepted[i], all as they were before the call.  A
-// thread owns one 16-byte column of one head of K or V and every row of it, so
-// reading all its rows (into its own shared-memory slots) before it writes the
-// first is enough: no two threads touch the same bytes.
+// Row len + i takes row len + accepted[i], all as they were before the call.  A thread
+// owns one 16-byte column of one head of K or V and every row of it, so reading all its
+// rows before it writes the first is enough: no two threads touch the same bytes.  The
+// rows' places are worked out once per block; up to kAcceptRegs rows are held in registers,
+// with every read in flight at once (the bound is the latency of three dependent reads:
+// index, page table, row), more of them in shared memory.
+constexpr int kAcceptRegs = 16;
+
+template <bool REGS>
 __global__ void accept_kernel(const __grid_constant__ AcceptParams p) {
     extern __shared__ uint4 stage[];
+    __shared__ int2 from[kMaxAccept], to[kMaxAccept];  // page and row; page -1: nothing moves
     const int b = blockIdx.y;
+    const int64_t len = p.t.len(b);
+    const int n = p.accepted_lens == nullptr ? p.A : min(max(p.accepted_lens[b], 0), p.A);
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        const int a = p.accepted[static_cast<int64_t>(b) * p.A + i];
+        int2 f{-1, 0}, t{-1, 0};
+        const bool ok = a >= 0 && a != i && p.t.locate(b, len + a, f.x, f.y);
+        if (!(p.t.locate(b, len + i, t.x, t.y) && ok)) f.x = -1;
+        from[i] = f;
+        to[i] = t;
+    }
+    __syncthreads();
     const int col = blockIdx.x * blockDim.x + threadIdx.x;
     if (col >= p.n) return;
     const int nch = p.D / 8;
     const int ch = col % nch, h = col / nch % p.Hkv;
     const Cache& c = col / nch / p.Hkv == 0 ? p.kc : p.vc;
     char* base = c.head(h, ch);
-    const int64_t len = p.t.len(b);
-    const int n = p.accepted_lens == nullptr ? p.A : min(max(p.accepted_lens[b], 0), p.A);
-    const int* acc = p.accepted + static_cast<int64_t>(b) * p.A;
-    auto source = [&](int i, int& page, int& row) {
-        const int a = acc[i];
-        return a >= 0 && a != i && p.t.locate(b, len + a, page, row);
-    };
-    for (int i = 0; i < n; ++i) {
-        int page, row;
-        if (source(i, page, row))
-            stage[i * blockDim.x + threadIdx.x] = *reinterpret_cast<const uint4*>(c.at(base, page, row));
-    }
-    for (int i = 0; i < n; ++i) {
-        int page, row, dpage, drow;
-        if (source(i, page, row) && p.t.locate(b, len + i, dpage, drow))
-            *reinterpret_cast<uint4*>(c.at(base, dpage, drow)) = stage[i * blockDim.x + threadIdx.x];
+    if constexpr (REGS) {
+        uint4 v[kAcceptRegs];
+#pragma unroll
+        for (int i = 0; i < kAcceptRegs; ++i)
+            if (i < n && from[i].x >= 0) v[i] = *reinterpret_cast<const uint4*>(c.at(base, from[i].x, from[i].y));
+#pragma unroll
+        for (int i = 0; i < kAcceptRegs; ++i)
+            if (i < n && from[i].x >= 0) *reinterpret_cast<uint4*>(c.at(base, to[i].x, to[i].y)) = v[i];
+    } else {
+        uint4* mine = stage + threadIdx.x;
+#pragma unroll 4
+        for (int i = 0; i < n; ++i)
+            if (from[i].x >= 0) mine[i * blockDim.x] = *reinterpret_cast<const uint4*>(c.at(base, from[i].x, from[i].y));
+        for (int i = 0; i < n; ++i)
+            if (from[i].x >= 0) *reinterpret_cast<uint4*>(c.at(base, to[i].x, to[i].y)) = mine[i * blockDim.x];
     }
 }
 

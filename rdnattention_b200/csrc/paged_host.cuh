@@ -246,13 +246,18 @@ int pagedAccept(const PagedAcceptParams& a, void* stream) {
     p.Hkv = static_cast<int>(a.c.numKvHeads);
     p.D = static_cast<int>(a.c.headDim);
     p.n = 2 * p.Hkv * (p.D / 8);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (p.A <= paged::kAcceptRegs) {
+        const dim3 grid((p.n + 127) / 128, p.B);
+        paged::accept_kernel<true><<<grid, 128, 0, st>>>(p);
+        return launched();
+    }
     // threads x rows x 16 bytes of staging: 128 threads up to 96 rows, else 32
     const int threads = p.A <= 96 ? 128 : 32;
-    const int smem = threads * p.A * 16;
-    const cudaError_t ce = prepare_kernel<paged::accept_kernel>(196608, 0);
+    const cudaError_t ce = prepare_kernel<paged::accept_kernel<false>>(196608, 0);
     if (ce != cudaSuccess) return fail(g_err_paged, "%s", cudaGetErrorString(ce));
     const dim3 grid((p.n + threads - 1) / threads, p.B);
-    paged::accept_kernel<<<grid, threads, smem, static_cast<cudaStream_t>(stream)>>>(p);
+    paged::accept_kernel<false><<<grid, threads, threads * p.A * 16, st>>>(p);
     return launched();
 }
 
