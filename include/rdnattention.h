@@ -352,9 +352,12 @@ RDNA_API int32_t rdna_paged_kv_append(const rdna_paged_append_args* args, void* 
  * mask[b][t][u].  window_size > 0: only the newest window_size of these, the new
  * tokens (in index order: parents before children) counting first.  Query rows
  * ([batch, num_heads, seq_len, head_dim]) are turned to their positions.  Output
- * rows t >= new_lens[b] and rows that see nothing are zero.  `workspace` (256-byte
- * aligned, any content, for this call alone until it has run) holds
- * rdna_attention_paged_workspace_size() bytes. */
+ * rows t >= new_lens[b] and rows that see nothing are zero.  At most 262144 rows
+ * (seq_len * num_heads / num_kv_heads) per KV head, 65536 above head_dim 128.
+ * `workspace` (256-byte aligned, any content, for this call alone until it has run)
+ * holds rdna_attention_paged_workspace_size() bytes.  New tokens below new_lens[b]
+ * must hold finite values; slots behind them, and in front of a window, may hold
+ * anything. */
 typedef struct rdna_paged_attention_args {
     rdna_paged_cache cache;
     const void* query;

@@ -33,7 +33,10 @@ namespace paged {
 constexpr int kMaxTree = 256;          // drafted tokens under a mask
 constexpr int kMaxList = 2048;         // sequences x row tiles per launch (the host splits larger batches)
 constexpr int KT = 64;                 // keys per tile
-constexpr int kLead = 4, kLeadMma = 8; // AttnParams::W of the two kernels
+// AttnParams::W of the two kernels: about the tiles' worth of time that a segment's start and
+// end take (ragged batch of 33: 157 us at 0, 112 at 4, 105 at 6, 107 at 8; trees of 64 tokens
+// in 16 contexts: 104 us at 8, 102 at 12, 101 at 16).
+constexpr int kLead = 6, kLeadMma = 12;
 
 // n / d for n < 2^31 by a multiplication: with l = ceil(log2 d) and m =
 // floor(2^(31 + l) / d) + 1, m d exceeds 2^(31 + l) by at most 2^l, so the error

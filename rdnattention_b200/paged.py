@@ -34,6 +34,12 @@ import torch
 
 from . import RDNAttentionError, _last_error, _lib_handle
 
+try:  # the stream's handle without a Stream object (2 us less per call)
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:
+    def _raw_stream(index):
+        return torch.cuda.current_stream(index).cuda_stream
+
 SUPPORTED_HEAD_DIMS_PAGED = tuple(range(32, 257, 32))
 MAX_TREE_TOKENS = 256
 MAX_ACCEPTED_TOKENS = 256
@@ -168,10 +174,10 @@ def _workspace_elements(device_index, *sizes):
 def _call(who, device, fn, args):
     """Runs a library call on `device`'s current stream, with `device` current."""
     if device.index == torch.cuda.current_device():
-        rc = fn(args, torch._C._cuda_getCurrentRawStream(device.index))
+        rc = fn(args, _raw_stream(device.index))
     else:
         with torch.cuda.device(device):
-            rc = fn(args, torch._C._cuda_getCurrentRawStream(device.index))
+            rc = fn(args, _raw_stream(device.index))
     if rc != 0:
         raise RDNAttentionError(f"{who} failed: {_last_error()}")
 

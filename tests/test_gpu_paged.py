@@ -259,8 +259,8 @@ def test_contiguous_cache_is_one_page_per_sequence():
 
 
 def test_more_sequences_than_one_launch():
-    """1100 sequences: two launches that share the workspace."""
-    lens = [(i * 7) % 50 for i in range(1100)]
+    """2100 sequences: two launches that share the workspace."""
+    lens = [(i * 7) % 50 for i in range(2100)]
     run_case(F16, 2, 1, 2, 32, 16, lens, rope=False)
 
 
@@ -450,6 +450,93 @@ def test_captured_step_replays_with_new_lengths():
         graph.replay()
         check(out, ref, 3 * bound)
     assert torch.equal(dl.cpu().long(), L)
+
+
+@pytest.mark.parametrize("T,kind", [(1, "chain"), (20, "tree")])
+def test_captured_single_sequence(T, kind):
+    """The forms a single sequence takes, captured, replayed over growing lengths, two replays in a row."""
+    g = torch.Generator().manual_seed(31)
+    H, Hkv, D, P = 32, 8, 128, 16
+    kc, vc, table = make_cache(g, BF16, [900], T, Hkv, P, D)
+    q = torch.randn(1, H, T, D, generator=g).to(BF16)
+    mask = tree(g, 1, T)[0] if kind == "tree" else None
+    dq, dk, dv, dt, dm = cuda(q), *cuda(kc, vc, table), cuda(mask)
+    lens = torch.zeros(1, dtype=torch.int32, device="cuda")
+    R.flash_attn_paged(dq, dk, dv, dt, lens, tree_mask=dm)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = [R.flash_attn_paged(dq, dk, dv, dt, lens, tree_mask=dm) for _ in range(2)]
+    for n in (0, 5, 64, 333, 900):
+        lens.fill_(n)
+        graph.replay()
+        graph.replay()
+        ref, bound = O.attention(q, kc, vc, table, [n], mask=mask)
+        for out in outs:
+            check(out, ref, bound)
+
+
+def test_python_refusals():
+    """What the entry points refuse before a launch."""
+    dev = "cuda"
+    kc = torch.zeros(4, 2, 16, 64, dtype=F16, device=dev)
+    table, lens = torch.zeros(2, 2, dtype=torch.int32, device=dev), torch.zeros(2, dtype=torch.int32, device=dev)
+    q, kv = (torch.zeros(2, h, 3, 64, dtype=F16, device=dev) for h in (4, 2))
+
+    def attend(q=q, k=kc, v=kc, t=table, n=lens, **kw):
+        return R.flash_attn_paged(q, k, v, t, n, **kw)
+
+    mask = torch.ones(3, 3, dtype=torch.bool, device=dev)
+    cos = torch.zeros(10, 32, device=dev)
+    i32 = torch.zeros(2, 3, dtype=torch.int32, device=dev)
+    for call, match in [
+        (lambda: attend(k=kc.float(), v=kc.float()), "float16 or bfloat16"),
+        (lambda: attend(v=kc.bfloat16()), "v_cache must be torch.float16"),
+        (lambda: attend(v=kc[:3]), "v_cache must have shape"),
+        (lambda: attend(k=kc[0], v=kc[0]), "k_cache must be 4D"),
+        (lambda: attend(k=kc.transpose(2, 3), v=kc.transpose(2, 3)), "contiguous head_dim"),
+        (lambda: attend(t=table.long()), "page_table must be torch.int32"),
+        (lambda: attend(t=table[0]), "page_table must be 2D"),
+        (lambda: attend(t=table.cpu()), "same device"),
+        (lambda: attend(n=lens[:1]), "cache_lens must have shape"),
+        (lambda: attend(n=torch.zeros(4, dtype=torch.int32, device=dev)[::2]), "cache_lens must be contiguous"),
+        (lambda: attend(q=q.bfloat16()), "query must be torch.float16"),
+        (lambda: attend(q=q[:1]), "query must be 4D"),
+        (lambda: attend(q=q[:, :3]), "multiple of the cache's heads"),
+        (lambda: attend(q=q.transpose(2, 3).contiguous().transpose(2, 3)), "query must have a contiguous head_dim"),
+        (lambda: attend(new_lens=lens.float()), "new_lens must be torch.int32"),
+        (lambda: attend(positions=i32.t().contiguous().t()), "positions must be contiguous"),
+        (lambda: attend(positions=i32[:, :2]), "positions must have shape"),
+        (lambda: attend(tree_mask=mask.int()), "tree_mask must be torch.bool"),
+        (lambda: attend(tree_mask=mask[:2]), "tree_mask must be"),
+        (lambda: attend(tree_mask=mask.t()[:, :].t()[:, torch.tensor([2, 1, 0], device=dev)].t()), "contiguous rows"),
+        (lambda: attend(rot_cos=cos), "both rot_cos and rot_sin"),
+        (lambda: attend(rot_cos=cos, rot_sin=cos[:5]), "shapes must match"),
+        (lambda: attend(rot_cos=cos[:, :16].contiguous(), rot_sin=cos[:, :16].contiguous()), "head_dim // 2"),
+        (lambda: attend(out=torch.zeros_like(q).bfloat16()), "out must be torch.float16"),
+        (lambda: attend(out=torch.zeros_like(kv)), "out must have shape"),
+        (lambda: R.paged_kv_append(q, kv, kc, kc, table, lens), "key must be 4D"),
+        (lambda: R.paged_kv_append(kv, kv[:, :, :2], kc, kc, table, lens), "key and value shapes"),
+        (lambda: R.paged_kv_accept(kc, kc, table, lens, i32.float()), "accepted must be torch.int32"),
+        (lambda: R.paged_kv_accept(kc, kc, table, lens, i32[:1]), "accepted must be contiguous"),
+    ]:
+        with pytest.raises(ValueError, match=match):
+            call()
+    with pytest.raises(R.RDNAttentionError, match="head_dim 48"):
+        x = torch.zeros(4, 2, 16, 48, dtype=F16, device=dev)
+        attend(k=x, v=x)
+    with pytest.raises(R.RDNAttentionError, match="page_size"):
+        x = torch.zeros(4, 2, 12, 64, dtype=F16, device=dev)
+        attend(k=x, v=x)
+    big = torch.zeros(2, 4, 257, 64, dtype=F16, device=dev)
+    with pytest.raises(ValueError, match="at most 256"):
+        attend(q=big, tree_mask=torch.ones(257, 257, dtype=torch.bool, device=dev))
+    with pytest.raises(ValueError, match="at most 256"):
+        R.paged_kv_accept(kc, kc, table, lens, torch.zeros(2, 257, dtype=torch.int32, device=dev))
+    # nothing to do is not an error
+    empty = torch.zeros(2, 4, 0, 64, dtype=F16, device=dev)
+    assert attend(q=empty).shape == empty.shape
+    assert R.paged_kv_accept(kc, kc, table, lens, i32[:, :0].contiguous())[0] is kc
 
 
 def test_two_streams_at_once():
