@@ -92,6 +92,29 @@ __device__ __forceinline__ float row_max(const float* x) {
     return fmax3(fmax3(m[0], m[1], m[2]), fmax3(m[3], m[4], m[5]), fmaxf(m[6], m[7]));
 }
 
+// 32 columns without waiting, and the wait that gives them (the registers pass through it, so
+// that nothing reads them before).
+__device__ __forceinline__ void tmem_ld_x32_begin(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_x32_end(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+                   "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
+
 // A warp's exchange between rows held by lanes (TMEM) and rows in global memory: 32 rows of
 // four 16-byte chunks, placed so that both orders of access are free of bank conflicts.
 // Four lanes side by side take one row's 64 bytes of global memory; a lane on its own per
@@ -371,40 +394,36 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
                 if (!wait(L::S_FULL + sb, i / L::NSB & 1, 0x701)) continue;
                 tc_fence_after();
                 // the first 32 scores stay in registers from the maximum to the exponentials, the last
-                // 32 are read twice (64 leave the compiler too few of its 168 registers)
+                // 32 are read again behind the first exponentials (64 leave the compiler too few
+                // registers); all reads are begun early
                 float mx = -INFINITY;
                 uint32_t raw[32], last[32];
                 float *x = reinterpret_cast<float*>(raw), *y = reinterpret_cast<float*>(last);
                 uint64_t see = ~0ull;
                 bool edge = false;
-                auto load_last = [&] {
-                    tmem_ld_x32(tS + 32, last);
+                auto hide = [&](float* v, uint32_t bits) {
                     if (edge) {
-                        const uint32_t bits = static_cast<uint32_t>(see >> 32);
 #pragma unroll
                         for (int c = 0; c < 32; ++c)
-                            if (!(bits >> c & 1u)) y[c] = -INFINITY;
+                            if (!(bits >> c & 1u)) v[c] = -INFINITY;
                     }
                 };
                 int k0, valid;
                 tile_keys(p, tile0 + i, k0, valid);
                 if (!idle) {
+                    tmem_ld_x32_begin(tS, raw);
+                    tmem_ld_x32_begin(tS + 32, last);
                     edge = valid < KT || k0 < all_lo || k0 + KT > all_hi;
                     if (edge) {
                         see = bits_between(rlo - k0, min(rhi - k0, valid));
                         if (p.mask != nullptr && k0 + KT > L0)
                             see &= bits_between(0, L0 - k0) | draft_bits(words + rw, nw, k0 - L0);
                     }
-                    load_last();
-                    mx = row_max<32>(y);
-                    tmem_ld_x32(tS, raw);
-                    if (edge) {
-                        const uint32_t bits = static_cast<uint32_t>(see);
-#pragma unroll
-                        for (int c = 0; c < 32; ++c)
-                            if (!(bits >> c & 1u)) x[c] = -INFINITY;
-                    }
-                    mx = fmaxf(mx, row_max<32>(x)) * sl2;
+                    tmem_ld_x32_end(raw);
+                    tmem_ld_x32_end(last);
+                    hide(x, static_cast<uint32_t>(see));
+                    hide(y, static_cast<uint32_t>(see >> 32));
+                    mx = fmaxf(row_max<32>(x), row_max<32>(y)) * sl2;
                 }
                 // the reference that the tile before left (the first tile of a segment has none)
                 if (i > i0 && !wait(L::TOKEN + (w ^ 1) * 4 + quad, (i - 1) / 2 & 1, 0x703)) continue;
@@ -456,10 +475,13 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
                         tmem_st_x8(tS + c0 / 2, pk);  // (over scores that have been read)
                     };
 #pragma unroll
-                    for (int c0 = 0; c0 < 32; c0 += 16) exponentials(x + c0, c0);
-                    load_last();
-#pragma unroll
-                    for (int c0 = 0; c0 < 32; c0 += 16) exponentials(y + c0, 32 + c0);
+                    exponentials(x, 0);
+                    tmem_ld_x32_begin(tS + 32, last);
+                    exponentials(x + 16, 16);
+                    tmem_ld_x32_end(last);
+                    hide(y, static_cast<uint32_t>(see >> 32));
+                    exponentials(y, 32);
+                    exponentials(y + 16, 48);
                     float s0, s1;
                     f2_split(fadd2(fadd2(ls[0], ls[1]), fadd2(ls[2], ls[3])), s0, s1);
                     l += s0 + s1;
