@@ -292,7 +292,8 @@ RDNA_API int32_t rdna_peer_barrier(int32_t world, int32_t rank, void* const* pee
 /* ---------------------------------------------------------------------------
  * Paged KV cache (extension; no counterpart in the reference): append, attention,
  * accept.  Arguments come in structs (a binding fills one in a single step; calls of a
- * few microseconds would otherwise wait for forty conversions).  Element type `dtype`: 0 = fp16, 1 = bf16, for every tensor of a call.
+ * few microseconds would otherwise wait for forty conversions).  Element type `dtype`:
+ * 0 = fp16, 1 = bf16, for every tensor of a call.
  *
  * k_cache / v_cache: [num_pages, num_kv_heads, page_size, head_dim], head_dim
  * contiguous, strides in elements (16-byte multiples) for the page / head / slot
@@ -308,7 +309,7 @@ RDNA_API int32_t rdna_peer_barrier(int32_t world, int32_t rank, void* const* pee
  * appended, and its attention row is zero.
  *
  * rot_cos / rot_sin: fp32 [rope_rows, head_dim / 2], contiguous, interleaved pairs,
- * or both null.  positions: int32 [batch, seq_len] contiguous, or null for
+ * rope_rows > 0, or both null.  positions: int32 [batch, seq_len] contiguous, or null for
  * cache_lens[b] + t.  new_lens: int32 [batch], how many of the seq_len tokens of
  * each sequence count, or null for all. */
 
@@ -356,8 +357,9 @@ RDNA_API int32_t rdna_paged_kv_append(const rdna_paged_append_args* args, void* 
  * (seq_len * num_heads / num_kv_heads) per KV head, 65536 above head_dim 128.
  * `workspace` (256-byte aligned, any content, for this call alone until it has run)
  * holds rdna_attention_paged_workspace_size() bytes.  New tokens below new_lens[b]
- * must hold finite values; slots behind them, and in front of a window, may hold
- * anything. */
+ * must hold finite values; slots behind them, and context slots that no token's window
+ * reaches, may hold anything.  `output` must not share memory with `query`.  The
+ * workspace size is 0 for arguments that the call refuses. */
 typedef struct rdna_paged_attention_args {
     rdna_paged_cache cache;
     const void* query;

@@ -14,10 +14,11 @@
 // some row of it sees.  The tiles of all units, each unit's led by W positions for
 // what starting a unit costs, form one list, and CTA c takes the c-th equal part of
 // it (row tiles slowest, so that the CTAs that read the same keys for other rows do so
-// at the same time and find them in L2): every CTA has the same time's work whatever the lengths are, and the lengths
-// stay on the device (a captured graph replays with new ones).  A unit that lies inside one CTA is finished there; the parts
-// of the others go to a workspace as (O, m, l) in fp32 and the combine kernel
-// joins them in list order, so results do not depend on timing.
+// at the same time and find them in L2): every CTA has the same time's work whatever
+// the lengths are, and the lengths stay on the device (a captured graph replays with
+// new ones).  A unit that lies inside one CTA is finished there; the parts
+// of the others go to a workspace as (O, m, l) in fp32 and the join kernel adds
+// them up in list order, so results do not depend on timing.
 #pragma once
 
 #include <cuda.h>
@@ -719,13 +720,23 @@ __device__ __forceinline__ void drain(uint32_t bars, uint32_t filled, int issued
         }
 }
 
+// First key that some row of the tile sees.  With a mask the window ends earlier than the
+// span says, by the drafted tokens that even the row with the fewest sees (a whole warp; the
+// mask is trimmed).
+__device__ __forceinline__ int first_seen(const AttnParams& p, const Segment& g, const int* ctx_lo, int lane) {
+    if (p.mask == nullptr || p.window <= 0) return g.s.lo;
+    int lo = INT_MAX;
+    for (int i = lane, nt = tile_tokens(p, g); i < nt; i += 32) lo = min(lo, ctx_lo[i]);
+    return __reduce_min_sync(0xffffffffu, lo);
+}
+
 // Slots no row of the unit sees may hold anything (0 * NaN): zeros over the V rows of a tile
-// whose keys k0 + r lie outside the unit's, rows r0 .. r0 + rows - 1, by n threads.
+// whose keys k0 + r lie outside [lo, hi), rows r0 .. r0 + rows - 1, by n threads.
 template <int DP>
-__device__ __forceinline__ void zero_unseen_v(uint8_t* v, const Span& s, int k0, int r0, int rows, int tid, int n) {
+__device__ __forceinline__ void zero_unseen_v(uint8_t* v, int lo, int hi, int k0, int r0, int rows, int tid, int n) {
     for (int idx = tid; idx < rows * (DP / 8); idx += n) {
         const int r = r0 + idx / (DP / 8);
-        if (k0 + r < s.lo || k0 + r >= s.hi)
+        if (k0 + r < lo || k0 + r >= hi)
             *reinterpret_cast<uint4*>(v + chunk_off(KT, r, idx % (DP / 8))) = uint4{0u, 0u, 0u, 0u};
     }
     fence_proxy_async_smem();  // before the tensor core's reads, or the slot's next copy
@@ -864,6 +875,7 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
         if (p.mask != nullptr) all_hi = min(all_hi, g.L);
         all_lo = __reduce_max_sync(0xffffffffu, all_lo);
         all_hi = __reduce_min_sync(0xffffffffu, all_hi);
+        const int seen_lo = first_seen(p, g, ctx_lo, lane);
         auto load_q = [&](int kk, int half, uint32_t* a) {
             ldsm4(qs + half * L::Q_BYTES + chunk_off(p.RT, wrg * 16 + (lane & 15), 2 * kk + (lane >> 4)), a);
         };
@@ -888,12 +900,12 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
             }
             // the last warp-half of a tile to finish frees its slot
             const bool last = NTG > 1 || (hh & 1);
-            const bool none = valid <= 0 || k0 >= g.s.hi || k0 + 32 <= g.s.lo;
+            const bool none = valid <= 0 || k0 >= g.s.hi || k0 + 32 <= seen_lo;
             const uint32_t kb = smem_u32(ring) + s * L::STAGE, vb = kb + L::TILE;
             const bool edge = valid < 32 || k0 < all_lo || k0 + 32 > all_hi;
-            const bool dirty = !none && (k0 < g.s.lo || k0 + 32 > g.s.hi);
+            const bool dirty = !none && (k0 < seen_lo || k0 + 32 > g.s.hi);
             if (dirty) {
-                zero_unseen_v<DP>(ring + s * L::STAGE + L::TILE, g.s, k0 - kh, kh, 32, lane, 32);
+                zero_unseen_v<DP>(ring + s * L::STAGE + L::TILE, seen_lo, g.s.hi, k0 - kh, kh, 32, lane, 32);
                 __syncwarp();
             }
             if (!none) {

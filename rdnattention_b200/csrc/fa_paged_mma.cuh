@@ -376,6 +376,11 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
                     named_bar_sync(1, 32 * L::NSW);
                 }
             }
+            if (p.mask != nullptr && p.window > 0) {
+                const int lo = first_seen(p, g, ctx_lo, lane);
+                if (lane == 0) g.s.lo = lo;
+                __syncwarp();
+            }
             int rlo, rhi;
             row_limits(p, g, r, qpos, ctx_lo, rlo, rhi);
             const bool dead = rlo >= rhi;
@@ -489,7 +494,7 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
                     tc_fence_before();
                 }
                 if (k0 < g.s.lo || k0 + KT > g.s.hi)
-                    zero_unseen_v<DP>(ring + i % L::NST * L::STAGE + L::TILE, g.s, k0, quad * (KT / 4), KT / 4, lane, 32);
+                    zero_unseen_v<DP>(ring + i % L::NST * L::STAGE + L::TILE, g.s.lo, g.s.hi, k0, quad * (KT / 4), KT / 4, lane, 32);
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(L::P_FULL + sb));
             }

@@ -169,7 +169,7 @@ constexpr int kMaxAccept = 256;
 
 struct AcceptParams {
     Cache kc, vc;
-    Table t;                  // t.T: drafted tokens that `accepted` may name
+    Table t;
     const int* accepted;      // [B][A]: drafted token that becomes the i-th accepted one
     const int* accepted_lens; // [B] or null: A
     int A, B, Hkv, D;

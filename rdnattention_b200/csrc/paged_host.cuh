@@ -59,6 +59,7 @@ const char* check_rope(const void* cos, const void* sin, const void* positions, 
     if (cos == nullptr && sin == nullptr) return nullptr;
     if (cos == nullptr || sin == nullptr) return "pass both rot_cos and rot_sin, or neither";
     if (!p16(cos) || !p16(sin)) return "rot_cos/rot_sin must be 16-byte aligned";
+    if (rows == 0) return "the rotation tables have no rows";
     if (rows > INT32_MAX) return "too many rotation table rows";
     return nullptr;
 }
@@ -173,6 +174,9 @@ struct PagedPlan {
     size_t partials, bytes;  // workspace: bytes of the partials, in all
 };
 
+// Rows of a KV head within the kernels' 32 bits (either factor may be any 32-bit number).
+bool rows_fit(uint32_t H, uint32_t Hkv, uint32_t T) { return H / Hkv <= (uint32_t(1) << 28) / std::max(T, 1u); }
+
 PagedPlan paged_plan(uint32_t B, uint32_t H, uint32_t Hkv, uint32_t T, uint32_t D, uint32_t P) {
     PagedPlan f{};
     f.dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
@@ -216,9 +220,9 @@ int pagedAppend(const PagedAppendParams& a, void* stream) {
     p.B = static_cast<int>(a.c.batchSize);
     p.Hkv = static_cast<int>(a.c.numKvHeads);
     p.D = static_cast<int>(a.c.headDim);
-    p.n = static_cast<int64_t>(p.B) * p.Hkv * a.seqLen * (p.D / 8);
-    if (static_cast<int64_t>(p.B) * p.Hkv > INT32_MAX || (p.n + 255) / 256 > INT32_MAX)
-        return pfail("problem too large for one launch");
+    const int64_t heads = static_cast<int64_t>(p.B) * p.Hkv, chunks = static_cast<int64_t>(a.seqLen) * (p.D / 8);
+    if (heads > INT32_MAX || heads > int64_t{INT32_MAX} * 256 / chunks) return pfail("problem too large for one launch");
+    p.n = heads * chunks;
     const unsigned grid = static_cast<unsigned>((p.n + 255) / 256);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (a.c.dtype == paged::DT_F16)
@@ -263,7 +267,8 @@ int pagedAccept(const PagedAcceptParams& a, void* stream) {
 
 size_t pagedAttentionWorkspaceBytes(const PagedAttentionParams& a) {
     if (a.c.numKvHeads == 0 || a.numHeads == 0 || a.numHeads % a.c.numKvHeads != 0 || a.c.headDim == 0 ||
-        a.c.headDim > 256 || a.seqLen == 0 || a.c.pageSize == 0)
+        a.c.headDim > 256 || a.seqLen == 0 || a.c.pageSize == 0 || a.c.numKvHeads > 65535 ||
+        !rows_fit(a.numHeads, a.c.numKvHeads, a.seqLen))
         return 0;
     return paged_plan(a.c.batchSize, a.numHeads, a.c.numKvHeads, a.seqLen, a.c.headDim, a.c.pageSize).bytes;
 }
@@ -277,8 +282,7 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
     if (a.seqLen == 0) return 0;
     if (a.treeMask != nullptr && a.seqLen > static_cast<uint32_t>(paged::kMaxTree))
         return pfail("tree_mask: more than 256 tokens");
-    const int64_t rows = static_cast<int64_t>(a.numHeads / c.numKvHeads) * a.seqLen;
-    if (rows > (1 << 28)) return pfail("sequence too long");
+    if (!rows_fit(a.numHeads, c.numKvHeads, a.seqLen)) return pfail("sequence too long");
     if (!p16(a.q) || !p16(a.o)) return pfail("tensor base pointers must be 16-byte aligned");
     if (!p4(a.newLens)) return pfail("new_lens must be 4-byte aligned");
     if (const char* e = check_strides(a.qStrideB, a.qStrideH, a.qStrideS, c.batchSize, a.numHeads, a.seqLen))
@@ -314,7 +318,7 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
     p.Hkv = static_cast<int>(c.numKvHeads);
     p.G = p.H / p.Hkv;
     p.D = static_cast<int>(c.headDim);
-    p.rows = static_cast<int>(rows);
+    p.rows = static_cast<int>(static_cast<uint32_t>(p.G) * a.seqLen);
     p.RT = f.RT;
     p.n_rt = f.n_rt;
     p.tpp = f.tpp;
@@ -331,7 +335,9 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
     p.grid = f.grid;
     p.W = f.mma ? paged::kLeadMma : paged::kLead;
 
-    // the list positions of one launch are 32-bit: as many sequences per launch as surely fit
+    // the list positions of one launch are 32-bit (n_rt <= 2^11, so none of these products
+    // passes 64 bits): as many sequences per launch as surely fit
+    if (p.n_rt > paged::kMaxList) return pfail("problem too large for one launch");
     const int64_t tiles = f.tpp == 0 ? (static_cast<int64_t>(c.maxPages) * c.pageSize + paged::KT - 1) / paged::KT
                                      : static_cast<int64_t>(c.maxPages) * f.tpp;
     const int64_t per_seq = (tiles + p.W) * p.n_rt * p.Hkv;

@@ -137,7 +137,7 @@ def _rope_tables(rot_cos, rot_sin, device, head_dim):
         shape = rot_cos.shape
         if (rot_cos.dtype is torch.float32 and rot_sin.dtype is torch.float32 and rot_cos.device == device
                 and rot_sin.device == device and len(shape) == 2 and rot_sin.shape == shape
-                and shape[1] == head_dim // 2 and rot_cos.is_contiguous() and rot_sin.is_contiguous()):
+                and shape[0] > 0 and shape[1] == head_dim // 2 and rot_cos.is_contiguous() and rot_sin.is_contiguous()):
             return rot_cos.data_ptr(), rot_sin.data_ptr(), shape[0]
     for name, t in (("rot_cos", rot_cos), ("rot_sin", rot_sin)):
         _tensor(name, t, torch.float32, device)
@@ -147,6 +147,8 @@ def _rope_tables(rot_cos, rot_sin, device, head_dim):
             raise ValueError(f"{name} must be contiguous - call .contiguous() first")
     if rot_cos.shape != rot_sin.shape:
         raise ValueError("rot_cos and rot_sin shapes must match")
+    if rot_cos.shape[0] == 0:
+        raise ValueError("rot_cos and rot_sin have no rows")
     return rot_cos.data_ptr(), rot_sin.data_ptr(), rot_cos.shape[0]
 
 
@@ -222,10 +224,12 @@ def flash_attn_paged(query, k_cache, v_cache, page_table, cache_lens, new_lens=N
     new_lens[b] with mask[b, t, u] (itself only if the mask says so).  window_size >
     0: a token sees only the newest window_size of these; its drafted tokens count
     first, in index order (parents before children).  Drafted tokens below
-    new_lens[b] must hold finite values; slots behind them may hold anything.
+    new_lens[b] must hold finite values; slots behind them, and context slots that no
+    token's window reaches, may hold anything.  At most 262144 rows (tokens * heads /
+    kv_heads) per sequence, 65536 above head_dim 128.
 
     Softmax scale: ``scale``, None for 1/sqrt(head_dim).  Returns ``out`` (or a new
-    tensor) shaped like query; rows t >= new_lens[b] and rows that see nothing are
+    tensor; it must not share memory with query) shaped like query; rows t >= new_lens[b] and rows that see nothing are
     zero."""
     device, (_, kv_heads, page_size, head_dim), batch, cache = _cache_args(k_cache, v_cache, page_table, cache_lens)
     tokens, qs = _new_rows("query", query, k_cache, batch, 0, head_dim)
@@ -254,6 +258,8 @@ def flash_attn_paged(query, k_cache, v_cache, page_table, cache_lens, new_lens=N
         _tensor("out", out, query.dtype, device, tuple(query.shape))
         if out.stride(3) != 1:
             raise ValueError("out must have a contiguous head_dim axis")
+        if out.data_ptr() == query.data_ptr() and out.numel():
+            raise ValueError("out must not share memory with query")
     if batch == 0 or tokens == 0:
         return out
     ws = query.new_empty(_workspace_elements(device.index, batch, heads, kv_heads, tokens, head_dim, page_size, cache[-3]))
@@ -261,7 +267,7 @@ def flash_attn_paged(query, k_cache, v_cache, page_table, cache_lens, new_lens=N
     _call("flash_attn_paged", device, _lib_handle().rdna_attention_forward_paged,
           _ATTENTION.pack(*cache, query.data_ptr(), out.data_ptr(), new_p, mask_p, pos_p, cos_p, sin_p, ws.data_ptr(),
                           2 * ws.numel(), qs[0], qs[1], qs[2], os_[0], os_[1], os_[2], mask_b, mask_t, heads, tokens,
-                          rows, int(window_size), head_dim ** -0.5 if scale is None else float(scale), 0))
+                          rows, max(-1, min(int(window_size), 2**31 - 1)), head_dim ** -0.5 if scale is None else float(scale), 0))
     return out
 
 

@@ -476,6 +476,24 @@ def test_captured_single_sequence(T, kind):
             check(out, ref, bound)
 
 
+@pytest.mark.parametrize("dtype,H,D,P,T", [(F16, 2, 64, 16, 6), (BF16, 4, 128, 8, 5), (F16, 4, 256, 64, 6),
+                                           (BF16, 4, 128, 16, 40), (F16, 2, 64, 64, 150)])
+def test_slots_no_token_sees_in_front_of_a_tree_window(dtype, H, D, P, T):
+    """Every token of a tree sees itself, so the context's part of a window of w is w - 1 at most:
+    slot len - w may be stale."""
+    g = torch.Generator().manual_seed(D + T)
+    lens, w = [37, 130], 20
+    kc, vc, table = make_cache(g, dtype, lens, T, 2, P, D)
+    q = torch.randn(2, H, T, D, generator=g).to(dtype)
+    mask, _ = tree(g, 2, T)
+    ref, bound = O.attention(q, kc, vc, table, lens, mask=mask, window=w)
+    for b, n in enumerate(lens):
+        for s in range(n - w + 1):
+            kc[table[b, s // P], :, s % P] = float("nan")
+            vc[table[b, s // P], :, s % P] = float("inf")
+    check(attend(q, kc, vc, table, lens, mask=mask, window_size=w), ref, bound)
+
+
 def test_python_refusals():
     """What the entry points refuse before a launch."""
     dev = "cuda"
@@ -515,6 +533,8 @@ def test_python_refusals():
         (lambda: attend(rot_cos=cos[:, :16].contiguous(), rot_sin=cos[:, :16].contiguous()), "head_dim // 2"),
         (lambda: attend(out=torch.zeros_like(q).bfloat16()), "out must be torch.float16"),
         (lambda: attend(out=torch.zeros_like(kv)), "out must have shape"),
+        (lambda: attend(out=q), "must not share memory"),
+        (lambda: attend(rot_cos=cos[:0], rot_sin=cos[:0]), "no rows"),
         (lambda: R.paged_kv_append(q, kv, kc, kc, table, lens), "key must be 4D"),
         (lambda: R.paged_kv_append(kv, kv[:, :, :2], kc, kc, table, lens), "key and value shapes"),
         (lambda: R.paged_kv_accept(kc, kc, table, lens, i32.float()), "accepted must be torch.int32"),

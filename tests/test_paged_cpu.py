@@ -152,6 +152,28 @@ def test_workspace_size():
     assert ws(1, 32, 0, 1, 128, 64, 64) == 0 and ws(1, 32, 5, 1, 128, 64, 64) == 0
 
 
+@pytest.mark.parametrize("call", [_append, _attend])
+def test_tables_without_rows_are_refused(call):
+    """No position lies inside them, and the kernels' reads start at row 0."""
+    rc, msg = call(cos=16, sin=32, rows=0)
+    assert rc == -3 and "no rows" in msg, msg
+
+
+@pytest.mark.parametrize("kw", [dict(B=1 << 15, Hkv=1 << 15, T=1 << 30), dict(B=1 << 15, Hkv=1 << 15, T=1 << 29, D=256)])
+def test_append_products_do_not_wrap(kw):
+    """2^15 x 2^15 x 2^30 x 128 / 8 chunks are 0 modulo 2^64."""
+    rc, msg = _append(**kw)
+    assert rc == -3 and "too large for one launch" in msg, msg
+
+
+@pytest.mark.parametrize("H,T", [(1 << 20, 1 << 19), (1 << 31, 1 << 31), ((1 << 32) - 1, (1 << 32) - 1), (1 << 28, 2)])
+def test_attention_products_do_not_wrap(H, T):
+    """2^20 heads x 2^19 tokens are 2^32 row tiles, 0 in 32 bits (and once a division by it)."""
+    assert R._lib_handle().rdna_attention_paged_workspace_size(1, H, 1, T, 128, 64, 64) == 0
+    rc, msg = _attend(B=1, H=H, Hkv=1, T=T)
+    assert rc == -3 and "sequence too long" in msg, msg
+
+
 def test_python_entries_check_their_tensors():
     c = torch.zeros(4, 2, 16, 64, dtype=torch.float16)
     t, n = torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
