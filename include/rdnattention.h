@@ -311,7 +311,8 @@ RDNA_API int32_t rdna_peer_barrier(int32_t world, int32_t rank, void* const* pee
  * rot_cos / rot_sin: fp32 [rope_rows, head_dim / 2], contiguous, interleaved pairs,
  * rope_rows > 0, or both null.  positions: int32 [batch, seq_len] contiguous, or null for
  * cache_lens[b] + t.  new_lens: int32 [batch], how many of the seq_len tokens of
- * each sequence count, or null for all. */
+ * each sequence count, or null for all.  (Kernel attributes are set once per device:
+ * calls after cudaDeviceReset are not supported.) */
 
 /* A cache and the batch that uses it; part of every call's arguments. */
 typedef struct rdna_paged_cache {

@@ -500,6 +500,11 @@ __device__ __forceinline__ void cluster_join(const AttnParams& p, const float* p
 // in 32 bits splits into them but for 2^-22 / 2^-16 of it in fp16 / bf16), and both
 // are multiplied with K: the bound is HBM, so the extra MMAs are free, and the
 // scores are as exact as an fp32 product.
+//
+// Measured (head_dim 128): 64 sequences of 32768 slots, 8 KV heads of 8 query heads:
+// 1.253 ms, 6.86 TB/s, 1.05 of the measured copy rate.  33 ragged sequences of up to 8192
+// slots, 32 / 8 heads, pages of 16: 105 to 114 us, 0.74 to 0.8 of the copy rate (what is
+// missing are the segments' starts, four or five per CTA, and the join).
 template <int DP>
 struct Layout {
     static constexpr int NCW = DP <= 128 ? 8 : 4;

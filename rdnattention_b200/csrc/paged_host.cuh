@@ -388,12 +388,14 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
             if (ce != cudaSuccess) return ce;
             return launch_timed(st, [&] { return cudaLaunchKernelEx(&cfg, kern, tmK, tmV, s); });
         };
-        // The cluster form, where it fits; false: the list.  It takes a single sequence's units,
+        // The cluster form, where it fits; else the list.  It takes a single sequence's units,
         // each by the widest cluster of which enough fit the device at once (8 units: 10 CTAs
-        // each), and joins the parts itself.  Few rows, head_dim 128, 4096 slots: 12.1 us for 8 KV
-        // heads, 10.8 for one, against 13.9 and 17.4 with the list; its CTAs are fewer, though, and
-        // the list is ahead from about 28 key tiles per CTA on (16384 slots, 8 heads: 21.0 and
-        // 21.7 us; 32768: 34.3 and 31.2).  The page table bounds the tiles.
+        // each, 4 or fewer: 16), and joins the parts itself.  One token at head_dim 128, cluster
+        // and list: 1024 slots, 8 KV heads 9.2 and 12.3 us; 4096 slots, 8, 4 and 1 heads 12.0 and
+        // 12.9, 11.1 and 14.0, 10.8 and 13.2; 8192 slots 14.6 and 15.4, 12.6 and 14.1, 12.2 and
+        // 16.9.  Its CTAs are fewer, though, and the list is ahead from about 18 key tiles per
+        // CTA on (16384 slots: 21.0 and 19.7, 16.4 and 16.7, 15.6 and 17.3; 32768: 34.5 and 29.8,
+        // 24.6 and 21.1, 22.3 and 18.6).  The page table bounds the tiles.
         bool joined = false;
         auto launch_cluster = [&](auto cluster, int threads, int smem) {
             constexpr auto kern = decltype(cluster)::value;
@@ -403,7 +405,7 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
             if (ce != cudaSuccess) return ce;
             int size = kMaxCluster;
             while (size > 1 && units > max_clusters<kern>(size, threads, smem)) --size;
-            if (size == 1 || tiles > 28 * size) return cudaSuccess;
+            if (size == 1 || tiles > 18 * size) return cudaSuccess;
             attr[1].id = cudaLaunchAttributeClusterDimension;
             attr[1].val.clusterDim.x = size;
             attr[1].val.clusterDim.y = 1;
