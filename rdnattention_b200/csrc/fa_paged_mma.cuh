@@ -403,7 +403,14 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
             for (int i = first; i < behind; i += 2) {
                 const int sb = i % L::NSB;
                 const uint32_t tS = tmem + lanes + L::S0 + sb * KT;
-                if (!wait(L::S_FULL + sb, i / L::NSB & 1, 0x701)) continue;
+                // the scores, and the reference that the tile before left (the first tile of a segment
+                // has none)
+                if (!aborted) {
+                    const bool here = mbar_wait(bar(L::S_FULL + sb), i / L::NSB & 1, ab, 0x701) &&
+                                      (i == i0 || mbar_wait(bar(L::TOKEN + (w ^ 1) * 4 + quad), (i - 1) / 2 & 1, ab, 0x703));
+                    if (!__all_sync(0xffffffffu, here)) aborted = true;
+                }
+                if (aborted) continue;
                 tc_fence_after();
                 // the first 32 scores stay in registers from the maximum to the exponentials, the last
                 // 32 are read again behind the first exponentials (64 leave the compiler too few
@@ -437,8 +444,6 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
                     hide(y, static_cast<uint32_t>(see >> 32));
                     mx = fmaxf(row_max<32>(x), row_max<32>(y)) * sl2;
                 }
-                // the reference that the tile before left (the first tile of a segment has none)
-                if (i > i0 && !wait(L::TOKEN + (w ^ 1) * 4 + quad, (i - 1) / 2 & 1, 0x703)) continue;
                 const float old = i > i0 ? ref[lr] : -INFINITY;
                 float now = old;
                 const bool grow = fmaxf(old, mx) > old + 8.f;
