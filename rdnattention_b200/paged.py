@@ -14,7 +14,7 @@ captured into a CUDA graph and replayed with new ones.  Extension: the reference
 has no cache.
 
 The cache: ``k_cache`` / ``v_cache`` float16 or bfloat16 [num_pages, kv_heads,
-page_size, head_dim], any page / head / slot strides (a [num_pages, page_size,
+page_size, head_dim], page / head / slot strides positive multiples of 16 bytes (a [num_pages, page_size,
 kv_heads, head_dim] cache is passed as ``.transpose(1, 2)``; a contiguous
 [batch, kv_heads, seq, head_dim] cache has page_size seq and the table
 ``arange(batch)[:, None]``).  page_size is a power of two from 8 up or any size
@@ -187,7 +187,8 @@ def _call(who, device, fn, args):
 def paged_kv_append(key, value, k_cache, v_cache, page_table, cache_lens, new_lens=None, positions=None,
                     rot_cos=None, rot_sin=None):
     """Writes new tokens into a paged cache, in place.  key / value: [batch, kv_heads,
-    tokens, head_dim] of the cache's type (any strides, head_dim contiguous).  Token
+    tokens, head_dim] of the cache's type (head_dim contiguous, the other strides
+    positive multiples of 16 bytes).  Token
     t < new_lens[b] (int32 [batch]; None: all) of sequence b goes to slot
     cache_lens[b] + t, its key turned to positions[b, t] (int32 [batch, tokens];
     None: cache_lens[b] + t) by the float32 [positions, head_dim // 2] tables
@@ -213,7 +214,7 @@ def flash_attn_paged(query, k_cache, v_cache, page_table, cache_lens, new_lens=N
                      rot_cos=None, rot_sin=None, window_size: int = -1, scale=None, out=None):
     """Attention of new tokens over a paged cache that holds them already (slots
     cache_lens[b] + t, see paged_kv_append).  query: [batch, heads, tokens,
-    head_dim] of the cache's type (any strides, head_dim contiguous; heads an exact
+    head_dim] of the cache's type (strides as for paged_kv_append; heads an exact
     multiple of the cache's); rot_cos / rot_sin turn it in the kernel to
     positions[b, t] (None: cache_lens[b] + t).
 
