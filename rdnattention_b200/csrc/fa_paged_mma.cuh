@@ -24,8 +24,8 @@
 // i - 1, rescales O and leaves the new one.
 //
 // Measured (32 / 8 heads, head_dim 128): trees of 64 tokens in 16 ragged contexts of up to
-// 8192, 99 us; 512 tokens of 2 prompts over 16384 slots, 375 to 400 us = 700 to 750 TFLOP/s
-// (half more with the products of lo) at the 1.4 to 1.5 GHz that the power cap leaves.  A tile
+// 8192, 99 to 101 us; 512 tokens of 2 prompts over 16384 slots, 370 us = 755 TFLOP/s (half more
+// with the products of lo) at the 1.4 to 1.5 GHz that the power cap leaves, 440 us in a long run.  A tile
 // takes about 1100 cycles: the two groups' chains from scores to P, 2200 each (waits 300,
 // reading the scores and their maximum 450, reference 150, exponentials to P 1100), of which the
 // exponential unit is busy 1024 for both.  A segment's start and end take about 10000 (lengths,
