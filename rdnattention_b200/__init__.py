@@ -601,19 +601,10 @@ def debug_read_status():
     return int(out[0]), int(out[1])
 
 
-_PAGED = ("paged_kv_append", "flash_attn_paged", "paged_kv_accept", "SUPPORTED_HEAD_DIMS_PAGED")
-
-
-def __getattr__(name):
-    """The paged-cache operators (paged.py), loaded with torch on first use."""
-    if name in _PAGED:
-        from . import paged
-
-        globals().update({n: getattr(paged, n) for n in _PAGED})
-        return globals()[name]
-    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
-
+from .paged import (SUPPORTED_HEAD_DIMS_PAGED, flash_attn_paged, paged_kv_accept,  # noqa: E402 (needs the names above)
+                    paged_kv_append)
 
 __all__ = ["flash_attn", "flash_attn_int8qk", "flash_attn_int8qk_quantized", "quantize_int8_perchannel_v",
            "quantize_int8_qk_pertoken", "quantize_int8_qkv", "has_device", "RDNAttentionError", "SUPPORTED_HEAD_DIMS",
-           "SUPPORTED_HEAD_DIMS_INT8", "__version__", *_PAGED]
+           "SUPPORTED_HEAD_DIMS_INT8", "__version__",
+           "paged_kv_append", "flash_attn_paged", "paged_kv_accept", "SUPPORTED_HEAD_DIMS_PAGED"]

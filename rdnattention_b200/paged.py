@@ -30,21 +30,14 @@ and its attention row is zero.
 import functools
 import struct
 
-import torch
-
 from . import RDNAttentionError, _last_error, _lib_handle
-
-try:  # the stream's handle without a Stream object (2 us less per call)
-    from torch._C import _cuda_getCurrentRawStream as _raw_stream
-except ImportError:
-    def _raw_stream(index):
-        return torch.cuda.current_stream(index).cuda_stream
 
 SUPPORTED_HEAD_DIMS_PAGED = tuple(range(32, 257, 32))
 MAX_TREE_TOKENS = 256
 MAX_ACCEPTED_TOKENS = 256
 
-_DTYPE_CODES = {torch.float16: 0, torch.bfloat16: 1}
+# torch and what depends on it: importing the package needs no torch, the first call loads it
+torch = _raw_stream = _DTYPE_CODES = None
 _HEAD_DIMS = frozenset(SUPPORTED_HEAD_DIMS_PAGED)
 
 # rdna_paged_cache and the argument structs that start with one (include/rdnattention.h).
@@ -54,6 +47,21 @@ _CACHE = "4Q7q6IiI"
 _APPEND = struct.Struct("=" + _CACHE + "6Q6q2I")
 _ATTENTION = struct.Struct("=" + _CACHE + "9Q8q3IifI")
 _ACCEPT = struct.Struct("=" + _CACHE + "2Q2I")
+
+
+def _load_torch():
+    global torch, _raw_stream, _DTYPE_CODES
+    import torch as module
+
+    try:  # the stream's handle without a Stream object (2 us less per call)
+        from torch._C import _cuda_getCurrentRawStream as raw_stream
+    except ImportError:
+        def raw_stream(index):
+            return module.cuda.current_stream(index).cuda_stream
+
+    _raw_stream = raw_stream
+    _DTYPE_CODES = {module.float16: 0, module.bfloat16: 1}
+    torch = module  # last: another thread's call may run as soon as it is set
 
 
 def _tensor(name, t, dtype, device, shape=None):
@@ -194,6 +202,8 @@ def paged_kv_append(key, value, k_cache, v_cache, page_table, cache_lens, new_le
     None: cache_lens[b] + t) by the float32 [positions, head_dim // 2] tables
     rot_cos / rot_sin as interleaved pairs (None: stored as it is).  No two tokens
     may go to the same row.  Returns (k_cache, v_cache)."""
+    if torch is None:
+        _load_torch()
     device, (_, heads, _, head_dim), batch, cache = _cache_args(k_cache, v_cache, page_table, cache_lens)
     tokens, ks = _new_rows("key", key, k_cache, batch, heads, head_dim)
     value_tokens, vs = _new_rows("value", value, k_cache, batch, heads, head_dim)
@@ -232,6 +242,8 @@ def flash_attn_paged(query, k_cache, v_cache, page_table, cache_lens, new_lens=N
     Softmax scale: ``scale``, None for 1/sqrt(head_dim).  Returns ``out`` (or a new
     tensor; it must not share memory with query) shaped like query; rows t >= new_lens[b] and rows that see nothing are
     zero."""
+    if torch is None:
+        _load_torch()
     device, (_, kv_heads, page_size, head_dim), batch, cache = _cache_args(k_cache, v_cache, page_table, cache_lens)
     tokens, qs = _new_rows("query", query, k_cache, batch, 0, head_dim)
     heads = query.shape[1]
@@ -280,6 +292,8 @@ def paged_kv_accept(k_cache, v_cache, page_table, cache_lens, accepted, accepted
     MAX_ACCEPTED_TOKENS; a negative entry, or one behind the page table, moves nothing.
     The drafted slots' pages must belong to one sequence only.  Returns (k_cache,
     v_cache)."""
+    if torch is None:
+        _load_torch()
     device, _, batch, cache = _cache_args(k_cache, v_cache, page_table, cache_lens)
     _tensor("accepted", accepted, torch.int32, device)
     if accepted.dim() != 2 or accepted.shape[0] != batch or not accepted.is_contiguous():
