@@ -360,7 +360,7 @@ RDNA_API int32_t rdna_paged_kv_append(const rdna_paged_append_args* args, void* 
  * holds rdna_attention_paged_workspace_size() bytes.  New tokens below new_lens[b]
  * must hold finite values; slots behind them, and context slots that no token's window
  * reaches, may hold anything.  `output` must not share memory with `query`.  The
- * workspace size is 0 for arguments that the call refuses. */
+ * workspace size is 0 for sizes that the call refuses. */
 typedef struct rdna_paged_attention_args {
     rdna_paged_cache cache;
     const void* query;

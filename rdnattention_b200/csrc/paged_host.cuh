@@ -30,19 +30,26 @@ const char* check_strides(int64_t s0, int64_t s1, int64_t s2, uint64_t n0, uint6
     return nullptr;
 }
 
-const char* check_cache(const PagedCacheParams& c) {
-    if (c.kCache == nullptr || c.vCache == nullptr || c.pageTable == nullptr || c.cacheLens == nullptr)
-        return "null tensor pointer";
-    if (c.dtype != paged::DT_F16 && c.dtype != paged::DT_BF16) return "dtype must be 0 (fp16) or 1 (bf16)";
-    if (c.batchSize == 0 || c.numKvHeads == 0 || c.numPages == 0 || c.maxPages == 0)
+// The sizes that a workspace query knows too.
+const char* check_cache_sizes(const PagedCacheParams& c) {
+    if (c.batchSize == 0 || c.numKvHeads == 0 || c.maxPages == 0)
         return "empty problem (batch_size, num_kv_heads, num_pages and max_pages must be > 0)";
     if (c.headDim < 32 || c.headDim > 256 || c.headDim % 32 != 0)
         return "unsupported head_dim (multiples of 32 from 32 to 256)";
     const bool pow2 = c.pageSize >= 8 && (c.pageSize & (c.pageSize - 1)) == 0;
     if (!pow2 && c.pageSize < 64) return "unsupported page_size (a power of two from 8 up, or any size from 64 up)";
     if (static_cast<uint64_t>(c.maxPages) * c.pageSize > (1u << 30)) return "max_pages * page_size exceeds 2^30";
-    if (c.numPages > INT32_MAX) return "too many pages";
     if (c.numKvHeads > 65535 || c.batchSize > (1u << 24)) return "too many heads or sequences";
+    return nullptr;
+}
+
+const char* check_cache(const PagedCacheParams& c) {
+    if (c.kCache == nullptr || c.vCache == nullptr || c.pageTable == nullptr || c.cacheLens == nullptr)
+        return "null tensor pointer";
+    if (c.dtype != paged::DT_F16 && c.dtype != paged::DT_BF16) return "dtype must be 0 (fp16) or 1 (bf16)";
+    if (c.numPages == 0) return "empty problem (batch_size, num_kv_heads, num_pages and max_pages must be > 0)";
+    if (const char* e = check_cache_sizes(c)) return e;
+    if (c.numPages > INT32_MAX) return "too many pages";
     if (!p16(c.kCache) || !p16(c.vCache)) return "cache base pointers must be 16-byte aligned";
     if (!p4(c.pageTable) || !p4(c.cacheLens)) return "page_table and cache_lens must be 4-byte aligned";
     if (c.batchSize > 1 && c.tableStride < 0) return "strides must be positive";
@@ -170,27 +177,52 @@ int launched() {
 struct PagedPlan {
     int dp;     // head_dim rounded up to the kernel's 64, 128 or 256
     bool mma;   // the tcgen05 kernel's row tiles of 128
-    int RT, n_rt, tpp, grid;
+    int RT, n_rt, tpp, grid, W;
+    int64_t tiles;  // key tiles of a full page table
+    int64_t step;   // sequences per launch; 0: the problem is too large
     size_t partials, bytes;  // workspace: bytes of the partials, in all
 };
 
 // Rows of a KV head within the kernels' 32 bits (either factor may be any 32-bit number).
 bool rows_fit(uint32_t H, uint32_t Hkv, uint32_t T) { return H / Hkv <= (uint32_t(1) << 28) / std::max(T, 1u); }
 
-PagedPlan paged_plan(uint32_t B, uint32_t H, uint32_t Hkv, uint32_t T, uint32_t D, uint32_t P) {
+PagedPlan paged_plan(const PagedAttentionParams& a) {
+    const PagedCacheParams& c = a.c;
     PagedPlan f{};
-    f.dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
-    const int64_t rows = static_cast<int64_t>(H / Hkv) * T;
+    f.dp = c.headDim <= 64 ? 64 : c.headDim <= 128 ? 128 : 256;
+    const int64_t rows = static_cast<int64_t>(a.numHeads / c.numKvHeads) * a.seqLen;
     f.mma = f.dp <= 128 && rows > 16;
     f.RT = f.mma ? 128 : f.dp <= 128 || rows <= 16 ? 16 : 32;
     f.n_rt = static_cast<int>((rows + f.RT - 1) / f.RT);
-    f.tpp = static_cast<int>(P) >= paged::KT ? (static_cast<int>(P) + paged::KT - 1) / paged::KT : 0;
+    const int64_t P = c.pageSize;
+    f.tpp = P >= paged::KT ? static_cast<int>((P + paged::KT - 1) / paged::KT) : 0;
+    f.tiles = f.tpp == 0 ? (c.maxPages * P + paged::KT - 1) / paged::KT : static_cast<int64_t>(c.maxPages) * f.tpp;
     f.grid = sm_count();
-    f.partials = align_up(static_cast<size_t>(2) * f.grid * f.RT * (D + 2) * sizeof(float));
-    // units of a launch: at most kMaxList (sequence, row tile) pairs
-    const int64_t seqs = std::max<int64_t>(1, std::min<int64_t>(B, paged::kMaxList / f.n_rt));
-    f.bytes = f.partials + align_up(static_cast<size_t>(seqs) * Hkv * f.n_rt * sizeof(int2));
+    f.W = f.mma ? paged::kLeadMma : paged::kLead;
+    // units of a launch: at most kMaxList (sequence, row tile) pairs, and list positions of 32
+    // bits (n_rt <= 2^11, so none of these products passes 64 bits)
+    if (f.n_rt > paged::kMaxList) return f;
+    const int64_t per_seq = (f.tiles + f.W) * f.n_rt * c.numKvHeads;
+    const int64_t join_blocks =
+        static_cast<int64_t>(c.numKvHeads) * f.n_rt * ((f.RT + paged::kJoinRows - 1) / paged::kJoinRows);
+    f.step = std::min<int64_t>(INT32_MAX / std::max(per_seq, join_blocks), paged::kMaxList / f.n_rt);
+    f.partials = align_up(static_cast<size_t>(2) * f.grid * f.RT * (c.headDim + 2) * sizeof(float));
+    const int64_t seqs = std::min<int64_t>(c.batchSize, f.step);
+    f.bytes = f.partials + align_up(static_cast<size_t>(seqs) * c.numKvHeads * f.n_rt * sizeof(int2));
     return f;
+}
+
+// The plan of a call, and which sizes no call takes: for the call and the workspace query alike.
+// (Nothing is planned for seqLen 0.)
+const char* plan_attention(const PagedAttentionParams& a, PagedPlan& f) {
+    f = PagedPlan{};
+    if (const char* e = check_cache_sizes(a.c)) return e;
+    if (a.numHeads == 0 || a.numHeads % a.c.numKvHeads != 0)
+        return "numHeads must be a positive multiple of numKvHeads";
+    if (a.seqLen == 0) return nullptr;
+    if (!rows_fit(a.numHeads, a.c.numKvHeads, a.seqLen)) return "sequence too long";
+    f = paged_plan(a);
+    return f.step == 0 ? "problem too large for one launch" : nullptr;
 }
 
 }  // namespace
@@ -266,23 +298,19 @@ int pagedAccept(const PagedAcceptParams& a, void* stream) {
 }
 
 size_t pagedAttentionWorkspaceBytes(const PagedAttentionParams& a) {
-    if (a.c.numKvHeads == 0 || a.numHeads == 0 || a.numHeads % a.c.numKvHeads != 0 || a.c.headDim == 0 ||
-        a.c.headDim > 256 || a.seqLen == 0 || a.c.pageSize == 0 || a.c.numKvHeads > 65535 ||
-        !rows_fit(a.numHeads, a.c.numKvHeads, a.seqLen))
-        return 0;
-    return paged_plan(a.c.batchSize, a.numHeads, a.c.numKvHeads, a.seqLen, a.c.headDim, a.c.pageSize).bytes;
+    PagedPlan f;
+    return plan_attention(a, f) != nullptr ? 0 : f.bytes;
 }
 
 int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t workspace_bytes, void* stream) {
     const PagedCacheParams& c = a.c;
     if (const char* e = check_cache(c)) return pfail(e);
     if (a.q == nullptr || a.o == nullptr) return pfail("null tensor pointer");
-    if (a.numHeads == 0 || a.numHeads % c.numKvHeads != 0)
-        return pfail("numHeads must be a positive multiple of numKvHeads");
+    PagedPlan f;
+    if (const char* e = plan_attention(a, f)) return pfail(e);
     if (a.seqLen == 0) return 0;
     if (a.treeMask != nullptr && a.seqLen > static_cast<uint32_t>(paged::kMaxTree))
         return pfail("tree_mask: more than 256 tokens");
-    if (!rows_fit(a.numHeads, c.numKvHeads, a.seqLen)) return pfail("sequence too long");
     if (!p16(a.q) || !p16(a.o)) return pfail("tensor base pointers must be 16-byte aligned");
     if (!p4(a.newLens)) return pfail("new_lens must be 4-byte aligned");
     if (const char* e = check_strides(a.qStrideB, a.qStrideH, a.qStrideS, c.batchSize, a.numHeads, a.seqLen))
@@ -292,7 +320,6 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
     if (a.treeMask != nullptr && (a.maskStrideB < 0 || a.maskStrideT < 0)) return pfail("strides must be positive");
     if (const char* e = check_rope(a.rotCos, a.rotSin, a.positions, a.ropeRows)) return pfail(e);
 
-    const PagedPlan f = paged_plan(c.batchSize, a.numHeads, c.numKvHeads, a.seqLen, c.headDim, c.pageSize);
     if (workspace == nullptr || workspace_bytes < f.bytes)
         return pfail("workspace missing or smaller than rdna_attention_paged_workspace_size()");
     if (reinterpret_cast<uintptr_t>(workspace) & (kWsAlign - 1)) return pfail("workspace must be 256-byte aligned");
@@ -333,18 +360,7 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
     p.ws = static_cast<float*>(workspace);
     p.units = reinterpret_cast<int2*>(static_cast<char*>(workspace) + f.partials);
     p.grid = f.grid;
-    p.W = f.mma ? paged::kLeadMma : paged::kLead;
-
-    // the list positions of one launch are 32-bit (n_rt <= 2^11, so none of these products
-    // passes 64 bits): as many sequences per launch as surely fit
-    if (p.n_rt > paged::kMaxList) return pfail("problem too large for one launch");
-    const int64_t tiles = f.tpp == 0 ? (static_cast<int64_t>(c.maxPages) * c.pageSize + paged::KT - 1) / paged::KT
-                                     : static_cast<int64_t>(c.maxPages) * f.tpp;
-    const int64_t per_seq = (tiles + p.W) * p.n_rt * p.Hkv;
-    const int64_t join_blocks = static_cast<int64_t>(p.Hkv) * p.n_rt * ((f.RT + paged::kJoinRows - 1) / paged::kJoinRows);
-    const int64_t fit = INT32_MAX / (per_seq > join_blocks ? per_seq : join_blocks);
-    const int64_t step = std::min<int64_t>(fit, paged::kMaxList / p.n_rt);
-    if (step == 0) return pfail("problem too large for one launch");
+    p.W = f.W;
 
     CUtensorMap tmK, tmV;
     const uint32_t box_rows = std::min<uint32_t>(c.pageSize, paged::KT);
@@ -358,9 +374,9 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
         return pfail(e);
 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    for (int64_t b0 = 0; b0 < c.batchSize; b0 += step) {
+    for (int64_t b0 = 0; b0 < c.batchSize; b0 += f.step) {
         paged::AttnParams s = p;
-        s.B = static_cast<int>(c.batchSize - b0 < step ? c.batchSize - b0 : step);
+        s.B = static_cast<int>(std::min<int64_t>(c.batchSize - b0, f.step));
         s.by_B.set(static_cast<uint32_t>(s.B));
         s.q += b0 * p.qsb;
         s.o += b0 * p.osb;
@@ -405,7 +421,7 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
             if (ce != cudaSuccess) return ce;
             int size = kMaxCluster;
             while (size > 1 && units > max_clusters<kern>(size, threads, smem)) --size;
-            if (size == 1 || tiles > 18 * size) return cudaSuccess;
+            if (size == 1 || f.tiles > 18 * size) return cudaSuccess;
             attr[1].id = cudaLaunchAttributeClusterDimension;
             attr[1].val.clusterDim.x = size;
             attr[1].val.clusterDim.y = 1;
