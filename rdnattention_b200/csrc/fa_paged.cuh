@@ -434,8 +434,9 @@ __device__ __forceinline__ float4 ld_dsmem4(uint32_t addr) {
 }
 
 // Joins the cluster's parts (at `part` in each CTA's shared memory: O [D / 4][RT] float4,
-// m [RT], l [RT]; a CTA without tiles has m = -inf) and writes the rows out; every thread of
-// every CTA takes part.
+// m [RT], l [RT]) and writes the rows out; every thread of every CTA takes part.  A part that
+// adds nothing has m = -inf and l = 0, and no O if its CTA had no tiles; scores that were all NaN
+// leave m at -inf too, but a sum of NaN.
 template <class E>
 __device__ __forceinline__ void cluster_join(const AttnParams& p, const float* part, int tid, int nthreads) {
     decode::cluster_sync_all();
@@ -453,6 +454,7 @@ __device__ __forceinline__ void cluster_join(const AttnParams& p, const float* p
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 m[k] = -INFINITY;
+                li[k] = 0.f;
                 if (k0 + k < size) {
                     const uint32_t a = decode::map_to_rank(base, k0 + k);
                     m[k] = decode::ld_dsmem(a + 4 * (p.RT * p.D + lr));
@@ -472,8 +474,8 @@ __device__ __forceinline__ void cluster_join(const AttnParams& p, const float* p
             o.w *= g;
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-                if (m[k] != -INFINITY) {
-                    const float f = ex2(m[k] - mx);
+                if (m[k] != -INFINITY || li[k] != 0.f) {
+                    const float f = m[k] == -INFINITY ? 0.f : ex2(m[k] - mx);
                     l += f * li[k];
                     o.x += f * x[k].x;
                     o.y += f * x[k].y;
@@ -812,8 +814,12 @@ __global__ void __launch_bounds__(Layout<DP>::THREADS, 1) fa_paged_kernel(
         const Segment g = CLUSTER ? cluster_segment(p) : segment_at(p, pre, pos, end, e);
         pos = g.next;
         if (g.count == 0) {
-            // (in a cluster: a part without weight)
-            if (CLUSTER && threadIdx.x < p.RT) reinterpret_cast<float*>(ring)[p.RT * p.D + threadIdx.x] = -INFINITY;
+            // (in a cluster: a part that adds nothing)
+            if (CLUSTER && threadIdx.x < p.RT) {
+                float* ml = reinterpret_cast<float*>(ring) + p.RT * p.D;
+                ml[threadIdx.x] = -INFINITY;
+                ml[p.RT + threadIdx.x] = 0.f;
+            }
             continue;
         }
         const int row0 = g.rt * p.RT, ta = p.by_G.div(row0);

@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
                     tmem_ld_x16(tO + c0, raw);
                     float* o = reinterpret_cast<float*>(raw);
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) o[k] = M == -INFINITY ? 0.f : o[k] * inv;
+                    for (int k = 0; k < 16; ++k) o[k] = lsum == 0.f ? 0.f : o[k] * inv;
                     if (whole) {
 #pragma unroll
                         for (int k = 0; k < 2; ++k)
