@@ -33,6 +33,12 @@ struct F16 {
         return __half22float2(*reinterpret_cast<const __half2*>(&v));
     }
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_half2(lo, hi); }
+    // Values beyond the type's largest become that instead of an infinity.
+    static __device__ __forceinline__ uint32_t pack_finite(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
 };
 struct BF16 {
     static __device__ __forceinline__ float2 unpack(uint32_t v) {
@@ -41,6 +47,11 @@ struct BF16 {
     static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
         uint32_t r;
         asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+        return r;
+    }
+    static __device__ __forceinline__ uint32_t pack_finite(float lo, float hi) {
+        uint32_t r;
+        asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
         return r;
     }
 };
@@ -53,12 +64,14 @@ __device__ __forceinline__ uint32_t rotate_pair(uint32_t v, float c, float s) {
     return E::pack(__fmaf_rn(x.x, c, -__fmul_rn(x.y, s)), __fmaf_rn(x.x, s, __fmul_rn(x.y, c)));
 }
 
-// The same, as hi + lo: the rounded pair and what the rounding left, rounded again.
+// The same, as hi + lo: the rounded pair and what the rounding left, rounded again.  A turn can
+// leave fp16's range by a factor of sqrt 2: hi is the largest value then, and lo holds the rest
+// (an infinity or NaN stays one, in lo).
 template <class E>
 __device__ __forceinline__ void turn_split(uint32_t& hi, uint32_t& lo, float c, float s) {
     const float2 x = E::unpack(hi);
     const float a = __fmaf_rn(x.x, c, -__fmul_rn(x.y, s)), b = __fmaf_rn(x.x, s, __fmul_rn(x.y, c));
-    hi = E::pack(a, b);
+    hi = E::pack_finite(a, b);
     const float2 h = E::unpack(hi);
     lo = E::pack(a - h.x, b - h.y);
 }

@@ -1,11 +1,12 @@
 """Values that are not finite, or hardly: NaN and infinities in the query and in keys that are seen
-reach the rows that see them, whatever the kernel and the cut of its work, and no other row."""
+reach the rows that see them, whatever the kernel and the cut of its work, and no other row; turned
+queries beyond fp16's range."""
 import pytest
 import torch
 
 import paged_bounds as PB
 from paged_bounds import BF16, F16
-from test_gpu_paged_bounds import attend
+from test_gpu_paged_bounds import attend, check
 
 pytestmark = pytest.mark.gpu
 
@@ -87,3 +88,18 @@ def test_padding_rows_stay_zero_beside_nan(kw):
         if T > 2:
             assert (got[b, :, 1] == 0).all()
     assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("kw", [kw for _, kw in PLANS if kw["dtype"] == F16], ids=[n for n, kw in PLANS if kw["dtype"] == F16])
+def test_turned_queries_beyond_fp16(kw):
+    """Pairs of 6e4 turned by an eighth of a circle reach 8.5e4, beyond fp16's 65504: the turned query
+    is not rounded to fp16, so the scores (times keys of 1e-3) and the output are ordinary."""
+    case = PB.plain_case(**{**kw, "kind": "chain"})
+    cos, sin = PB.O.tables(1, kw["D"])
+    case.update(cos=cos.expand(2, -1).contiguous(), sin=sin.expand(2, -1).contiguous(),
+                positions=torch.ones(len(kw["lens"]), kw["T"], dtype=torch.int32))
+    case["cos"][1], case["sin"][1] = 0.5 ** 0.5, 0.5 ** 0.5
+    case["q"][..., :2] = torch.tensor([6e4, 6e4])
+    case["q"][..., 2:4] = torch.tensor([6e4, -6e4])
+    case["k_cache"][..., :4] *= 2.0 ** -10
+    check(case)
