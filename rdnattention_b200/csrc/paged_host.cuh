@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <limits>
 #include <type_traits>
 
 namespace rdna {
@@ -353,9 +354,9 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
     p.by_P.set(c.pageSize);
     p.by_tpp.set(f.tpp == 0 ? 1 : static_cast<uint32_t>(f.tpp));
     p.window = a.windowSize > 0 ? a.windowSize : 0;
-    // (a scale of 0 becomes one whose scores are 0 in fp32)
-    p.scale_log2 = std::fabs(a.scale) * 1.4426950408889634f;
-    if (p.scale_log2 < 1e-30f) p.scale_log2 = 1e-30f;
+    // (never 0, which times a masked score of -inf would be NaN: a scale of 0 becomes the smallest
+    // normal number, and products of up to 1e30 give scores below 2e-8, which no weight shows)
+    p.scale_log2 = std::max(std::fabs(a.scale) * 1.4426950408889634f, std::numeric_limits<float>::min());
     p.flip = a.scale < 0.f ? 0x80008000u : 0u;
     p.ws = static_cast<float*>(workspace);
     p.units = reinterpret_cast<int2*>(static_cast<char*>(workspace) + f.partials);

@@ -1,6 +1,6 @@
 """Values that are not finite, or hardly: NaN and infinities in the query and in keys that are seen
 reach the rows that see them, whatever the kernel and the cut of its work, and no other row; turned
-queries beyond fp16's range."""
+queries beyond fp16's range; a scale of zero."""
 import pytest
 import torch
 
@@ -102,4 +102,13 @@ def test_turned_queries_beyond_fp16(kw):
     case["q"][..., :2] = torch.tensor([6e4, 6e4])
     case["q"][..., 2:4] = torch.tensor([6e4, -6e4])
     case["k_cache"][..., :4] *= 2.0 ** -10
+    check(case)
+
+
+@pytest.mark.parametrize("kw", [kw for _, kw in PLANS if kw["dtype"] == BF16], ids=[n for n, kw in PLANS if kw["dtype"] == BF16])
+def test_scale_of_zero(kw):
+    """Products of 1e30 to 1e32 times nothing: every visible slot weighs the same."""
+    case = PB.plain_case(scale=0.0, rope=False, **kw)
+    case["q"] *= 1e15
+    case["k_cache"] *= 1e15
     check(case)
