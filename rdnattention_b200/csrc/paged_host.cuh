@@ -56,8 +56,8 @@ const char* check_cache(const PagedCacheParams& c) {
     if (c.batchSize > 1 && c.tableStride < 0) return "strides must be positive";
     if (const char* e = check_strides(c.kcStrideP, c.kcStrideH, c.kcStrideS, c.numPages, c.numKvHeads, c.pageSize))
         return e;
-    // the kernels hold the page and slot strides as 32 bits of bytes
-    for (int64_t s : {c.kcStrideP, c.kcStrideS, c.vcStrideP, c.vcStrideS})
+    // the kernels hold the page and slot strides as 32 bits of bytes (one page has no stride)
+    for (int64_t s : {c.kcStrideS, c.vcStrideS, c.numPages > 1 ? c.kcStrideP : 0, c.numPages > 1 ? c.vcStrideP : 0})
         if (s >= (int64_t(1) << 31)) return "cache page or slot stride too large";
     return check_strides(c.vcStrideP, c.vcStrideH, c.vcStrideS, c.numPages, c.numKvHeads, c.pageSize);
 }

@@ -14,11 +14,12 @@ captured into a CUDA graph and replayed with new ones.  Extension: the reference
 has no cache.
 
 The cache: ``k_cache`` / ``v_cache`` float16 or bfloat16 [num_pages, kv_heads,
-page_size, head_dim], page / head / slot strides positive multiples of 16 bytes (a [num_pages, page_size,
-kv_heads, head_dim] cache is passed as ``.transpose(1, 2)``; a contiguous
-[batch, kv_heads, seq, head_dim] cache has page_size seq and the table
-``arange(batch)[:, None]``).  page_size is a power of two from 8 up or any size
-from 64 up, head_dim one of SUPPORTED_HEAD_DIMS_PAGED.  ``page_table`` int32
+page_size, head_dim], page / head / slot strides positive multiples of 16 bytes,
+page and slot strides below 2**31 elements (a [num_pages, page_size, kv_heads,
+head_dim] cache is passed as ``.transpose(1, 2)``; a contiguous [batch, kv_heads,
+seq, head_dim] cache has page_size seq and the table ``arange(batch)[:, None]``).
+page_size is a power of two from 8 up or any size from 64 up, head_dim one of
+SUPPORTED_HEAD_DIMS_PAGED.  ``page_table`` int32
 [batch, max_pages] and ``cache_lens`` int32 [batch]: slot s of sequence b is row
 s % page_size of page page_table[b, s // page_size].  Keys are stored rotated.
 
