@@ -545,6 +545,7 @@ __device__ __forceinline__ uint32_t chunk_off(int rows, int r, int c) {
     return static_cast<uint32_t>((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
+// (With a memory clobber, unlike the dense decode kernel's: here the tile is also written by its reader.)
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -561,11 +562,7 @@ template <class E>
 __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
 template <>
 __device__ __forceinline__ void mma16816<F16>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    decode::mma16816(c, a, b0, b1);
 }
 template <>
 __device__ __forceinline__ void mma16816<BF16>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {

@@ -493,7 +493,6 @@ __global__ void __launch_bounds__(MmaLayout<DP>::THREADS, 1) fa_paged_mma_kernel
                         }
                         tmem_st_x8(tS + c0 / 2, pk);  // (over scores that have been read)
                     };
-#pragma unroll
                     exponentials(x, 0);
                     tmem_ld_x32_begin(tS + 32, last);
                     exponentials(x + 16, 16);

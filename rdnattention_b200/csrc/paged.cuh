@@ -18,6 +18,7 @@
 
 #include <cstdint>
 
+#include "rope.cuh"
 #include "sm100.cuh"
 
 namespace rdna {
@@ -57,11 +58,15 @@ struct BF16 {
 };
 
 // One interleaved pair turned by its angle, fp32 math with explicit roundings
-// (the same bits in every kernel), rounded once to the element type.
+// (the same bits in every kernel, the dense ones' function in fp16), rounded once to the element type.
 template <class E>
 __device__ __forceinline__ uint32_t rotate_pair(uint32_t v, float c, float s) {
     const float2 x = E::unpack(v);
     return E::pack(__fmaf_rn(x.x, c, -__fmul_rn(x.y, s)), __fmaf_rn(x.x, s, __fmul_rn(x.y, c)));
+}
+template <>
+__device__ __forceinline__ uint32_t rotate_pair<F16>(uint32_t v, float c, float s) {
+    return rope::rotate_pair(v, c, s);
 }
 
 // The same, as hi + lo: the rounded pair and what the rounding left, rounded again.  A turn can
