@@ -504,9 +504,10 @@ __device__ __forceinline__ void cluster_join(const AttnParams& p, const float* p
 // scores are as exact as an fp32 product.
 //
 // Measured (head_dim 128): 64 sequences of 32768 slots, 8 KV heads of 8 query heads:
-// 1.253 ms, 6.86 TB/s, 1.05 of the measured copy rate.  33 ragged sequences of up to 8192
-// slots, 32 / 8 heads, pages of 16: 105 to 114 us, 0.74 to 0.8 of the copy rate (what is
-// missing are the segments' starts, four or five per CTA, and the join).
+// 1.24 ms = 6.9 TB/s replayed on one input, 1.34 ms = 6.4 TB/s called over changing ones, 1.06 and
+// 0.98 of the measured copy rate.  33 ragged sequences of up to 8192 slots, 32 / 8 heads, pages
+// of 16: 106 to 111 us, 0.76 to 0.79 of the copy rate (what is missing are the segments' starts,
+// four or five per CTA, and the join).
 template <int DP>
 struct Layout {
     static constexpr int NCW = DP <= 128 ? 8 : 4;
@@ -670,9 +671,9 @@ __device__ __forceinline__ bool produce(const AttnParams& p, const CUtensorMap* 
                                         const Segment& g, int i, uint32_t bars, uint32_t ring, uint32_t& filled,
                                         int& issued, const Abort& ab, int lane) {
     // Keys that four or more row tiles read stay in L2 if they can; with fewer, what one CTA has
-    // read is soon read by another or never again (32 / 8 heads, kept and evicted first: 512 tokens of
-    // 2 prompts over 16384 slots 411 and 448 us, 128 tokens 101 and 108, 96 tokens 84 and 83; ragged
-    // trees of 64 tokens in 16 contexts 117 and 111).
+    // read is soon read by another or never again (32 / 8 heads, sustained, kept and evicted first: 512
+    // tokens of 2 prompts over 16384 slots 437 and 479 us, 128 tokens 101 and 108, 96 tokens 84 and
+    // 83; ragged trees of 64 tokens in 16 contexts 117 and 111).
     const uint64_t pol = p.n_rt >= 4 ? policy_evict_last() : policy_evict_first();
     const int ppt = uniform(p.tpp == 0 ? KT >> p.t.Pshift : 1), box = min(p.t.P, KT) * 128;  // pages per tile
     const int* pages = p.t.pages + g.b * p.t.stride;

@@ -1,10 +1,11 @@
 // The many-rows kernel of the paged attention: row tiles of 128 on tcgen05.
 //
 // Trees of drafted tokens and chunks of prompts bring 17 to thousands of rows per KV
-// head.  Per 64-key tile of head_dim 128 an SM receives 32 KB (about 1340 cycles of
-// its share of the HBM bandwidth), and 128 rows need 8192 exponentials (512 cycles)
-// and three products of 128 cycles, so a tile of rows is HBM-bound as long as the
-// softmax keeps up; more row tiles read the same keys again, mostly from L2.
+// head.  Per 64-key tile of head_dim 128 an SM receives 32 KB (about 1400 cycles of
+// its share of the HBM bandwidth at 1.9 GHz), and 128 rows need 8192 exponentials (512
+// cycles) and three products of 256 cycles (Q K^T for hi and for lo, P V), so one row
+// tile per KV head is HBM-bound if the tensor pipe and the softmax overlap; more row
+// tiles read the same keys again, partly from L2, and are bound on the SM.
 //
 //   warps 0..3, 4..7   two softmax groups (thread = row = TMEM lane); key tile i of
 //                      the CTA goes to group i & 1
@@ -24,13 +25,14 @@
 // i - 1, rescales O and leaves the new one.
 //
 // Measured (32 / 8 heads, head_dim 128): trees of 64 tokens in 16 ragged contexts of up to
-// 8192, 99 to 101 us; 512 tokens of 2 prompts over 16384 slots, 370 us = 755 TFLOP/s (half more
-// with the products of lo) at the 1.4 to 1.5 GHz that the power cap leaves, 440 us in a long run.  A tile
-// takes about 1100 cycles: the two groups' chains from scores to P, 2200 each (waits 300,
-// reading the scores and their maximum 450, reference 150, exponentials to P 1100), of which the
-// exponential unit is busy 1024 for both.  A segment's start and end take about 10000 (lengths,
-// positions, Q and the tables in turn; then O), which is why units lead the list by kLeadMma
-// positions.
+// 8192, 100 to 105 us; 512 tokens of 2 prompts over 16384 slots, 353 to 371 us = 750 to 790
+// TFLOP/s (half more with the products of lo) in short runs at 1.5 GHz, 437 us sustained at the
+// 1.2 to 1.3 GHz that the power cap leaves.  There a tile takes about 1100 cycles, of which the
+// tensor pipe is busy 768 (70 %) and the exponential unit 512 (48 %): the two groups' chains from
+// scores to P take 2200 each (waits 300, reading the scores and their maximum 450, reference 150,
+// exponentials to P 1100), and the products of a tile wait for them in turn.  A segment's start
+// and end take about 10000 (lengths, positions, Q and the tables in turn; then O), which is why
+// units lead the list by kLeadMma positions.
 #pragma once
 
 #include "fa_paged.cuh"

@@ -152,11 +152,13 @@ struct AppendParams {
     int64_t n;  // B * Hkv * T * (D / 8) 16-byte chunks
 };
 
-// One 16-byte chunk of K and of V per thread: load, turn K, store.  Nothing is
-// read twice; the chunk index runs fastest, then the token, so that both sides
-// of the copy are contiguous within a page.  Bound by HBM: 4 prompts of 4096
-// tokens, 8 heads of 128, 24.7 us = 0.88 of the measured copy rate; small calls by
-// the latency of the length, page and row reads (2.2 us for one token).
+// One 16-byte chunk of K and of V per thread: load, turn K, store.  K and V are
+// read once; the rows of the tables and the page entries are read again for every
+// head and sequence, from L2.  The chunk index runs fastest, then the token, so that
+// both sides of the copy are contiguous within a page.  Bound by HBM: 4 prompts of 4096
+// tokens, 8 heads of 128 (134 MB of rows and 2 MB of tables), 27.5 us over changing
+// inputs = 0.76 of the measured copy rate, 25.2 us = 0.83 over the same; small calls by
+// the latency of the length, page and row reads (2.4 us for one token).
 template <class E>
 __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendParams p) {
     const int nch = p.D / 8;

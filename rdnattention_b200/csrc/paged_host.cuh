@@ -412,7 +412,8 @@ int pagedAttention(const PagedAttentionParams& a, void* workspace, size_t worksp
         // 12.9, 11.1 and 14.0, 10.8 and 13.2; 8192 slots 14.6 and 15.4, 12.6 and 14.1, 12.2 and
         // 16.9.  Its CTAs are fewer, though, and the list is ahead from about 18 key tiles per
         // CTA on (16384 slots: 21.0 and 19.7, 16.4 and 16.7, 15.6 and 17.3; 32768: 34.5 and 29.8,
-        // 24.6 and 21.1, 22.3 and 18.6).  The page table bounds the tiles.
+        // 24.6 and 21.1, 22.3 and 18.6).  The lengths are on the device, so the width of the page
+        // table bounds the tiles: a short sequence in a wide table takes the list.
         bool joined = false;
         auto launch_cluster = [&](auto cluster, int threads, int smem) {
             constexpr auto kern = decltype(cluster)::value;

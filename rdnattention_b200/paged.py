@@ -22,6 +22,9 @@ page_size is a power of two from 8 up or any size from 64 up, head_dim one of
 SUPPORTED_HEAD_DIMS_PAGED.  ``page_table`` int32
 [batch, max_pages] and ``cache_lens`` int32 [batch]: slot s of sequence b is row
 s % page_size of page page_table[b, s // page_size].  Keys are stored rotated.
+A single sequence is attended to faster through a table no wider than it needs
+(up to 11000 slots with 8 kv_heads, 18000 with 4 or fewer), ``page_table[:, :n]``: the host, which chooses between
+two forms, knows the table's width and not the length.
 
 These values are not known to the host, so the kernels check them: lengths are
 clamped to the table's capacity; a page outside the cache is not written and reads
@@ -235,7 +238,9 @@ def flash_attn_paged(query, k_cache, v_cache, page_table, cache_lens, new_lens=N
     token t sees every slot below cache_lens[b] and the drafted tokens u <
     new_lens[b] with mask[b, t, u] (itself only if the mask says so).  window_size >
     0: a token sees only the newest window_size of these; its drafted tokens count
-    first, in index order (parents before children).  Drafted tokens below
+    first, in index order (parents before children).  (Tokens are counted, positions are
+    not compared: for masks of a token and its ancestors at positions cache_lens[b] +
+    depth both are the same.)  Drafted tokens below
     new_lens[b] must hold finite values; slots behind them, and context slots that no
     token's window reaches, may hold anything.  At most 262144 rows (tokens * heads /
     kv_heads) per sequence, 65536 above head_dim 128.
