@@ -297,9 +297,9 @@ RDNA_API int32_t rdna_peer_barrier(int32_t world, int32_t rank, void* const* pee
  *
  * k_cache / v_cache: [num_pages, num_kv_heads, page_size, head_dim], head_dim
  * contiguous, strides in elements (16-byte multiples; page and slot below 2^31) for
- * the page / head / slot axes.  page_size: a power of two from 8 up, or any size from 64 up.  head_dim:
- * a multiple of 32 up to 256.  page_table: int32 [batch, max_pages], rows
- * `table_stride` entries apart; cache_lens: int32 [batch], the slots in use before
+ * the page / head / slot axes.  page_size: a power of two from 8 up, or any size
+ * from 64 up.  head_dim: a multiple of 32 up to 256.  page_table: int32 [batch,
+ * max_pages], rows `table_stride` entries apart; cache_lens: int32 [batch], the slots in use before
  * the call's new tokens.  Slot s of sequence b is row s % page_size of page
  * page_table[b][s / page_size]; max_pages * page_size must not exceed 2^30.
  *
