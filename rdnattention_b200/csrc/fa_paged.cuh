@@ -36,7 +36,7 @@ constexpr int kMaxList = 2048;         // sequences x row tiles per launch (the 
 constexpr int KT = 64;                 // keys per tile
 // AttnParams::W of the two kernels: about the tiles' worth of time that a segment's start and
 // end take (ragged batch of 33: 157 us at 0, 112 at 4, 105 at 6, 107 at 8; trees of 64 tokens
-// in 16 contexts: 104 us at 8, 102 at 12, 101 at 16).
+// in 16 contexts: 104 us at 8, 102 at 12, 101 at 16; all at head_dim 128, other widths take the same).
 constexpr int kLead = 6, kLeadMma = 12;
 
 // n / d for n < 2^31 by a multiplication: with l = ceil(log2 d) and m =
